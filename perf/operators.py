@@ -1,0 +1,474 @@
+"""The operators of a KV cache held in 8 bits, measured call by call.
+
+Three kinds of case, each one public entry point of include/q3t_ops.h:
+
+  tables   block tables, positions and slot maps of a batch, built on the GPU from the requests' lengths, pages taken from and
+           given back to a pool (q3t_launch_page_tables)
+  append   keys and values of new tokens quantised into pages of 16 tokens, one scale for each page, head and plane
+           (q3t_launch_kv8_append)
+  attend   causal attention of new tokens over such a cache: one token a row (decode), a few (drafts to be verified), or a
+           whole prompt or a chunk of one (q3t_launch_kv8_attention)
+
+Every state is made from the seed alone.  Keys and values lie in packed projections, as a decoder layer leaves them; pages lie
+anywhere in a pool that has more of them than the batch needs.
+"""
+import ctypes as C
+import importlib
+import math
+
+import torch
+
+own = False
+
+PAGE = 16                      # tokens of a page
+SMALLEST = 2.0 ** -126         # of the scales
+MOST = {"int8": 127.0, "e4m3": 448.0}
+Q_HEADS, KV_HEADS, HEAD_DIM = 16, 8, 128
+
+
+def listed():
+    return [
+        # one step of a full lockstep batch: a token for each of 64 sessions
+        {"name": "tables_decode_64", "kind": "tables", "rows": 64, "shortest": 64, "longest": 2048, "prompt": 0, "stride": 512},
+        # a large server's step: most requests decode, every eighth one comes with a prompt or leaves
+        {"name": "tables_mixed_1000", "kind": "tables", "rows": 1000, "shortest": 1, "longest": 7000, "prompt": 1500, "stride": 1024},
+        # the keys and values of a decode step of 64 sessions, one layer
+        {"name": "append_decode_64", "kind": "append", "format": "int8", "rows": 64, "shortest": 64, "longest": 2048, "new": 1,
+         "heads": KV_HEADS, "dim": HEAD_DIM},
+        # a long passage on top of a cached voice description that ends inside a page
+        {"name": "append_prompt_1500", "kind": "append", "format": "e4m3", "rows": 1, "shortest": 707, "longest": 707, "new": 1500,
+         "heads": KV_HEADS, "dim": HEAD_DIM},
+        # 43 prompts at once: the largest append
+        {"name": "append_batch_65k", "kind": "append", "format": "int8", "rows": 43, "shortest": 0, "longest": 301, "new": 1525,
+         "heads": KV_HEADS, "dim": HEAD_DIM},
+        # one listener, far into a long reading
+        {"name": "attend_1_3000", "kind": "attend", "format": "int8", "rows": 1, "shortest": 3000, "longest": 3000, "new": 1,
+         "query_heads": Q_HEADS, "heads": KV_HEADS, "dim": HEAD_DIM},
+        # a full lockstep batch, ragged
+        {"name": "attend_64_2048", "kind": "attend", "format": "int8", "rows": 64, "shortest": 64, "longest": 2048, "new": 1,
+         "query_heads": Q_HEADS, "heads": KV_HEADS, "dim": HEAD_DIM},
+        # a few very long contexts, 8 query heads to a key head
+        {"name": "attend_7_130k", "kind": "attend", "format": "e4m3", "rows": 7, "shortest": 90001, "longest": 131072, "new": 1,
+         "query_heads": 32, "heads": 4, "dim": 128},
+        # drafts of five tokens verified in an odd batch, heads of 64
+        {"name": "attend_draft_23", "kind": "attend", "format": "e4m3", "rows": 23, "shortest": 100, "longest": 4001, "new": 5,
+         "query_heads": Q_HEADS, "heads": KV_HEADS, "dim": 64},
+        # a long passage, from nothing
+        {"name": "attend_prompt_1500", "kind": "attend", "format": "int8", "rows": 1, "shortest": 1500, "longest": 1500, "new": 1500,
+         "query_heads": Q_HEADS, "heads": KV_HEADS, "dim": HEAD_DIM},
+        # a chunk of a very long prompt over what is cached of it
+        {"name": "attend_chunk_16k", "kind": "attend", "format": "int8", "rows": 1, "shortest": 16384, "longest": 16384, "new": 4096,
+         "query_heads": Q_HEADS, "heads": KV_HEADS, "dim": HEAD_DIM},
+        # a batch of ragged prompts behind a cached prefix, four query heads to a key head
+        {"name": "attend_prompts_11", "kind": "attend", "format": "e4m3", "rows": 11, "shortest": 1400, "longest": 3333, "new": 1333,
+         "query_heads": 32, "heads": 8, "dim": 128},
+    ]
+
+
+def _log_uniform(rng, low, high):
+    return min(high, max(low, int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))))
+
+
+def draw(rng):
+    kind = rng.choice(["tables", "append", "append", "attend", "attend", "attend"])
+    if kind == "tables":
+        return {"kind": kind, "rows": _log_uniform(rng, 1, 1000), "shortest": rng.randint(0, 300), "longest": _log_uniform(rng, 300, 7000),
+                "prompt": rng.choice([0, _log_uniform(rng, 20, 1500)]), "stride": rng.choice([512, 600, 1024])}
+    heads, dim = rng.choice([(8, 128), (8, 64), (4, 128), (1, 128), (2, 64)])
+    new = rng.choice([1, _log_uniform(rng, 2, 1500)])
+    case = {"kind": kind, "format": rng.choice(["int8", "e4m3"]), "heads": heads, "dim": dim}
+    if kind == "append":
+        rows = _log_uniform(rng, 1, 64 if new == 1 else max(1, 40000 // new))
+        shortest = rng.randint(0, 500)
+        return {**case, "rows": rows, "shortest": shortest, "longest": shortest + _log_uniform(rng, 1, 1500), "new": new}
+    group = rng.choice([1, 2, 4, 8])
+    if new == 1:
+        rows = _log_uniform(rng, 1, 64)
+        longest = _log_uniform(rng, 16, max(64, 130000 // rows))
+        shortest = rng.randint(1, longest)
+    else:
+        rows = _log_uniform(rng, 1, max(1, 6000 // new))
+        shortest = new + _log_uniform(rng, 1, 3000) - 1
+        longest = shortest + rng.randint(0, 2000)
+    return {**case, "rows": rows, "shortest": shortest, "longest": longest, "new": new, "query_heads": heads * group}
+
+
+# ---- inputs ------------------------------------------------------------------------------------------------------------
+
+def _spread(low, high, count):
+    """`count` lengths from low to high, both among them where there are two."""
+    return [high] if count == 1 else [low + (high - low) * i // (count - 1) for i in range(count)]
+
+
+def _new_tokens(case):
+    """New tokens of each row: `new`, where that is above one spread down to half of it."""
+    new, rows = case["new"], case["rows"]
+    return [new] * rows if new < 8 or rows == 1 else _spread((new + 1) // 2, new, rows)[::-1]
+
+
+def _generator(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _order(case, generator):
+    return torch.randperm(case["rows"], generator=generator, device="cuda").tolist()
+
+
+def _pool(lengths, generator, spare):
+    """A page table for rows of these lengths, and the pages of the pool: the ids in any order, -1 behind a row's last page."""
+    counts = [(n + PAGE - 1) // PAGE for n in lengths]
+    pages = sum(counts) + spare
+    ids = torch.randperm(pages, generator=generator, device="cuda").to(torch.int32)
+    stride = max(max(counts), 1)
+    starts = torch.tensor([sum(counts[:i]) for i in range(len(counts))], device="cuda")
+    column = torch.arange(stride, device="cuda")
+    inside = column[None, :] < torch.tensor(counts, device="cuda")[:, None]
+    table = torch.where(inside, ids[(starts[:, None] + column).clamp(max=pages - 1)], -1).to(torch.int32).contiguous()
+    return table, pages
+
+
+def _codes(values, form):
+    return values.round().clamp(-127, 127).to(torch.int8) if form == "int8" else values.clamp(-448, 448).to(torch.float8_e4m3fn)
+
+
+def _cache(case, pages, generator):
+    """Pages of values of about unit size, as the append leaves them."""
+    form, heads, dim = case["format"], case["heads"], case["dim"]
+    most = MOST[form]
+
+    def plane():
+        largest = 2.4 + 1.6 * torch.rand((pages, heads), generator=generator, device="cuda")
+        codes = torch.empty((pages, heads, PAGE, dim), dtype=torch.int8 if form == "int8" else torch.float8_e4m3fn, device="cuda")
+        for first in range(0, pages, 8192):
+            part = torch.randn((min(8192, pages - first), heads, PAGE, dim), generator=generator, device="cuda")
+            codes[first:first + 8192] = _codes(part * (most / largest[first:first + 8192, :, None, None]), form)
+        return codes, largest / most
+
+    k, ks = plane()
+    v, vs = plane()
+    return {"key": k, "value": v, "key_scales": ks, "value_scales": vs}
+
+
+def _tables_state(case, seed):
+    g = _generator(seed)
+    rows, stride, prompt = case["rows"], case["stride"], case["prompt"]
+    order = _order(case, g)
+    lengths = [_spread(case["shortest"], case["longest"], rows)[i] for i in order]
+    changes = []
+    for i, n in enumerate(lengths):
+        if prompt and i % 16 == 3:
+            changes.append(-n)                                            # done: all of its pages go back
+        elif prompt and i % 8 == 7:
+            changes.append(1 + (prompt - 1) * (i % 5 + 1) // 5)           # a prompt, or the next part of one
+        else:
+            changes.append(1)
+    table, used = _pool(lengths, g, 0)
+    coming = sum(max(0, c) for c in changes)
+    spare = coming // PAGE + 2 * rows
+    pages = used + spare
+    wide = torch.full((rows, stride), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table[:, :stride]
+    capacity = max(coming, 1)
+    free = torch.cat([used + torch.randperm(spare, generator=g, device="cuda"), torch.zeros(used, device="cuda")]).to(torch.int32)
+    ints = {"lengths": lengths, "changes": changes, "free_count": [spare]}
+    state = {name: torch.tensor(v, dtype=torch.int32, device="cuda") for name, v in ints.items()}
+    return {**state, "case": case, "pages": pages, "capacity": capacity, "page_table": wide, "free_pages": free,
+            "new_lengths": torch.zeros(rows, dtype=torch.int32, device="cuda"), "status": torch.zeros(rows, dtype=torch.int32, device="cuda"),
+            "new_free_count": torch.zeros(1, dtype=torch.int32, device="cuda"),
+            "token_starts": torch.zeros(rows + 1, dtype=torch.int32, device="cuda"),
+            "positions": torch.full((capacity,), -1, dtype=torch.int32, device="cuda"),
+            "slots": torch.full((capacity,), -1, dtype=torch.int64, device="cuda")}
+
+
+def _starts(new):
+    starts = [0]
+    for n in new:
+        starts.append(starts[-1] + n)
+    return torch.tensor(starts, dtype=torch.int32, device="cuda")
+
+
+def _append_state(case, seed):
+    g = _generator(seed)
+    order = _order(case, g)
+    heads, dim, rows = case["heads"], case["dim"], case["rows"]
+    held = [_spread(case["shortest"], case["longest"], rows)[i] for i in order]
+    new = [_new_tokens(case)[i] for i in order]
+    table, pages = _pool([h + n for h, n in zip(held, new)], g, 5)
+    cache = _cache(case, pages, g)
+    starts, count = _starts(new), sum(new)
+    row = torch.repeat_interleave(torch.arange(rows, device="cuda"), torch.tensor(new, device="cuda"))
+    position = torch.tensor(held, device="cuda")[row] + torch.arange(count, device="cuda") - starts[:-1][row]
+    slots = table[row, position // PAGE].to(torch.int64) * PAGE + position % PAGE
+    width = heads * dim
+    packed = torch.randn((count, 4 * width), generator=g, device="cuda")                      # q | k | v of a projection
+    packed *= 1.0 + 0.5 * torch.rand((count, 1), generator=g, device="cuda")                  # some tokens are larger than others
+    packed = packed.to(torch.bfloat16)
+    return {"case": case, "pages": pages, "tokens": count, "slots": slots, "starts": starts, "packed": packed,
+            "keys": packed[:, 2 * width:3 * width], "values": packed[:, 3 * width:], **cache}
+
+
+def _attend_state(case, seed):
+    g = _generator(seed)
+    order = _order(case, g)
+    new = [_new_tokens(case)[i] for i in order]
+    lengths = [max(_spread(case["shortest"], case["longest"], case["rows"])[i], n) for i, n in zip(order, new)]
+    table, pages = _pool(lengths, g, 5)
+    cache = _cache(case, pages, g)
+    width, count = case["query_heads"] * case["dim"], sum(new)
+    size = (1.0 + torch.rand((count, case["query_heads"], 1), generator=g, device="cuda"))    # some heads look more closely than others
+    q = (torch.randn((count, case["query_heads"], case["dim"]), generator=g, device="cuda") * size).to(torch.bfloat16)
+    return {"case": case, "pages": pages, "tokens": count, "most": max(new), "longest": max(lengths), "page_table": table,
+            "starts": _starts(new), "lengths": torch.tensor(lengths, dtype=torch.int32, device="cuda"), "query": q.view(count, width),
+            "output": torch.zeros((count, width), dtype=torch.bfloat16, device="cuda"), **cache}
+
+
+def prepare(case, seed):
+    return {"tables": _tables_state, "append": _append_state, "attend": _attend_state}[case["kind"]](case, seed)
+
+
+# ---- the plain forms ---------------------------------------------------------------------------------------------------
+
+def _plain_tables(s):
+    """Releases first, in the rows' order, then pages for the rows that grow, from the top of the pool."""
+    stride, pages, capacity = s["case"]["stride"], s["pages"], s["capacity"]
+    length, change = s["lengths"].to(torch.int64), s["changes"].to(torch.int64)
+    free = s["free_count"].to(torch.int64)
+    want = length + change
+    valid = (length >= 0) & (length <= stride * PAGE) & (want >= 0) & (want <= stride * PAGE)
+    before, after = (length + PAGE - 1) // PAGE, (want + PAGE - 1) // PAGE
+    grows, shrinks = valid & (change > 0), valid & (change < 0)
+    asked = torch.where(grows, change, 0)
+    need = torch.where(grows, after - before, 0)
+    given = torch.where(shrinks, before - after, 0)
+    needed, gone = need.cumsum(0), given.cumsum(0)
+    available = free + gone[-1]
+    room = asked.cumsum(0) <= capacity
+    paged = (need == 0) | (needed <= available)
+    served = grows & room & paged
+    status = torch.where(~valid, 2, torch.where(grows & ~room, 3, torch.where(grows & ~paged, 1, 0)))
+    left = available - torch.where(served, need, 0).sum()
+    column = torch.arange(stride, device="cuda")
+    table = s["page_table"]
+    back = shrinks[:, None] & (column >= after[:, None]) & (column < before[:, None])
+    place = torch.where(back, free + (gone - given)[:, None] + column - after[:, None], pages)
+    stack = torch.cat([s["free_pages"], s["free_pages"][:1]])
+    stack[place.clamp(max=pages)] = table
+    taken = served[:, None] & (column >= before[:, None]) & (column < after[:, None])
+    top = available - 1 - ((needed - need)[:, None] + column - before[:, None])
+    table = torch.where(taken, stack[top.clamp(0, pages)], table)
+    index = torch.arange(pages, device="cuda")
+    free_pages = torch.where((index >= free) & (index < left), stack[:pages], s["free_pages"])
+    tokens = torch.where(served, change, 0).cumsum(0)
+    starts = torch.cat([torch.zeros_like(tokens[:1]), tokens])
+    token = torch.arange(capacity, device="cuda")
+    row = (torch.searchsorted(starts, token, right=True) - 1).clamp(max=len(length) - 1)
+    position = length[row] + token - starts[row]
+    page = table[row, (position // PAGE).clamp(max=stride - 1)].to(torch.int64)
+    made = token < tokens[-1]
+    whole = lambda t: t.to(torch.int32)  # noqa: E731
+    return {"page_table": table, "free_pages": free_pages, "new_free_count": whole(left), "status": whole(status), "token_starts": whole(starts),
+            "new_lengths": whole(torch.where(served | shrinks, want, length)),
+            "positions": whole(torch.where(made, position, -1)), "slots": torch.where(made, page * PAGE + position % PAGE, -1)}
+
+
+def _round(values, form):
+    return torch.round(values) if form == "int8" else values.to(torch.float8_e4m3fn).float()
+
+
+def _plain_plane(s, name, tokens):
+    """The new tokens of a page share its scale with those that it holds, which are rounded again where the scale has grown."""
+    form, heads, dim = s["case"]["format"], s["case"]["heads"], s["case"]["dim"]
+    codes, old = s[name], s[name + "_scales"]
+    page, place = s["slots"] // PAGE, s["slots"] % PAGE
+    x = tokens.float().reshape(-1, heads, dim)
+    most = torch.full((), MOST[form], device="cuda")                                          # a tensor: divided by, not multiplied
+    largest = torch.full_like(old, -1.0).index_reduce(0, page, x.abs().amax(2), "amax")
+    first = s["slots"][s["starts"][:-1].to(torch.int64)]                                      # of each row: the page that may hold tokens
+    held = torch.zeros(old.shape[0], dtype=torch.int64, device="cuda").index_put((first // PAGE,), first % PAGE)
+    fresh = (largest / most).clamp(min=SMALLEST)
+    scale = torch.where(largest < 0, old, torch.where(held[:, None] > 0, torch.maximum(old, fresh), fresh))
+    inverse = 1.0 / scale
+    at = first // PAGE
+    kept = codes[at].float()
+    again = _round(kept * (old[at] * inverse[at])[:, :, None, None], form)
+    again = torch.where((scale[at] > old[at])[:, :, None, None] & (torch.arange(PAGE, device="cuda")[:, None] < held[at][:, None, None, None]), again, kept)
+    codes[at] = again.to(codes.dtype)
+    codes[page, :, place] = _round(x * inverse[page][:, :, None], form).to(codes.dtype)
+    old.copy_(scale)
+    return codes, old
+
+
+def _plain_append(s):
+    k, ks = _plain_plane(s, "key", s["keys"])
+    v, vs = _plain_plane(s, "value", s["values"])
+    return {"key": k, "value": v, "key_scales": ks, "value_scales": vs}
+
+
+def _plain_attend(s):
+    """Every row padded to the longest context and to the most new tokens of one."""
+    case = s["case"]
+    rows, heads, dim, most, count = case["rows"], case["heads"], case["dim"], s["most"], s["tokens"]
+    group = case["query_heads"] // heads
+    table = s["page_table"].clamp(min=0).to(torch.int64)
+
+    def plane(name):
+        x = s[name][table].float() * s[name + "_scales"][table][..., None, None]              # [rows][pages][heads][16][dim]
+        return x.permute(0, 2, 1, 3, 4).reshape(rows, heads, -1, dim)
+
+    starts, length = s["starts"].to(torch.int64), s["lengths"].to(torch.int64)
+    new = starts[1:] - starts[:-1]
+    step = torch.arange(most, device="cuda")
+    q = s["query"][(starts[:-1, None] + step).clamp(max=count - 1)].float().view(rows, most, heads, group, dim)
+    q = q.permute(0, 2, 3, 1, 4).reshape(rows, heads, group * most, dim)
+    scores = torch.matmul(q, plane("key").transpose(2, 3)).view(rows, heads, group, most, -1) / math.sqrt(dim)
+    position = length[:, None] - new[:, None] + step
+    seen = torch.arange(scores.shape[-1], device="cuda") <= position[..., None]
+    scores.masked_fill_(~seen[:, None, None], -math.inf)
+    scores -= scores.amax(-1, keepdim=True)
+    weights = scores.exp_()
+    total = weights.sum(-1, keepdim=True)
+    out = torch.matmul(weights.view(rows, heads, group * most, -1), plane("value")).view(rows, heads, group, most, dim) / total
+    out = out.permute(0, 3, 1, 2, 4).reshape(rows, most, -1)
+    row = torch.repeat_interleave(torch.arange(rows, device="cuda"), new, output_size=count)
+    return out[row, torch.arange(count, device="cuda") - starts[row]].to(torch.bfloat16)
+
+
+# ---- the framework's calls ---------------------------------------------------------------------------------------------
+
+def _pointer(t):
+    return t.data_ptr()
+
+
+def _own_cache(ops, s):
+    return ops.kv8_cache(s["key"], s["value"], s["key_scales"], s["value_scales"])
+
+
+def _own_call(s):
+    """What a host keeps of a call: the function and its arguments, addresses and sizes alone."""
+    package = importlib.import_module("qwen3-tts-native_b200")
+    ops = importlib.import_module("qwen3-tts-native_b200.ops")
+    lib, case = package.library(), s["case"]
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    if case["kind"] == "tables":
+        d = ops.PageTablesDescC(rows=case["rows"], page_table_stride=case["stride"], pages=s["pages"], token_capacity=s["capacity"])
+        d.struct_size = C.sizeof(d)
+        for name in ("lengths", "changes", "new_lengths", "page_table", "free_pages", "free_count", "new_free_count", "status",
+                     "token_starts", "positions", "slots"):
+            setattr(d, name, _pointer(s[name]))
+        return lib.q3t_launch_page_tables, (C.byref(d), stream), [d]
+    cache = _own_cache(ops, s)
+    if case["kind"] == "append":
+        args = (C.byref(cache), C.c_void_p(_pointer(s["keys"])), C.c_void_p(_pointer(s["values"])), C.c_void_p(_pointer(s["slots"])), None,
+                s["tokens"], s["keys"].stride(0), s["values"].stride(0), stream)
+        return lib.q3t_launch_kv8_append, args, [cache]
+    d = ops.Kv8AttentionDescC(rows=case["rows"], query_heads=case["query_heads"], page_table_stride=s["page_table"].shape[1], tokens=s["tokens"],
+                              max_row_tokens=s["most"], max_sequence_length=s["longest"])
+    d.struct_size = C.sizeof(d)
+    d.cache = C.addressof(cache)
+    for name, held in (("query", "query"), ("output", "output"), ("page_table", "page_table"), ("lengths", "lengths"), ("token_starts", "starts")):
+        setattr(d, name, _pointer(s[held]))
+    size = int(lib.q3t_kv8_attention_scratch_bytes(C.byref(d)))
+    scratch = torch.empty(max(size, 16), dtype=torch.uint8, device="cuda")
+    d.scratch, d.scratch_bytes = _pointer(scratch), size
+    return lib.q3t_launch_kv8_attention, (C.byref(d), stream), [d, cache, scratch]
+
+
+def _own(s):
+    if "call" not in s:
+        s["call"] = _own_call(s)
+    function, arguments, _ = s["call"]
+    status = function(*arguments)
+    if status != 0:
+        raise RuntimeError("launch returned %d" % status)
+    kind = s["case"]["kind"]
+    if kind == "attend":
+        return s["output"]
+    names = ("key", "value", "key_scales", "value_scales") if kind == "append" else (
+        "page_table", "free_pages", "new_free_count", "status", "token_starts", "new_lengths", "positions", "slots")
+    return {name: s[name] for name in names}
+
+
+def run(state):
+    if own:
+        return _own(state)
+    return {"tables": _plain_tables, "append": _plain_append, "attend": _plain_attend}[state["case"]["kind"]](state)
+
+
+# ---- what a pass cannot do without -------------------------------------------------------------------------------------
+
+def work(case):
+    rows = case["rows"]
+    if case["kind"] == "tables":
+        prompts = sum(1 for i in range(rows) if i % 16 != 3 and i % 8 == 7) if case["prompt"] else 0
+        tokens = rows + prompts * case["prompt"] * 3 // 5
+        return {"bytes": rows * 20 + tokens * 12 + (tokens // PAGE + rows) * 8, "flops": tokens}
+    width = case["heads"] * case["dim"]
+    new = sum(_new_tokens(case))
+    if case["kind"] == "append":
+        blocks = new // PAGE + rows
+        return {"bytes": new * (2 * width * 3 + 8) + blocks * case["heads"] * 2 * 4, "flops": new * 2 * width * 4}
+    lengths = [max(n, c) for n, c in zip(_spread(case["shortest"], case["longest"], rows), _new_tokens(case))]
+    pages = sum((n + PAGE - 1) // PAGE for n in lengths)
+    seen = sum(c * n - c * (c - 1) // 2 for n, c in zip(lengths, _new_tokens(case)))
+    return {"bytes": sum(lengths) * 2 * width + pages * (case["heads"] * 8 + 4) + new * case["query_heads"] * case["dim"] * 4,
+            "flops": 4 * seen * case["query_heads"] * case["dim"]}
+
+
+# ---- the definition in 64 bits -----------------------------------------------------------------------------------------
+
+def _nearest(v, form):
+    if form == "int8":
+        return v.round().clamp(-127, 127)
+    step = torch.exp2(torch.floor(torch.log2(v.abs().clamp(min=2.0 ** -6))) - 3)
+    return ((v / step).round() * step).clamp(-448, 448)
+
+
+def _exact_append(s):
+    case, out = s["case"], {}
+    form, heads, dim = case["format"], case["heads"], case["dim"]
+    slots = s["slots"].tolist()
+    for name, source in (("key", s["keys"]), ("value", s["values"])):
+        x = source.double().view(-1, heads, dim)
+        codes, scales = s[name].double(), s[name + "_scales"].double()
+        first = 0
+        while first < len(slots):
+            page, last = slots[first] // PAGE, first
+            while last < len(slots) and slots[last] // PAGE == page:
+                last += 1
+            low, new = slots[first] % PAGE, x[first:last]
+            scale = (new.abs().amax(dim=(0, 2)) / MOST[form]).clamp(min=SMALLEST)
+            if low > 0:
+                scale = torch.maximum(scale, scales[page])
+                codes[page, :, :low] = _nearest(codes[page, :, :low] * (scales[page] / scale)[:, None, None], form)
+            codes[page, :, low:low + last - first] = _nearest(new / scale[:, None], form).transpose(0, 1)
+            scales[page] = scale
+            first = last
+        out[name] = None if form == "int8" else codes
+        out[name + "_scales"] = scales
+    return out
+
+
+def _exact_attend(s):
+    case = s["case"]
+    heads, dim = case["heads"], case["dim"]
+    group = case["query_heads"] // heads
+    out = torch.zeros((s["tokens"], case["query_heads"], dim), dtype=torch.float64, device="cuda")
+    starts, lengths = s["starts"].tolist(), s["lengths"].tolist()
+    for r, length in enumerate(lengths):
+        ids = s["page_table"][r, :(length + PAGE - 1) // PAGE].long()
+        q = s["query"][starts[r]:starts[r + 1]].double().view(-1, heads, group, dim)
+        limit = length - q.shape[0] + torch.arange(q.shape[0], device="cuda")
+        for h in range(heads):
+            k = (s["key"][ids, h].double() * s["key_scales"][ids, h].double()[:, None, None]).reshape(-1, dim)[:length]
+            v = (s["value"][ids, h].double() * s["value_scales"][ids, h].double()[:, None, None]).reshape(-1, dim)[:length]
+            for i in range(group):
+                a = q[:, h, i] @ k.T * dim ** -0.5
+                a = torch.softmax(a.masked_fill(torch.arange(length, device="cuda") > limit[:, None], -math.inf), dim=1)
+                out[starts[r]:starts[r + 1], h * group + i] = a @ v
+    return out.view(s["tokens"], -1)
+
+
+def exact(case, seed):
+    if case["kind"] == "tables":
+        return None                                                                           # whole numbers alone
+    return (_exact_append if case["kind"] == "append" else _exact_attend)(prepare(case, seed))
