@@ -348,6 +348,120 @@ QWEN3_TTS_API int32_t q3t_launch_decode_attention_ex(const Q3tAttentionDesc* des
  * overwritten.  Returns when it is done. */
 QWEN3_TTS_API int32_t q3t_test_prompt_attention(const Q3tAttentionDesc* desc, int32_t base);
 
+/* ---- KV cache in 8 bits ------------------------------------------------------------------
+ * No counterpart in the reference, whose caches are bf16.  Three operators for hosts with a decoder loop of their own and
+ * more context than bf16 caches have room for: page tables from the requests' lengths, quantising append, attention.
+ * All of them read lengths and page ids on the device, so that a captured step stays valid while its batch moves on.
+ * Pointers in descriptors are device pointers unless said otherwise; the descriptors themselves are host memory and are
+ * read before the call returns.  Launches go to the current device.  Buffers must not overlap unless said otherwise. */
+
+/* Block tables and slot maps.  Row r holds lengths[r] tokens in pages of Q3T_KV_PAGE_TOKENS whose ids are the first entries of
+ * its row of the page table; changes[r] > 0 tokens are to come, or -changes[r] are given back from the end (all of them: the
+ * request is done).  Ids that nobody has lie on a stack.  In the order of the rows, first the pages given back go onto
+ * the stack (a row's own in the order of its table), then rows that grow take theirs from its top.  Same inputs, same tables.
+ * A row is served whole or not at all: status[r] says which, and one that is not served keeps its length and table and gets
+ * no tokens.  What it asked for still counts against the rows behind it; rows that need no page are served either way.
+ * New tokens get numbers in the order of the rows: those of row r are token_starts[r] .. token_starts[r + 1] - 1, at the
+ * positions lengths[r], lengths[r] + 1, ... and in the slots page id * 16 + position % 16.  positions and slots behind the last
+ * token, table entries behind a row's last page and stack entries from *new_free_count on are left as they were.
+ * The tables are what Q3tAttentionDesc (bf16 pages) and Q3tKv8AttentionDesc take. */
+#define Q3T_MAX_TABLE_ROWS 4096
+enum {
+    Q3T_TABLE_OK = 0,
+    Q3T_TABLE_NO_PAGES = 1,      /* the pool does not have the pages that rows up to this one ask for */
+    Q3T_TABLE_LENGTH = 2,        /* the length before or after is negative or more than the table's row has room for */
+    Q3T_TABLE_NO_TOKENS = 3      /* rows up to this one ask for more than token_capacity tokens */
+};
+typedef struct Q3tPageTablesDesc {
+    uint32_t struct_size;        /* sizeof(Q3tPageTablesDesc) */
+    int32_t rows;                /* 1..Q3T_MAX_TABLE_ROWS */
+    const int32_t* lengths;      /* [rows] */
+    const int32_t* changes;      /* [rows] */
+    int32_t* new_lengths;        /* [rows]; may be lengths */
+    int32_t* page_table;         /* [rows][page_table_stride] */
+    int32_t* free_pages;         /* [pages]: the stack, its top at *free_count - 1 */
+    const int32_t* free_count;   /* [1]; taken as 0..pages */
+    int32_t* new_free_count;     /* [1]; may be free_count */
+    int32_t* status;             /* [rows] Q3T_TABLE_* */
+    int32_t* token_starts;       /* [rows + 1] */
+    int32_t* positions;          /* [token_capacity], optional */
+    int64_t* slots;              /* [token_capacity], optional */
+    int32_t page_table_stride;
+    int32_t pages;               /* of the pool */
+    int32_t token_capacity;
+    int32_t reserved;            /* 0 */
+} Q3tPageTablesDesc;
+QWEN3_TTS_API int32_t q3t_launch_page_tables(const Q3tPageTablesDesc* desc, void* stream);
+
+/* A cache of 8-bit codes.  A page holds 16 tokens of one plane (K or V) as [key_value_heads][16][head_dimension] codes, the
+ * layout of the bf16 pages, and has one fp32 scale for each head: value = code * scale.  Codes are int8 (-127..127) or
+ * e4m3.  The planes' pages may lie apart (page_stride, scale_stride), so that one pool can hold many layers. */
+enum { Q3T_KV8_INT8 = 0, Q3T_KV8_E4M3 = 1 };
+typedef struct Q3tKv8Cache {
+    uint32_t struct_size;        /* sizeof(Q3tKv8Cache) */
+    int32_t format;              /* Q3T_KV8_* */
+    uint8_t* key_pages;          /* 16-byte aligned */
+    uint8_t* value_pages;
+    float* key_scales;
+    float* value_scales;
+    int64_t page_stride;         /* bytes between consecutive pages of a plane, a multiple of 16; 0: they lie side by side */
+    int64_t scale_stride;        /* elements between the scales of consecutive pages; 0: key_value_heads */
+    int32_t pages;               /* ids are 0..pages - 1 */
+    int32_t key_value_heads;     /* 1..64 */
+    int32_t head_dimension;      /* 64, 128 */
+    int32_t reserved;            /* 0 */
+} Q3tKv8Cache;
+
+/* Quantises the keys and values of new tokens (bf16, [tokens][stride], head h at h * head_dimension; 16-byte aligned, strides
+ * multiples of 8 elements, 0: key_value_heads * head_dimension) into their slots.  A token whose slot is negative is left
+ * out (padding); token_count, when given, is read on the device (token_starts + rows, for one) and cuts `tokens` short.
+ *   scale = max(largest |x| of the page's new tokens in the head / M, 2^-126), M = 127 (int8) or 448 (e4m3),
+ *   code  = round(x * (1 / scale)), to nearest even, every operation in fp32.
+ * A page is filled from its first slot on: tokens in slots below the new ones are held.  With such, the scale is the larger of that
+ * and the page's own, and where it has grown the held codes become round(code * (own scale * (1 / scale))); nothing else of the
+ * page changes.  The same tokens appended again change nothing, and slots may be filled anew from any point on.
+ * Tokens of one page stand next to each other; where they name a slot twice the last one is kept.  (Tokens of a page that
+ * stand apart leave some of its values and its scale unspecified.)  A value that is not finite is stored as the largest finite
+ * bf16 of its sign and its page, head and plane counted (process-wide per device) by q3t_kv8_nonfinite_count; a slot past the
+ * last page is left out and counted by q3t_kv8_page_error_count. */
+QWEN3_TTS_API int32_t q3t_launch_kv8_append(const Q3tKv8Cache* cache, const uint16_t* key, const uint16_t* value,
+                                            const int64_t* slots, const int32_t* token_count, int32_t tokens,
+                                            int32_t key_stride, int32_t value_stride, void* stream);
+
+/* Causal attention of the new tokens of `rows` rows over such a cache.  Row r has the tokens token_starts[r] .. token_starts[r + 1] - 1
+ * of query and output (none, one, a draft, a prompt, a chunk of one), which are the last ones of its lengths[r]; each attends to
+ * the positions up to its own.  Query head h reads key/value head h / (query_heads / key_value_heads).  A token without a
+ * position (a row shorter than its new tokens) gets zeros; output behind the last token is left as it was.
+ * Scores, statistics and sums are fp32; query and weights enter the products as fp16 with 11 bits kept, scaled by powers of two so
+ * that neither size matters.  Bounds that the host gives (tokens, max_row_tokens, max_sequence_length) cut what the device finds
+ * larger: a row is then computed over its first max_sequence_length tokens and counted by q3t_attention_range_error_count. A page id
+ * outside 0..pages - 1 is left out of the attention, as if masked, and counted by q3t_kv8_page_error_count. */
+typedef struct Q3tKv8AttentionDesc {
+    uint32_t struct_size;        /* sizeof(Q3tKv8AttentionDesc) */
+    int32_t rows;                /* 1..Q3T_MAX_TABLE_ROWS */
+    const Q3tKv8Cache* cache;    /* host pointer */
+    const uint16_t* query;       /* [tokens][query_stride], 16-byte aligned */
+    uint16_t* output;            /* [tokens][output_stride], 16-byte aligned */
+    float* output_f32;           /* optional: [tokens][query_heads * head_dimension], before the last bf16 round */
+    const int32_t* page_table;   /* [rows][page_table_stride] */
+    const int32_t* lengths;      /* [rows] tokens in the cache, the new ones among them */
+    const int32_t* token_starts; /* [rows + 1], ascending; NULL: one token a row */
+    int32_t page_table_stride;
+    int32_t query_heads;         /* a multiple of key_value_heads, up to 64 to each */
+    int32_t query_stride;        /* elements, a multiple of 8; 0: query_heads * head_dimension */
+    int32_t output_stride;
+    int32_t tokens;              /* token_starts[rows] at most */
+    int32_t max_row_tokens;      /* most new tokens of a row */
+    int32_t max_sequence_length; /* largest length, at most page_table_stride * 16 */
+    float scale;                 /* of the scores; 0: 1 / sqrt(head_dimension) */
+    void* scratch;               /* 16-byte aligned; launches that share it must be ordered */
+    size_t scratch_bytes;
+} Q3tKv8AttentionDesc;
+QWEN3_TTS_API size_t q3t_kv8_attention_scratch_bytes(const Q3tKv8AttentionDesc* desc);      /* 0: arguments that are refused */
+QWEN3_TTS_API int32_t q3t_launch_kv8_attention(const Q3tKv8AttentionDesc* desc, void* stream);
+QWEN3_TTS_API uint32_t q3t_kv8_nonfinite_count(void);
+QWEN3_TTS_API uint32_t q3t_kv8_page_error_count(void);
+
 /* ---- sampler (sampling_kernels.cu) ------------------------------------------------------- */
 
 /* launch_sample_logits (sampling_kernels.cu:460-498) */

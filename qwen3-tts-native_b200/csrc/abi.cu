@@ -1164,7 +1164,7 @@ uint32_t q3t_kernel_error_count(void) {
     return gemm_tc_error_count() + gemm_wide_error_count() + gemm_pair_error_count() + gemv_mma_error_count() + chain_error_count() + lockstep_error_count() + prompt_attention_error_count();
 }
 
-uint32_t q3t_attention_range_error_count(void) { return attention_range_error_count(); }
+uint32_t q3t_attention_range_error_count(void) { return attention_range_error_count() + kv8_range_error_count(); }
 
 int32_t q3t_session_current_token(Qwen3TtsSessionHandle session, uint16_t* token, char* error,
                                   size_t error_capacity) {

@@ -1,0 +1,87 @@
+// What the kernels of the 8-bit KV cache share: the view of a cache, its codes, the span of a row's new tokens.
+//
+// A page of one plane (K or V) holds 16 tokens as [kv head][16][head_dim] codes, head-major like the bf16 pages, and one fp32
+// scale for each head; a value is code * scale.
+#pragma once
+
+#include "q3t_common.cuh"
+#include "q3t_ops.h"
+
+#include <cuda_fp16.h>
+
+namespace q3t {
+
+constexpr float kKv8SmallestScale = 1.17549435e-38f;      // 2^-126: its reciprocal is finite, and neither is subnormal
+
+struct Kv8View {
+    uint8_t* k;
+    uint8_t* v;
+    float* k_scales;
+    float* v_scales;
+    long long page_stride;       // bytes
+    long long scale_stride;      // elements
+    int pages;
+    int heads;
+};
+
+// false: the descriptor is refused
+inline bool kv8_view(const Q3tKv8Cache* c, Kv8View* view) {
+    if (c == nullptr || c->struct_size != sizeof(Q3tKv8Cache) || (c->format != Q3T_KV8_INT8 && c->format != Q3T_KV8_E4M3)
+        || c->key_pages == nullptr || c->value_pages == nullptr || c->key_scales == nullptr || c->value_scales == nullptr
+        || c->pages < 1 || c->key_value_heads < 1 || c->key_value_heads > 64 || (c->head_dimension != 64 && c->head_dimension != 128)
+        || c->reserved != 0) {
+        return false;
+    }
+    const long long page_bytes = (long long)c->key_value_heads * kPageTokens * c->head_dimension;
+    view->k = c->key_pages;
+    view->v = c->value_pages;
+    view->k_scales = c->key_scales;
+    view->v_scales = c->value_scales;
+    view->page_stride = c->page_stride != 0 ? c->page_stride : page_bytes;
+    view->scale_stride = c->scale_stride != 0 ? c->scale_stride : c->key_value_heads;
+    view->pages = c->pages;
+    view->heads = c->key_value_heads;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(c->key_pages) | reinterpret_cast<uintptr_t>(c->value_pages);
+    const uintptr_t scales_at = reinterpret_cast<uintptr_t>(c->key_scales) | reinterpret_cast<uintptr_t>(c->value_scales);
+    return view->page_stride >= page_bytes && view->page_stride % 16 == 0 && view->scale_stride >= c->key_value_heads && at % 16 == 0
+           && scales_at % sizeof(float) == 0;
+}
+
+// two e4m3 codes (the low 16 bits) as fp16, exact
+__device__ __forceinline__ uint32_t e4m3_to_half2(uint32_t codes) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<unsigned short>(codes)));
+    return r;
+}
+// (lo, hi) rounded to e4m3, lo in the low byte
+__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
+    unsigned short r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// The new tokens of one row, as the device finds them, cut to what the host said of them
+struct RowSpan {
+    int first;        // number of its first new token
+    int count;        // computed, 0 and more
+    int base;         // position of the first one (negative: the row is shorter than its new tokens)
+    bool cut;         // something was larger than the host said
+};
+__device__ __forceinline__ RowSpan row_span(const int* starts, const int* lengths, int row, int tokens, int most, int max_sequence) {
+    RowSpan s;
+    const int length = lengths[row];
+    int from = row, to = row + 1;
+    if (starts != nullptr) {
+        from = starts[row];
+        to = starts[row + 1];
+    }
+    s.first = min(max(from, 0), tokens);
+    const int end = min(max(to, s.first), tokens);
+    const int whole = end - s.first;
+    s.count = min(whole, most);
+    s.base = length - whole;
+    s.cut = from != s.first || to != end || s.count != whole || length > max_sequence;
+    return s;
+}
+
+}  // namespace q3t

@@ -213,6 +213,7 @@ cudaError_t launch_attention_reference_order(const AttentionArgs& args, cudaStre
 // launcher that honours it: in mode 0 a fused call appends with the split-KV kernel's prologue,
 // then attends in the reference's order.
 // rows seen so far whose position lay outside what the launch was sized for (clamped and counted)
+unsigned int kv8_range_error_count();          // kv8_attention.cu
 unsigned int attention_range_error_count();
 cudaError_t set_attention_error_sink(unsigned int* device_visible_word);
 int set_attention_mode(int mode);

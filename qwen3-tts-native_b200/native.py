@@ -132,6 +132,8 @@ EXPORTED_SYMBOLS = (
     "q3t_packet_stager_create", "q3t_packet_stager_destroy", "q3t_packet_stager_device_bytes",
     "q3t_packet_stager_staged_frames", "q3t_packet_stager_stage_frame", "q3t_packet_stager_packet_view",
     "q3t_packet_stager_release_after_consumer",
+    "q3t_launch_page_tables", "q3t_launch_kv8_append", "q3t_kv8_attention_scratch_bytes", "q3t_launch_kv8_attention",
+    "q3t_kv8_nonfinite_count", "q3t_kv8_page_error_count",
 )
 
 _lib: Optional[C.CDLL] = None
@@ -153,6 +155,9 @@ def library() -> C.CDLL:
         for name, restype in (("q3t_attention_scratch_bytes", C.c_size_t),
                               ("q3t_attention_static_scratch_capacity", C.c_size_t),
                               ("q3t_kernel_error_count", C.c_uint32),
+                              ("q3t_kv8_attention_scratch_bytes", C.c_size_t),
+                              ("q3t_kv8_nonfinite_count", C.c_uint32),
+                              ("q3t_kv8_page_error_count", C.c_uint32),
                               ("q3t_test_fail_launch_after", None),
                               ("q3t_test_fail_allocation_after", None)):
             if hasattr(lib, name):

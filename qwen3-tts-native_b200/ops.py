@@ -41,6 +41,36 @@ class AttentionDescC(C.Structure):   # include/q3t_ops.h Q3tAttentionDesc
                 ("scratch_bytes", C.c_size_t)]
 
 
+class PageTablesDescC(C.Structure):   # include/q3t_ops.h Q3tPageTablesDesc
+    _fields_ = [("struct_size", C.c_uint32), ("rows", C.c_int32), ("lengths", C.c_void_p),
+                ("changes", C.c_void_p), ("new_lengths", C.c_void_p), ("page_table", C.c_void_p),
+                ("free_pages", C.c_void_p), ("free_count", C.c_void_p), ("new_free_count", C.c_void_p),
+                ("status", C.c_void_p), ("token_starts", C.c_void_p), ("positions", C.c_void_p),
+                ("slots", C.c_void_p), ("page_table_stride", C.c_int32), ("pages", C.c_int32),
+                ("token_capacity", C.c_int32), ("reserved", C.c_int32)]
+
+
+class Kv8CacheC(C.Structure):   # include/q3t_ops.h Q3tKv8Cache
+    _fields_ = [("struct_size", C.c_uint32), ("format", C.c_int32), ("key_pages", C.c_void_p),
+                ("value_pages", C.c_void_p), ("key_scales", C.c_void_p), ("value_scales", C.c_void_p),
+                ("page_stride", C.c_int64), ("scale_stride", C.c_int64), ("pages", C.c_int32),
+                ("key_value_heads", C.c_int32), ("head_dimension", C.c_int32), ("reserved", C.c_int32)]
+
+
+class Kv8AttentionDescC(C.Structure):   # include/q3t_ops.h Q3tKv8AttentionDesc
+    _fields_ = [("struct_size", C.c_uint32), ("rows", C.c_int32), ("cache", C.c_void_p),
+                ("query", C.c_void_p), ("output", C.c_void_p), ("output_f32", C.c_void_p),
+                ("page_table", C.c_void_p), ("lengths", C.c_void_p), ("token_starts", C.c_void_p),
+                ("page_table_stride", C.c_int32), ("query_heads", C.c_int32),
+                ("query_stride", C.c_int32), ("output_stride", C.c_int32), ("tokens", C.c_int32),
+                ("max_row_tokens", C.c_int32), ("max_sequence_length", C.c_int32),
+                ("scale", C.c_float), ("scratch", C.c_void_p), ("scratch_bytes", C.c_size_t)]
+
+
+TABLE_OK, TABLE_NO_PAGES, TABLE_LENGTH, TABLE_NO_TOKENS = range(4)
+KV8_INT8, KV8_E4M3 = range(2)
+
+
 def _dev(a: Optional[np.ndarray], device="cuda") -> Optional[torch.Tensor]:
     if a is None:
         return None
@@ -364,3 +394,98 @@ def sample(logits, rng_state: int, *, suppress=False, history: Optional[Sequence
                                           _ptr(dt), None)
     _ok(rc, "q3t_launch_sample_logits")
     return int(dt.item()), int(dr.cpu().numpy().view(np.uint64)[0])
+
+
+def page_tables(lengths, changes, page_table, free_pages, free_count, *, token_capacity=None, fill=-7, want_slots=True):
+    """Block tables and slot maps of a batch.  Returns dict(page_table, free_pages, free_count, lengths, status, starts,
+    positions, slots): copies of what the launch leaves; positions and slots of `token_capacity` entries, `fill` where nothing was written."""
+    lengths = np.asarray(lengths, dtype=np.int32)
+    rows = lengths.size
+    free_pages = np.asarray(free_pages, dtype=np.int32)
+    capacity = int(np.clip(np.asarray(changes, dtype=np.int64), 0, None).sum()) if token_capacity is None else token_capacity
+    held = {"lengths": _dev(lengths), "changes": _dev(np.asarray(changes, dtype=np.int32)),
+            "page_table": _dev(np.asarray(page_table, dtype=np.int32)), "free_pages": _dev(free_pages),
+            "free_count": _dev(np.array([free_count], dtype=np.int32))}
+    for name, count in (("new_lengths", rows), ("new_free_count", 1), ("status", rows), ("token_starts", rows + 1),
+                        ("positions", max(capacity, 1))):
+        held[name] = torch.full((count,), fill, dtype=torch.int32, device="cuda")
+    held["slots"] = torch.full((max(capacity, 1),), fill, dtype=torch.int64, device="cuda")
+    d = PageTablesDescC(rows=rows, page_table_stride=held["page_table"].shape[1], pages=free_pages.size, token_capacity=capacity)
+    d.struct_size = C.sizeof(d)
+    for name, t in held.items():
+        if want_slots or name not in ("positions", "slots"):
+            setattr(d, name, t.data_ptr())
+    _ok(native.library().q3t_launch_page_tables(C.byref(d), None), "q3t_launch_page_tables")
+    got = {name: t.cpu().numpy() for name, t in held.items()}
+    return dict(page_table=got["page_table"], free_pages=got["free_pages"], free_count=int(got["new_free_count"][0]),
+                lengths=got["new_lengths"], status=got["status"], starts=got["token_starts"],
+                positions=got["positions"][:capacity], slots=got["slots"][:capacity])
+
+
+def kv8_cache(key, value, key_scales, value_scales) -> Kv8CacheC:
+    """The descriptor of a cache whose planes are CUDA tensors [pages][kv heads][16][head dim] of int8 or float8_e4m3fn and whose
+    scales are [pages][kv heads] of float32; heads have to be dense, pages may lie apart (the same way in both planes)."""
+    pages, heads, tokens, dim = key.shape
+    for plane, scale in ((key, key_scales), (value, value_scales)):
+        if (plane.dtype not in (torch.int8, torch.float8_e4m3fn) or plane.dtype != key.dtype or plane.shape != key.shape or tokens != 16
+                or plane.stride() != (key.stride(0), 16 * dim, dim, 1) or scale.dtype != torch.float32
+                or scale.shape != (pages, heads) or scale.stride() != (key_scales.stride(0), 1)):
+            raise ValueError("planes are [pages][heads][16][dim] of one 8-bit type, dense but for the pages; scales [pages][heads] of float32")
+    c = Kv8CacheC(format=KV8_INT8 if key.dtype == torch.int8 else KV8_E4M3, pages=pages, key_value_heads=heads, head_dimension=dim,
+                  page_stride=key.stride(0), scale_stride=key_scales.stride(0))
+    c.struct_size = C.sizeof(c)
+    c.key_pages, c.value_pages = key.data_ptr(), value.data_ptr()
+    c.key_scales, c.value_scales = key_scales.data_ptr(), value_scales.data_ptr()
+    return c
+
+
+def _planes(key, value, key_scales, value_scales, e4m3):
+    """Device copies of numpy planes of codes (uint8 bit patterns) and scales."""
+    kind = torch.float8_e4m3fn if e4m3 else torch.int8
+    codes = [torch.from_numpy(np.ascontiguousarray(p, dtype=np.uint8)).cuda().view(kind) for p in (key, value)]
+    return codes + [_dev(np.asarray(s, dtype=np.float32)) for s in (key_scales, value_scales)]
+
+
+def kv8_append(key, value, key_scales, value_scales, k_new, v_new, slots, *, e4m3=False, count=None):
+    """Quantises bf16 rows k_new, v_new [tokens][heads * dim] into planes of codes [pages][heads][16][dim] (uint8 bit patterns) with scales
+    [pages][heads]; `count`: read on the device in place of the rows' number.  Returns the four arrays afterwards."""
+    planes = _planes(key, value, key_scales, value_scales, e4m3)
+    c = kv8_cache(*planes)
+    dk, dv = _dev(np.asarray(k_new, dtype=np.uint16)), _dev(np.asarray(v_new, dtype=np.uint16))
+    ds = _dev(np.asarray(slots, dtype=np.int64))
+    dc = _dev(np.array([count], dtype=np.int32)) if count is not None else None
+    _ok(native.library().q3t_launch_kv8_append(C.byref(c), _ptr(dk), _ptr(dv), _ptr(ds), _ptr(dc), ds.numel(), 0, 0, None),
+        "q3t_launch_kv8_append")
+    return [p.view(torch.uint8).cpu().numpy() for p in planes[:2]] + [p.cpu().numpy() for p in planes[2:]]
+
+
+def kv8_attention(q, key, value, key_scales, value_scales, page_table, lengths, starts=None, *, e4m3=False, max_row_tokens=None,
+                  max_seq=None, scale=0.0, want_f32=False, fill=0x7fc0):
+    """Attention of the new tokens q [tokens][query heads * dim] (bf16) over an 8-bit cache.  Returns (out, f32 or None); rows of `out`
+    that no token fills keep the bits `fill`."""
+    lib = native.library()
+    planes = _planes(key, value, key_scales, value_scales, e4m3)
+    c = kv8_cache(*planes)
+    q = np.ascontiguousarray(q, dtype=np.uint16)
+    lengths = np.asarray(lengths, dtype=np.int32)
+    page_table = np.asarray(page_table, dtype=np.int32)
+    dim = key.shape[3]
+    held = {"query": _dev(q), "page_table": _dev(page_table), "lengths": _dev(lengths),
+            "output": _dev(np.full(q.shape, fill, dtype=np.uint16))}
+    if starts is not None:
+        held["token_starts"] = _dev(np.asarray(starts, dtype=np.int32))
+    if want_f32:
+        held["output_f32"] = torch.full(q.shape, float("nan"), dtype=torch.float32, device="cuda")
+    if max_row_tokens is None:
+        max_row_tokens = 1 if starts is None else int(np.diff(np.asarray(starts)).max())
+    d = Kv8AttentionDescC(rows=lengths.size, query_heads=q.shape[1] // dim, page_table_stride=page_table.shape[1], tokens=q.shape[0],
+                          max_row_tokens=max_row_tokens, max_sequence_length=max_seq or page_table.shape[1] * 16, scale=scale)
+    d.struct_size = C.sizeof(d)
+    d.cache = C.addressof(c)
+    for name, t in held.items():
+        setattr(d, name, t.data_ptr())
+    nbytes = int(lib.q3t_kv8_attention_scratch_bytes(C.byref(d)))
+    scratch = torch.full((max(nbytes, 16),), 0xa5, dtype=torch.uint8, device="cuda")
+    d.scratch, d.scratch_bytes = scratch.data_ptr(), nbytes
+    _ok(lib.q3t_launch_kv8_attention(C.byref(d), None), "q3t_launch_kv8_attention")
+    return _u16(held["output"]), held["output_f32"].cpu().numpy() if want_f32 else None
