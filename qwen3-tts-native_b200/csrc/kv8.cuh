@@ -9,6 +9,8 @@
 
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 namespace q3t {
 
 constexpr float kKv8SmallestScale = 1.17549435e-38f;      // 2^-126: its reciprocal is finite, and neither is subnormal
@@ -45,6 +47,19 @@ inline bool kv8_view(const Q3tKv8Cache* c, Kv8View* view) {
     const uintptr_t scales_at = reinterpret_cast<uintptr_t>(c->key_scales) | reinterpret_cast<uintptr_t>(c->value_scales);
     return view->page_stride >= page_bytes && view->page_stride % 16 == 0 && view->scale_stride >= c->key_value_heads && at % 16 == 0
            && scales_at % sizeof(float) == 0;
+}
+
+// Dynamic shared memory past what a kernel gets unasked; once a device (a bit each of `done`), and not an operation of a stream, so
+// that a launch may be captured without one before it
+template <class Kernel>
+inline cudaError_t kv8_allow_smem(std::atomic<unsigned long long>& done, Kernel* kernel, int bytes) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    const unsigned long long bit = 1ull << (device & 63);
+    if (e != cudaSuccess || (done.load(std::memory_order_acquire) & bit) != 0) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
 }
 
 // two e4m3 codes (the low 16 bits) as fp16, exact

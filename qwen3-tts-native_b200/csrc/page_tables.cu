@@ -10,10 +10,9 @@
 // a new token that are written.  Every CTA repeats the sums, which are cheap beside a second launch; a barrier over the
 // cluster separates the last read of lengths and free_count from the first write of what may be the same memory.
 
+#include "kv8.cuh"
 #include "q3t_kernels.cuh"
-#include "q3t_ops.h"
 
-#include <atomic>
 #include <climits>
 
 namespace q3t {
@@ -38,10 +37,6 @@ struct TableArgs {
     int* positions;
     long long* slots;
     int rows, stride, pages, capacity;
-};
-
-struct Sums {
-    long long asked, need, given;
 };
 
 // exclusive prefix sums over the threads of the block; `total` gets the sums over all of them
@@ -258,20 +253,9 @@ extern "C" int32_t q3t_launch_page_tables(const Q3tPageTablesDesc* d, void* stre
         || d->pages < 1 || d->token_capacity < 0 || d->reserved != 0) {
         return cudaErrorInvalidValue;
     }
-    // (shared memory past 48 KB: 4 * 4096 rows * 4 bytes; asked for once a device)
     const size_t smem = (size_t)d->rows * 4 * sizeof(int);
-    if (smem > 32 * 1024) {
-        static std::atomic<unsigned long long> done{0};
-        int device = 0;
-        cudaError_t e = cudaGetDevice(&device);
-        if (e != cudaSuccess) return e;
-        const unsigned long long bit = 1ull << (device & 63);
-        if ((done.load(std::memory_order_acquire) & bit) == 0) {
-            e = cudaFuncSetAttribute(page_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Q3T_MAX_TABLE_ROWS * 4 * (int)sizeof(int));
-            if (e != cudaSuccess) return e;
-            done.fetch_or(bit, std::memory_order_release);
-        }
-    }
+    static std::atomic<unsigned long long> allowed{0};
+    if (const cudaError_t e = kv8_allow_smem(allowed, page_tables_kernel, Q3T_MAX_TABLE_ROWS * 4 * (int)sizeof(int))) return e;
     TableArgs a;
     a.lengths = d->lengths; a.changes = d->changes; a.new_lengths = d->new_lengths; a.table = d->page_table;
     a.stack = d->free_pages; a.free_count = d->free_count; a.new_free_count = d->new_free_count; a.status = d->status;
