@@ -11,9 +11,10 @@
 // maximum until a score exceeds it by 2^8, so that outputs are rescaled almost never; weights are kept 2^6 times larger than that
 // needs, which leaves fp16 its 11 bits down to 2^-20 of the largest.
 //
-// The batch's work, groups of 8 pages (one a warp) of every (row, KV head, 8 columns), is cut into as many equal ranges as there are
-// CTAs, wherever that falls.  A CTA merges its warps in shared memory; of what is cut every CTA leaves (reference, sum, output)
-// and the one with the last ticket folds them in order, so a result depends on the batch's lengths, not on timing.
+// The batch's work, the pages of every (row, KV head, 8 columns), is cut into as many equal ranges as there are warps, wherever
+// that falls.  A warp writes what it has whole; what is cut is merged by the CTA in shared memory, and of what its range cuts
+// the CTA leaves (reference, sum, output) and the one with the last ticket folds them in order, so a result depends on
+// the batch's lengths, not on timing.
 
 #include "kv8.cuh"
 #include "q3t_kernels.cuh"
@@ -24,7 +25,7 @@ namespace q3t {
 namespace {
 
 constexpr int kRowThreads = 256;
-constexpr int kRowWarps = kRowThreads / kWarp;         // = pages of a group
+constexpr int kRowWarps = kRowThreads / kWarp;
 constexpr int kRowCtas = 2 * 148;
 constexpr int kColumns = 8;
 constexpr float kSlack = 8.0f;                         // log2 of how far a score may exceed its column's reference
@@ -59,6 +60,11 @@ __device__ __forceinline__ float exp2_ftz(float x) {
 __device__ __forceinline__ float log2_fast(float x) {
     float r;
     asm("lg2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float reciprocal_fast(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
@@ -102,20 +108,46 @@ __device__ __forceinline__ int4 load16(const uint8_t* p) {
     return v;
 }
 
+__device__ __forceinline__ void add8(float (&v)[8], float f, const float4& lo, const float4& hi) {
+    v[0] = fmaf(f, lo.x, v[0]);
+    v[1] = fmaf(f, lo.y, v[1]);
+    v[2] = fmaf(f, lo.z, v[2]);
+    v[3] = fmaf(f, lo.w, v[3]);
+    v[4] = fmaf(f, hi.x, v[4]);
+    v[5] = fmaf(f, hi.y, v[5]);
+    v[6] = fmaf(f, hi.z, v[6]);
+    v[7] = fmaf(f, hi.w, v[7]);
+}
+
 // What a row asks of the kernel
 struct RowWork {
     RowSpan span;
     int last;          // tokens that some new token of the row sees
     int blocks;        // of 8 columns
-    int groups;        // of 8 pages, at least one: rows that see nothing have zeros to write
+    int pages;         // at least one: rows that see nothing have zeros to write
 };
 __device__ __forceinline__ RowWork row_work(const Kv8AttentionArgs& a, int row, int group) {
     RowWork w;
     w.span = row_span(a.starts, a.lengths, row, a.tokens, a.most, a.max_sequence);
     w.last = min(max(w.span.base + w.span.count, 0), a.max_sequence);
     w.blocks = (w.span.count * group + kColumns - 1) / kColumns;
-    w.groups = max(1, (w.last + kRowWarps * kPageTokens - 1) / (kRowWarps * kPageTokens));
+    w.pages = max(1, (w.last + kPageTokens - 1) / kPageTokens);
     return w;
+}
+
+// A part of a segment, (row, KV head, 8 columns): whose it is
+struct Piece {
+    long long start;   // first unit of the segment, -1: none
+    int pages;         // of the segment
+    int first;         // number of the row's first new token
+    int kv_head;
+    int column;        // of the row and KV head: the segment's first
+    int columns;       // of the segment
+};
+
+template <int HD>
+constexpr size_t rows_smem(int rows) {
+    return (size_t)rows * sizeof(long long) + (size_t)2 * kRowWarps * kColumns * (HD + 4) * sizeof(float);
 }
 
 template <int HD, bool E4M3>
@@ -123,25 +155,27 @@ __global__ void __launch_bounds__(kRowThreads, 2) kv8_rows_kernel(const Kv8Atten
     constexpr int kParts = HD / 64;                    // 16-byte pieces of a key that a lane holds
     constexpr int kTiles = HD / 16;                    // of 16 dims
     constexpr int kWords = HD / 32;                    // of a value's dims that a lane holds
-    constexpr int kPitch = HD + 4;
-    extern __shared__ long long before[];              // [rows]: units of the rows up to each
-    __shared__ float part[kRowWarps][kColumns][kPitch];
-    __shared__ float tops[kRowWarps][kColumns], totals[kRowWarps][kColumns];
-    __shared__ float fold_scale[kRowCtas][kColumns];
+    constexpr int kPitch = HD + 4;                     // of a column of a piece: its output, then top and sum
+    constexpr int kPiece = kColumns * kPitch;
+    extern __shared__ __align__(16) unsigned char smem[];
+    float* const parts = reinterpret_cast<float*>(smem);                                    // [warp][2] pieces
+    long long* const before = reinterpret_cast<long long*>(parts + 2 * kRowWarps * kPiece);  // [rows]: units of the rows up to each
+    __shared__ Piece held[2 * kRowWarps];
+    __shared__ float fold_scale[2][kRowCtas][kColumns];
     __shared__ long long scan[kRowWarps];
-    __shared__ int ticket;
+    __shared__ int beyond[2], tickets[2];              // segments that go beyond the CTA at its start and its end
     const int tid = threadIdx.x, lane = tid % kWarp, warp = __shfl_sync(0xffffffffu, tid / kWarp, 0);
     const int g = lane >> 2, q4 = lane & 3;
     const int heads = a.cache.heads, group = a.query_heads / heads;
 
-    // ---- the batch's units, as prefix sums over the rows; the first CTA counts what lies outside the host's bounds
+    // ---- the batch's units (pages of a segment), as prefix sums over the rows; the first CTA counts what lies outside the host's bounds
     long long sum = 0;
     for (int first = 0; first < a.rows; first += kRowThreads) {
         const int row = first + tid;
         long long mine = 0;
         if (row < a.rows) {
             const RowWork w = row_work(a, row, group);
-            mine = (long long)w.blocks * heads * w.groups;
+            mine = (long long)w.blocks * heads * w.pages;
             if (w.span.cut && blockIdx.x == 0) atomicAdd(&g_kv8_range_errors, 1u);
         }
 #pragma unroll
@@ -157,10 +191,11 @@ __global__ void __launch_bounds__(kRowThreads, 2) kv8_rows_kernel(const Kv8Atten
         __syncthreads();
     }
     const long long units = sum;
-    const int ctas = (int)min((long long)gridDim.x, units);
+    const int ctas = (int)min((long long)gridDim.x, (units + kRowWarps - 1) / kRowWarps);
     if ((int)blockIdx.x >= ctas) return;
-    long long unit = units * blockIdx.x / ctas;
-    const long long unit_first = unit, unit_end = units * (blockIdx.x + 1) / ctas;
+    const long long cta_first = units * blockIdx.x / ctas, cta_end = units * (blockIdx.x + 1) / ctas;
+    long long unit = cta_first + (cta_end - cta_first) * warp / kRowWarps;
+    const long long unit_end = cta_first + (cta_end - cta_first) * (warp + 1) / kRowWarps;
     int row;
     {
         int low = 0, high = a.rows - 1;
@@ -171,72 +206,59 @@ __global__ void __launch_bounds__(kRowThreads, 2) kv8_rows_kernel(const Kv8Atten
         }
         row = low;
     }
+    // 8 dims of a column
+    auto write8 = [&](int first, int kv_head, int column, int d, const float (&v)[8]) {
+        const int i = column / group;
+        const size_t token = first + i, at = (size_t)(kv_head * group + column - i * group) * HD + d;
+        __nv_bfloat162 x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+        *reinterpret_cast<int4*>(a.out + token * a.out_stride + at) = *reinterpret_cast<const int4*>(x);
+        if (a.out32 != nullptr) {
+            float* const to = a.out32 + token * a.query_heads * HD + at;
+            *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4*>(to + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        }
+    };
+    if (tid < 2) beyond[tid] = -1;
+    if (lane < 2) held[2 * warp + lane].start = -1;
+    __syncwarp();
 
-    bool waited = false;
+    int pieces_held = 0;
     while (unit < unit_end) {
         while (before[row] <= unit) ++row;
         const RowWork w = row_work(a, row, group);
-        const long long in_row = unit - (row > 0 ? before[row - 1] : 0);
-        const int segment = (int)(in_row / w.groups);              // (KV head, block of columns)
-        const int group_first = (int)(in_row - (long long)segment * w.groups);
-        const int group_end = (int)min((long long)w.groups, group_first + (unit_end - unit));
+        const long long row_first = row > 0 ? before[row - 1] : 0;
+        const int segment = (int)((unit - row_first) / w.pages);              // (KV head, block of columns)
+        const long long start = row_first + (long long)segment * w.pages;
+        const int page_first = (int)(unit - start);
+        const int page_end = (int)min((long long)w.pages, page_first + (unit_end - unit));
         const int kv_head = segment / w.blocks, block = segment - kv_head * w.blocks;
         const int columns = min(kColumns, w.span.count * group - block * kColumns);
+
+        // ---- pages: their ids a lane each, 32 at a time (one that is not there is read as page 0 and masked)
+        const int* const ids_at = a.table + (size_t)row * a.table_stride;
+        auto usable = [&](int id) { return id >= 0 && id < a.cache.pages; };
+        auto ids_from = [&](int first) { return first + lane < page_end && (first + lane) * kPageTokens < w.last ? ids_at[first + lane] : -1; };
+        int ids = ids_from(page_first);
 
         // ---- queries: this lane's column and dims, to fp16 by a power of two that brings the largest to 2^7..2^8
         uint32_t qf[kParts][4][2];
         float column_scale;
         int column_seen;
+        int4 raw[kParts][2];
         {
             const int column = block * kColumns + g;
             const bool real = g < columns;
             const int i = real ? column / group : 0;
             const bf16* q = a.query + (size_t)(w.span.first + i) * a.query_stride + (size_t)(kv_head * group + column % group) * HD + q4 * 16;
-            int4 raw[kParts][2];
-            uint32_t most = 0u;
 #pragma unroll
             for (int j = 0; j < kParts; ++j) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    raw[j][h] = real ? *reinterpret_cast<const int4*>(q + 64 * j + 8 * h) : make_int4(0, 0, 0, 0);
-                    const uint32_t x[4] = {(uint32_t)raw[j][h].x, (uint32_t)raw[j][h].y, (uint32_t)raw[j][h].z, (uint32_t)raw[j][h].w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) most = __vmaxu2(most, x[e] & 0x7fff7fffu);
-                }
+                for (int h = 0; h < 2; ++h) raw[j][h] = real ? *reinterpret_cast<const int4*>(q + 64 * j + 8 * h) : make_int4(0, 0, 0, 0);
             }
-            most = max(most & 0xffffu, most >> 16);
-            most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-            most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-            const int shift = min(134 - (int)min(most >> 7, 254u), 127);
-            const float up = ldexpf(1.0f, shift);
-            column_scale = ldexpf(a.scale * 1.4426950408889634f, -shift);
             column_seen = real ? min(max(w.span.base + i + 1, 0), a.max_sequence) : 0;
-#pragma unroll
-            for (int j = 0; j < kParts; ++j) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t x[4] = {(uint32_t)raw[j][h].x, (uint32_t)raw[j][h].y, (uint32_t)raw[j][h].z, (uint32_t)raw[j][h].w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) qf[j][2 * h + e / 2][e & 1] = pack_half2(bf_lo(x[e]) * up, bf_hi(x[e]) * up);
-                }
-            }
         }
-        // of the columns whose scores this lane gets
-        const float scale0 = __shfl_sync(0xffffffffu, column_scale, 8 * q4), scale1 = __shfl_sync(0xffffffffu, column_scale, 8 * q4 + 4);
-        const int seen0 = __shfl_sync(0xffffffffu, column_seen, 8 * q4), seen1 = __shfl_sync(0xffffffffu, column_seen, 8 * q4 + 4);
-
-        float o[kTiles][4];
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.0f;
-        float top0 = -INFINITY, top1 = -INFINITY, sum0 = 0.0f, sum1 = 0.0f;
-
-        // ---- this warp's pages: 8 g + warp; their ids a lane each, 32 at a time
-        const int* const ids_at = a.table + (size_t)row * a.table_stride + warp;
-        const int pages_end = (w.last + kPageTokens - 1) / kPageTokens;
-        auto ids_from = [&](int first) {
-            const int page = (first + lane) * kRowWarps + warp;
-            return first + lane < group_end && page < pages_end ? ids_at[(size_t)(first + lane) * kRowWarps] : -1;
-        };
         int4 kr[kParts][2], vr[4];
         float key_scale, value_scale;
         const size_t k_offset = (size_t)kv_head * (kPageTokens * HD) + g * HD + q4 * 16;
@@ -265,25 +287,53 @@ __global__ void __launch_bounds__(kRowThreads, 2) kv8_rows_kernel(const Kv8Atten
             }
             value_scale = a.cache.v_scales[(long long)id * a.cache.scale_stride + kv_head];
         };
-        int ids = ids_from(group_first);
         int raw_id = __shfl_sync(0xffffffffu, ids, 0);
-        // (a page that is not there is read as page 0 and masked)
-        auto usable = [&](int id) { return id >= 0 && id < a.cache.pages; };
-        const bool any = group_first * kRowWarps + warp < pages_end;
-        if (any) {
-            load_keys(usable(raw_id) ? raw_id : 0);
-            load_values(usable(raw_id) ? raw_id : 0);
+        load_keys(usable(raw_id) ? raw_id : 0);
+        load_values(usable(raw_id) ? raw_id : 0);
+        {
+            uint32_t most = 0u;
+#pragma unroll
+            for (int j = 0; j < kParts; ++j) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t x[4] = {(uint32_t)raw[j][h].x, (uint32_t)raw[j][h].y, (uint32_t)raw[j][h].z, (uint32_t)raw[j][h].w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) most = __vmaxu2(most, x[e] & 0x7fff7fffu);
+                }
+            }
+            most = max(most & 0xffffu, most >> 16);
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            const int shift = min(134 - (int)min(most >> 7, 254u), 127);
+            const float up = ldexpf(1.0f, shift);
+            column_scale = ldexpf(a.scale * 1.4426950408889634f, -shift);
+#pragma unroll
+            for (int j = 0; j < kParts; ++j) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t x[4] = {(uint32_t)raw[j][h].x, (uint32_t)raw[j][h].y, (uint32_t)raw[j][h].z, (uint32_t)raw[j][h].w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) qf[j][2 * h + e / 2][e & 1] = pack_half2(bf_lo(x[e]) * up, bf_hi(x[e]) * up);
+                }
+            }
         }
-        for (int gr = group_first; gr < group_end; ++gr) {
-            const int page = gr * kRowWarps + warp;
-            if (page >= pages_end) break;
+        // of the columns whose scores this lane gets
+        const float scale0 = __shfl_sync(0xffffffffu, column_scale, 8 * q4), scale1 = __shfl_sync(0xffffffffu, column_scale, 8 * q4 + 4);
+        const int seen0 = __shfl_sync(0xffffffffu, column_seen, 8 * q4), seen1 = __shfl_sync(0xffffffffu, column_seen, 8 * q4 + 4);
+
+        float o[kTiles][4];
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.0f;
+        float top0 = -INFINITY, top1 = -INFINITY, sum0 = 0.0f, sum1 = 0.0f;
+
+        for (int page = page_first; page < page_end; ++page) {
             const bool there = usable(raw_id);
-            if (!there && segment == 0 && lane == 0) atomicAdd(&g_kv8_page_errors, 1u);
-            const int next = gr + 1 - group_first;
-            if ((next & 31) == 0) ids = ids_from(gr + 1);
+            if (!there && segment == 0 && lane == 0 && page * kPageTokens < w.last) atomicAdd(&g_kv8_page_errors, 1u);
+            const int next = page + 1 - page_first;
+            if ((next & 31) == 0) ids = ids_from(page + 1);
             const int next_raw = __shfl_sync(0xffffffffu, ids, next & 31);
             const int next_id = usable(next_raw) ? next_raw : 0;
-            const bool more = gr + 1 < group_end && page + kRowWarps < pages_end;
+            const bool more = page + 1 < page_end;
 
             // ---- scores
             float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -332,7 +382,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) kv8_rows_kernel(const Kv8Atten
             // (nothing but -inf so far: weights of zero)
             const float r0 = top0 == -INFINITY ? 0.0f : top0 - kLift, r1 = top1 == -INFINITY ? 0.0f : top1 - kLift;
             const float w0 = exp2_ftz(s[0] - r0), w1 = exp2_ftz(s[1] - r1), w2 = exp2_ftz(s[2] - r0), w3 = exp2_ftz(s[3] - r1);
-            const float inverse = __frcp_rn(vs);
+            const float inverse = reciprocal_fast(vs);
             sum0 = fmaf(w0 + w2, inverse, sum0);
             sum1 = fmaf(w1 + w3, inverse, sum1);
             const uint32_t b0 = transpose8(pack_half2(w0, w1)), b1 = transpose8(pack_half2(w2, w3));
@@ -359,111 +409,170 @@ __global__ void __launch_bounds__(kRowThreads, 2) kv8_rows_kernel(const Kv8Atten
             if (more) load_values(next_id);
             raw_id = next_raw;
         }
-
-        // ---- the CTA's warps together
 #pragma unroll
         for (int x = 4; x < kWarp; x <<= 1) {
             sum0 += __shfl_xor_sync(0xffffffffu, sum0, x);
             sum1 += __shfl_xor_sync(0xffffffffu, sum1, x);
         }
+        // ---- whole: written; cut: into shared memory
+        const bool whole = page_first == 0 && page_end == w.pages;
+        float* const piece = parts + (size_t)(2 * warp + pieces_held) * kPiece;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            if (2 * q4 + c < columns) {
-                float* const at = &part[warp][2 * q4 + c][g * (HD / 8)];
+            if (2 * q4 + c >= columns) continue;
+            if (whole) {
+                const float total = c == 0 ? sum0 : sum1, inverse = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+                for (int t = 0; t < kTiles; t += 4) {
+                    const float v[8] = {o[t][c] * inverse, o[t][c + 2] * inverse, o[t + 1][c] * inverse, o[t + 1][c + 2] * inverse,
+                                        o[t + 2][c] * inverse, o[t + 2][c + 2] * inverse, o[t + 3][c] * inverse, o[t + 3][c + 2] * inverse};
+                    write8(w.span.first, kv_head, block * kColumns + 2 * q4 + c, g * (HD / 8) + 2 * t, v);
+                }
+            } else {
+                float* const at = piece + (2 * q4 + c) * kPitch;
 #pragma unroll
                 for (int t = 0; t < kTiles; t += 2) {
-                    *reinterpret_cast<float4*>(at + 2 * t) = make_float4(o[t][c], o[t][c + 2], o[t + 1][c], o[t + 1][c + 2]);
+                    *reinterpret_cast<float4*>(at + g * (HD / 8) + 2 * t) = make_float4(o[t][c], o[t][c + 2], o[t + 1][c], o[t + 1][c + 2]);
                 }
-            }
-        }
-        if (g == 0) {
-            tops[warp][2 * q4] = top0;
-            tops[warp][2 * q4 + 1] = top1;
-            totals[warp][2 * q4] = sum0;
-            totals[warp][2 * q4 + 1] = sum1;
-        }
-        __syncthreads();
-        const bool whole = group_first == 0 && group_end == w.groups;
-        float* const pieces = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + kCounterBytes);
-        constexpr int kPiece = kColumns * (HD + 2);                // [column][HD], then tops, then sums
-        float* const piece = pieces + (size_t)(2 * blockIdx.x + (unit == unit_first ? 0 : 1)) * kPiece;
-        auto write = [&](int column, int d, float value) {
-            const int c = block * kColumns + column, i = c / group;
-            const size_t token = w.span.first + i, at = (size_t)(kv_head * group + c % group) * HD + d;
-            a.out[token * a.out_stride + at] = f2bf(value);
-            if (a.out32 != nullptr) a.out32[token * a.query_heads * HD + at] = value;
-        };
-        for (int x = tid; x < columns * HD; x += kRowThreads) {
-            const int column = x / HD, d = x % HD;
-            float top = tops[0][column], total = 0.0f, value = 0.0f;
-#pragma unroll
-            for (int v = 1; v < kRowWarps; ++v) top = fmaxf(top, tops[v][column]);
-#pragma unroll
-            for (int v = 0; v < kRowWarps; ++v) {
-                const float f = tops[v][column] == -INFINITY ? 0.0f : exp2_ftz(tops[v][column] - top);
-                total += f * totals[v][column];
-                value += f * part[v][column][d];
-            }
-            if (whole) {
-                write(column, d, total == 0.0f ? 0.0f : value / total);
-            } else {
-                piece[column * HD + d] = value;
-                if (d == 0) {
-                    piece[kColumns * HD + column] = top;
-                    piece[kColumns * (HD + 1) + column] = total;
+                if (g == 0) {
+                    at[HD] = c == 0 ? top0 : top1;
+                    at[HD + 1] = c == 0 ? sum0 : sum1;
                 }
             }
         }
         if (!whole) {
-            // ---- of the CTAs that share the segment the last one folds what they left
-            const long long start = unit - group_first, end = start + w.groups - 1;
-            auto owner = [&](long long u) { return (int)(((u + 1) * ctas - 1) / units); };
-            const int first_cta = owner(start), last_cta = owner(end), count = last_cta - first_cta + 1;
-            if (!waited) {
-                pdl_wait();                                        // the counters are zero
-                waited = true;
+            if (lane == 0) held[2 * warp + pieces_held] = Piece{start, w.pages, w.span.first, kv_head, block * kColumns, columns};
+            ++pieces_held;
+        }
+        unit += page_end - page_first;
+    }
+    __syncthreads();
+
+    // ---- pieces of a segment that lie in this CTA stand in order; a warp a segment merges them
+    float* const left = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + kCounterBytes);
+    auto left_by = [&](int cta, int which) { return left + (size_t)(2 * cta + which) * kPiece; };
+    {
+        const long long mine = lane < 2 * kRowWarps ? held[lane].start : -1;
+        const unsigned int real = __ballot_sync(0xffffffffu, mine >= 0);
+        const unsigned int lower = real & ((1u << lane) - 1u);
+        const long long previous = __shfl_sync(0xffffffffu, mine, lower != 0u ? 31 - __clz(lower) : 0);
+        unsigned int leads = __ballot_sync(0xffffffffu, mine >= 0 && (lower == 0u || previous != mine));
+        for (int n = 0; leads != 0u; ++n) {
+            const int first = __ffs(leads) - 1;
+            leads &= leads - 1;
+            if (n % kRowWarps != warp) continue;
+            const unsigned int parts_here = real & ~((1u << first) - 1u) & (leads != 0u ? (leads & -leads) - 1u : ~0u);
+            const Piece p = held[first];
+            const bool whole = p.start >= cta_first && p.start + p.pages <= cta_end;
+            const int which = p.start < cta_first ? 0 : 1;
+            float* const to = left_by(blockIdx.x, which);
+            for (int x = lane; x < p.columns * (HD / 8); x += kWarp) {
+                const int column = x / (HD / 8), d = x % (HD / 8) * 8;
+                const float* const at = parts + column * kPitch;
+                float top = -INFINITY, total = 0.0f, v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+                for (unsigned int left_over = parts_here; left_over != 0u; left_over &= left_over - 1) {
+                    top = fmaxf(top, at[(__ffs(left_over) - 1) * kPiece + HD]);
+                }
+                for (unsigned int left_over = parts_here; left_over != 0u; left_over &= left_over - 1) {
+                    const float* const from = at + (__ffs(left_over) - 1) * kPiece;
+                    const float f = from[HD] == -INFINITY ? 0.0f : exp2_ftz(from[HD] - top);
+                    total = fmaf(f, from[HD + 1], total);
+                    const float4 lo = *reinterpret_cast<const float4*>(from + d), hi = *reinterpret_cast<const float4*>(from + d + 4);
+                    add8(v, f, lo, hi);
+                }
+                if (whole) {
+                    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] *= inverse;
+                    write8(p.first, p.kv_head, p.column + column, d, v);
+                } else {
+                    *reinterpret_cast<float4*>(to + column * kPitch + d) = make_float4(v[0], v[1], v[2], v[3]);
+                    *reinterpret_cast<float4*>(to + column * kPitch + d + 4) = make_float4(v[4], v[5], v[6], v[7]);
+                    if (d == 0) *reinterpret_cast<float2*>(to + column * kPitch + HD) = make_float2(top, total);
+                }
             }
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) ticket = (int)atomicAdd(static_cast<unsigned int*>(a.scratch) + first_cta, 1u);
-            __syncthreads();
-            if (ticket == count - 1) {
+            if (!whole) {
                 __threadfence();
-                // the first CTA's range may begin before the segment: its second piece then
-                const int lead = units * first_cta / ctas == start ? 0 : 1;
-                auto piece_of = [&](int n) { return pieces + (size_t)(2 * (first_cta + n) + (n == 0 ? lead : 0)) * kPiece; };
-                for (int x = tid; x < count * kColumns; x += kRowThreads) {
-                    if (x % kColumns < columns) fold_scale[x / kColumns][x % kColumns] = __ldcg(piece_of(x / kColumns) + kColumns * HD + x % kColumns);
-                }
-                __syncthreads();
-                for (int x = tid; x < columns * HD; x += kRowThreads) {
-                    const int column = x / HD, d = x % HD;
-                    float top = -INFINITY, total = 0.0f, value = 0.0f;
-                    for (int n = 0; n < count; ++n) top = fmaxf(top, fold_scale[n][column]);
-#pragma unroll 4
-                    for (int n = 0; n < count; ++n) {
-                        const float f = fold_scale[n][column] == -INFINITY ? 0.0f : exp2_ftz(fold_scale[n][column] - top);
-                        total += f * __ldcg(piece_of(n) + kColumns * (HD + 1) + column);
-                        value += f * __ldcg(piece_of(n) + column * HD + d);
-                    }
-                    write(column, d, total == 0.0f ? 0.0f : value / total);
-                }
+                if (lane == 0) beyond[which] = first;
             }
         }
-        __syncthreads();
-        unit += group_end - group_first;
     }
-    if (!waited) pdl_wait();
+    pdl_wait();                                            // the counters are zero
+    __syncthreads();
+    if (beyond[0] < 0 && beyond[1] < 0) {
+        pdl_trigger();
+        return;
+    }
+    // ---- of the CTAs that share a segment the last one folds what they left: half of the CTA for each of the two
+    constexpr int kHalf = kRowWarps / 2;
+    const int which = warp / kHalf, in_half = tid % (kRowThreads / 2);
+    const Piece p = held[max(beyond[which], 0)];
+    auto owner = [&](long long u) { return (int)(((u + 1) * ctas - 1) / units); };
+    const int first_cta = owner(p.start), count = owner(p.start + p.pages - 1) - first_cta + 1;
+    if (in_half == 0) tickets[which] = beyond[which] >= 0 ? (int)atomicAdd(static_cast<unsigned int*>(a.scratch) + first_cta, 1u) : -1;
+    __syncthreads();
+    const bool folds[2] = {tickets[0] >= 0, tickets[1] >= 0};
+    const bool mine = folds[which] && tickets[which] == count - 1;
+    if (!__syncthreads_or(mine)) {
+        pdl_trigger();
+        return;
+    }
+    __threadfence();
+    // the segment begins in the first CTA's range, whose second piece it is
+    auto piece_of = [&](int n) { return left_by(first_cta + n, n == 0 ? 1 : 0); };
+    if (mine) {
+        for (int x = in_half; x < count * p.columns; x += kRowThreads / 2) {
+            fold_scale[which][x / p.columns][x % p.columns] = __ldcg(piece_of(x / p.columns) + x % p.columns * kPitch + HD);
+        }
+    }
+    __syncthreads();
+    const int share = warp % kHalf;                        // pieces share, share + kHalf, ...
+    if (mine) {
+        for (int x = lane; x < p.columns * (HD / 8); x += kWarp) {
+            const int column = x / (HD / 8), d = x % (HD / 8) * 8;
+            float top = -INFINITY, total = 0.0f, v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+            for (int n = 0; n < count; ++n) top = fmaxf(top, fold_scale[which][n][column]);
+#pragma unroll 4
+            for (int n = share; n < count; n += kHalf) {
+                const float* const from = piece_of(n) + column * kPitch;
+                const float piece_top = fold_scale[which][n][column], f = piece_top == -INFINITY ? 0.0f : exp2_ftz(piece_top - top);
+                const float4 lo = __ldcg(reinterpret_cast<const float4*>(from + d)), hi = __ldcg(reinterpret_cast<const float4*>(from + d + 4));
+                total = fmaf(f, __ldcg(from + HD + 1), total);
+                add8(v, f, lo, hi);
+            }
+            float* const to = parts + (size_t)warp * kPiece + column * kPitch;
+            *reinterpret_cast<float4*>(to + d) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4*>(to + d + 4) = make_float4(v[4], v[5], v[6], v[7]);
+            if (d == 0) to[HD] = total;
+        }
+    }
+    __syncthreads();
+    if (mine) {
+        for (int x = in_half; x < p.columns * (HD / 8); x += kRowThreads / 2) {
+            const int column = x / (HD / 8), d = x % (HD / 8) * 8;
+            float total = 0.0f, v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int n = 0; n < kHalf; ++n) {
+                const float* const from = parts + (size_t)(which * kHalf + n) * kPiece + column * kPitch;
+                total += from[HD];
+                add8(v, 1.0f, *reinterpret_cast<const float4*>(from + d), *reinterpret_cast<const float4*>(from + d + 4));
+            }
+            const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= inverse;
+            write8(p.first, p.kv_head, p.column + column, d, v);
+        }
+    }
     pdl_trigger();
 }
 
 template <int HD, bool E4M3>
 cudaError_t launch_rows(const Kv8AttentionArgs& a, cudaStream_t stream) {
     static std::atomic<unsigned long long> allowed{0};
-    cudaError_t e = kv8_allow_smem(allowed, kv8_rows_kernel<HD, E4M3>, Q3T_MAX_TABLE_ROWS * (int)sizeof(long long));
+    cudaError_t e = kv8_allow_smem(allowed, kv8_rows_kernel<HD, E4M3>, (int)rows_smem<HD>(Q3T_MAX_TABLE_ROWS));
     if (e == cudaSuccess) e = launch_zero_counters(static_cast<unsigned int*>(a.scratch), kRowCtas, stream);
     if (e != cudaSuccess) return e;
-    return launch_pdl(kv8_rows_kernel<HD, E4M3>, dim3(kRowCtas), dim3(kRowThreads), (size_t)a.rows * sizeof(long long), stream, a);
+    return launch_pdl(kv8_rows_kernel<HD, E4M3>, dim3(kRowCtas), dim3(kRowThreads), rows_smem<HD>(a.rows), stream, a);
 }
 
 // false: refused
@@ -519,7 +628,7 @@ extern "C" uint32_t q3t_kv8_page_error_count(void) {
 extern "C" size_t q3t_kv8_attention_scratch_bytes(const Q3tKv8AttentionDesc* desc) {
     q3t::Kv8AttentionArgs a;
     if (!q3t::attention_args(desc, &a)) return 0;
-    return q3t::kCounterBytes + (size_t)q3t::kRowCtas * 2 * q3t::kColumns * (desc->cache->head_dimension + 2) * sizeof(float);
+    return q3t::kCounterBytes + (size_t)q3t::kRowCtas * 2 * q3t::kColumns * (desc->cache->head_dimension + 4) * sizeof(float);
 }
 
 extern "C" int32_t q3t_launch_kv8_attention(const Q3tKv8AttentionDesc* desc, void* stream) {
