@@ -99,4 +99,65 @@ __device__ __forceinline__ RowSpan row_span(const int* starts, const int* length
     return s;
 }
 
+// ---- attention (kv8_attention.cu, kv8_prompt.cu)
+
+constexpr float kKv8Slack = 8.0f;         // log2 of how far a score may exceed its row's reference
+constexpr float kKv8Lift = 6.0f;          // log2 of the weight at the reference
+constexpr int kKv8RowColumns = 64;        // (new tokens x query heads of a KV head) of a row up to which kv8_attention.cu takes it
+
+struct Kv8AttentionArgs {
+    Kv8View cache;
+    const bf16* query;
+    bf16* out;
+    float* out32;
+    const int* table;
+    const int* lengths;
+    const int* starts;
+    int table_stride;
+    int rows;
+    int query_heads;
+    int query_stride, out_stride;
+    int tokens, most, max_sequence;
+    float scale;
+    void* scratch;
+    int prompts;              // a launch of kv8_prompt.cu follows
+};
+
+__device__ __forceinline__ float exp2_ftz(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float log2_fast(float x) {
+    float r;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float reciprocal_fast(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// four codes as two pairs of fp16
+template <bool E4M3>
+__device__ __forceinline__ void codes_to_half(uint32_t word, uint32_t& lo, uint32_t& hi) {
+    if (E4M3) {
+        lo = e4m3_to_half2(word);
+        hi = e4m3_to_half2(word >> 16);
+    } else {
+        // the byte behind 0x64 is 1024 + it as fp16, with its sign bit turned over 1152 + the code
+        const uint32_t biased = word ^ 0x80808080u;
+        const __half2 offset = __half2half2(__ushort_as_half(0x6480));
+        const uint32_t a = __byte_perm(biased, 0x64646464u, 0x4140), b = __byte_perm(biased, 0x64646464u, 0x4342);
+        const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), offset), y = __hsub2(*reinterpret_cast<const __half2*>(&b), offset);
+        lo = *reinterpret_cast<const uint32_t*>(&x);
+        hi = *reinterpret_cast<const uint32_t*>(&y);
+    }
+}
+
 }  // namespace q3t

@@ -1,4 +1,4 @@
-// Causal attention over an 8-bit paged cache (q3t_launch_kv8_attention): few new tokens a row.
+// Causal attention over an 8-bit paged cache (q3t_launch_kv8_attention): rows of few new tokens.  kv8_prompt.cu has the others.
 //
 // out = sum_j p_j v_j / sum_j p_j, p_j = exp(scale * q . k_j - max), over the positions up to the token's own; k_j and v_j are codes times the
 // scale of their page and head.  A (new token, query head) of a KV head is a column; a warp takes pages of 16 tokens for 8 columns:
@@ -22,56 +22,20 @@
 #include <climits>
 
 namespace q3t {
+
+cudaError_t launch_kv8_prompts(const Kv8AttentionArgs& a, int head_dim, bool e4m3, cudaStream_t stream);      // kv8_prompt.cu
+
 namespace {
 
 constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / kWarp;
 constexpr int kRowCtas = 2 * 148;
 constexpr int kColumns = 8;
-constexpr float kSlack = 8.0f;                         // log2 of how far a score may exceed its column's reference
-constexpr float kLift = 6.0f;                          // log2 of the weight at the reference
 constexpr int kCounterBytes = (kRowCtas * 4 + 255) / 256 * 256;
 
 __device__ unsigned int g_kv8_range_errors = 0;
 __device__ unsigned int g_kv8_page_errors = 0;
 
-struct Kv8AttentionArgs {
-    Kv8View cache;
-    const bf16* query;
-    bf16* out;
-    float* out32;
-    const int* table;
-    const int* lengths;
-    const int* starts;
-    int table_stride;
-    int rows;
-    int query_heads;
-    int query_stride, out_stride;
-    int tokens, most, max_sequence;
-    float scale;
-    void* scratch;
-};
-
-__device__ __forceinline__ float exp2_ftz(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-__device__ __forceinline__ float log2_fast(float x) {
-    float r;
-    asm("lg2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-__device__ __forceinline__ float reciprocal_fast(float x) {
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
 // D += A (16 x 16, fp16) * B (16 x 8); fragments as in attention.cu
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -80,28 +44,11 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // an 8 x 8 tile of fp16 across the warp, rows for columns
-__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+__device__ __forceinline__ uint32_t transposkv8_allow_smem(uint32_t x) {
     uint32_t r;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
     return r;
 }
-// four codes as two pairs of fp16
-template <bool E4M3>
-__device__ __forceinline__ void codes_to_half(uint32_t word, uint32_t& lo, uint32_t& hi) {
-    if (E4M3) {
-        lo = e4m3_to_half2(word);
-        hi = e4m3_to_half2(word >> 16);
-    } else {
-        // the byte behind 0x64 is 1024 + it as fp16, with its sign bit turned over 1152 + the code
-        const uint32_t biased = word ^ 0x80808080u;
-        const __half2 offset = __half2half2(__ushort_as_half(0x6480));
-        const uint32_t a = __byte_perm(biased, 0x64646464u, 0x4140), b = __byte_perm(biased, 0x64646464u, 0x4342);
-        const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), offset), y = __hsub2(*reinterpret_cast<const __half2*>(&b), offset);
-        lo = *reinterpret_cast<const uint32_t*>(&x);
-        hi = *reinterpret_cast<const uint32_t*>(&y);
-    }
-}
-
 __device__ __forceinline__ int4 load16(const uint8_t* p) {
     int4 v;
     asm volatile("ld.global.L1::no_allocate.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
@@ -123,14 +70,14 @@ __device__ __forceinline__ void add8(float (&v)[8], float f, const float4& lo, c
 struct RowWork {
     RowSpan span;
     int last;          // tokens that some new token of the row sees
-    int blocks;        // of 8 columns
+    int blocks;        // of 8 columns; none where the row is kv8_prompt.cu's
     int pages;         // at least one: rows that see nothing have zeros to write
 };
 __device__ __forceinline__ RowWork row_work(const Kv8AttentionArgs& a, int row, int group) {
     RowWork w;
     w.span = row_span(a.starts, a.lengths, row, a.tokens, a.most, a.max_sequence);
     w.last = min(max(w.span.base + w.span.count, 0), a.max_sequence);
-    w.blocks = (w.span.count * group + kColumns - 1) / kColumns;
+    w.blocks = w.span.count * group > kKv8RowColumns ? 0 : (w.span.count * group + kColumns - 1) / kColumns;
     w.pages = max(1, (w.last + kPageTokens - 1) / kPageTokens);
     return w;
 }
@@ -168,6 +115,10 @@ __global__ void __launch_bounds__(kRowThreads, 2) kv8_rows_kernel(const Kv8Atten
     const int g = lane >> 2, q4 = lane & 3;
     const int heads = a.cache.heads, group = a.query_heads / heads;
 
+    if (a.prompts) {                                   // (they may run beside this one)
+        pdl_wait();
+        pdl_trigger();
+    }
     // ---- the batch's units (pages of a segment), as prefix sums over the rows; the first CTA counts what lies outside the host's bounds
     long long sum = 0;
     for (int first = 0; first < a.rows; first += kRowThreads) {
@@ -359,16 +310,16 @@ __global__ void __launch_bounds__(kRowThreads, 2) kv8_rows_kernel(const Kv8Atten
             s[2] = there && t_high < seen0 ? fmaf(s[2], f0, lv) : -INFINITY;
             s[3] = there && t_high < seen1 ? fmaf(s[3], f1, lv) : -INFINITY;
             float m0 = fmaxf(s[0], s[2]), m1 = fmaxf(s[1], s[3]);
-            if (__any_sync(0xffffffffu, m0 > top0 + kSlack || m1 > top1 + kSlack)) {
+            if (__any_sync(0xffffffffu, m0 > top0 + kKv8Slack || m1 > top1 + kKv8Slack)) {
 #pragma unroll
                 for (int x = 4; x < kWarp; x <<= 1) {
                     m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, x));
                     m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, x));
                 }
-                const float keep0 = m0 > top0 + kSlack ? exp2_ftz(top0 - m0) : 1.0f;
-                const float keep1 = m1 > top1 + kSlack ? exp2_ftz(top1 - m1) : 1.0f;
-                top0 = m0 > top0 + kSlack ? m0 : top0;
-                top1 = m1 > top1 + kSlack ? m1 : top1;
+                const float keep0 = m0 > top0 + kKv8Slack ? exp2_ftz(top0 - m0) : 1.0f;
+                const float keep1 = m1 > top1 + kKv8Slack ? exp2_ftz(top1 - m1) : 1.0f;
+                top0 = m0 > top0 + kKv8Slack ? m0 : top0;
+                top1 = m1 > top1 + kKv8Slack ? m1 : top1;
                 sum0 *= keep0;
                 sum1 *= keep1;
 #pragma unroll
@@ -380,12 +331,12 @@ __global__ void __launch_bounds__(kRowThreads, 2) kv8_rows_kernel(const Kv8Atten
                 }
             }
             // (nothing but -inf so far: weights of zero)
-            const float r0 = top0 == -INFINITY ? 0.0f : top0 - kLift, r1 = top1 == -INFINITY ? 0.0f : top1 - kLift;
+            const float r0 = top0 == -INFINITY ? 0.0f : top0 - kKv8Lift, r1 = top1 == -INFINITY ? 0.0f : top1 - kKv8Lift;
             const float w0 = exp2_ftz(s[0] - r0), w1 = exp2_ftz(s[1] - r1), w2 = exp2_ftz(s[2] - r0), w3 = exp2_ftz(s[3] - r1);
             const float inverse = reciprocal_fast(vs);
             sum0 = fmaf(w0 + w2, inverse, sum0);
             sum1 = fmaf(w1 + w3, inverse, sum1);
-            const uint32_t b0 = transpose8(pack_half2(w0, w1)), b1 = transpose8(pack_half2(w2, w3));
+            const uint32_t b0 = transposkv8_allow_smem(pack_half2(w0, w1)), b1 = transposkv8_allow_smem(pack_half2(w2, w3));
             // ---- output; what lies behind the row's last token may read as NaN, which no weight of zero removes
             if (E4M3 && (page + 1) * kPageTokens > w.last) {
 #pragma unroll
@@ -572,7 +523,8 @@ cudaError_t launch_rows(const Kv8AttentionArgs& a, cudaStream_t stream) {
     cudaError_t e = kv8_allow_smem(allowed, kv8_rows_kernel<HD, E4M3>, (int)rows_smem<HD>(Q3T_MAX_TABLE_ROWS));
     if (e == cudaSuccess) e = launch_zero_counters(static_cast<unsigned int*>(a.scratch), kRowCtas, stream);
     if (e != cudaSuccess) return e;
-    return launch_pdl(kv8_rows_kernel<HD, E4M3>, dim3(kRowCtas), dim3(kRowThreads), rows_smem<HD>(a.rows), stream, a);
+    e = launch_pdl(kv8_rows_kernel<HD, E4M3>, dim3(kRowCtas), dim3(kRowThreads), rows_smem<HD>(a.rows), stream, a);
+    return e != cudaSuccess || !a.prompts ? e : launch_kv8_prompts(a, HD, E4M3, stream);
 }
 
 // false: refused
@@ -613,6 +565,7 @@ bool attention_args(const Q3tKv8AttentionDesc* d, Kv8AttentionArgs* a) {
 }  // namespace
 
 unsigned int kv8_append_page_error_count();
+unsigned int kv8_prompt_page_error_count();
 unsigned int kv8_range_error_count() {
     unsigned int v = 0;
     return cudaMemcpyFromSymbol(&v, g_kv8_range_errors, sizeof(v)) == cudaSuccess ? v : ~0u;
@@ -622,7 +575,7 @@ unsigned int kv8_range_error_count() {
 
 extern "C" uint32_t q3t_kv8_page_error_count(void) {
     unsigned int v = 0;
-    return cudaMemcpyFromSymbol(&v, q3t::g_kv8_page_errors, sizeof(v)) == cudaSuccess ? v + q3t::kv8_append_page_error_count() : ~0u;
+    return cudaMemcpyFromSymbol(&v, q3t::g_kv8_page_errors, sizeof(v)) == cudaSuccess ? v + q3t::kv8_append_page_error_count() + q3t::kv8_prompt_page_error_count() : ~0u;
 }
 
 extern "C" size_t q3t_kv8_attention_scratch_bytes(const Q3tKv8AttentionDesc* desc) {
@@ -640,6 +593,7 @@ extern "C" int32_t q3t_launch_kv8_attention(const Q3tKv8AttentionDesc* desc, voi
     }
     if (a.most == 0) return cudaSuccess;
     a.scratch = desc->scratch;
+    a.prompts = (long long)a.most * (a.query_heads / a.cache.heads) > kKv8RowColumns ? 1 : 0;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool e4m3 = desc->cache->format == Q3T_KV8_E4M3;
     if (desc->cache->head_dimension == 128) return static_cast<int32_t>(e4m3 ? launch_rows<128, true>(a, s) : launch_rows<128, false>(a, s));

@@ -1,0 +1,535 @@
+// Causal attention over an 8-bit paged cache (q3t_launch_kv8_attention): rows of many new tokens.  The formula, and what makes a page's
+// value scale an addend of the exponent, are in kv8_attention.cu.
+//
+// A CTA takes 256 columns ((new token, query head) pairs of a KV head, two tiles of 128 rows of the tensor cores) of a row and walks
+// what they see of its cache once, 128 tokens a step:
+//   copies    codes from their pages to registers, to fp16 (exact) and into shared memory, swizzled: K by four warps, V by four; the
+//             next step's are requested before the present one's are stored
+//   scores    S = Q K^T, tcgen05.mma from shared memory into 128 columns of tensor memory a tile
+//   softmax   a thread a row: w = exp2(s * key scale + log2(value scale) - reference) as fp16 over the scores' place
+//   output    O += W V, the weights from tensor memory
+// While one tile's scores are in the softmax the other's products run: the tiles take turns.  A row's reference follows its scores
+// only when they exceed it by 2^8, so that the output in tensor memory is rescaled almost never.
+
+#include "kv8.cuh"
+#include "q3t_kernels.cuh"
+#include "q3t_tcgen05.cuh"
+
+namespace q3t {
+namespace {
+
+constexpr int kTileRows = 128;
+constexpr int kStep = 128;                              // tokens
+constexpr int kStepPages = kStep / kPageTokens;
+constexpr int kPromptThreads = 640;                     // warps 0..7 softmax (a tile each four), 8..11 K, 12..15 V, 16 products
+constexpr int kKeyWarp = 8, kValueWarp = 12, kProductWarp = 16;
+// What setmaxnreg hands out is what the block was launched with
+constexpr int kLaunchRegisters = 96, kSoftmaxRegisters = 152, kCopyRegisters = 64, kProductRegisters = 48;
+static_assert(2 * kSoftmaxRegisters + 2 * kCopyRegisters + kProductRegisters <= 5 * kLaunchRegisters, "registers of the five warpgroups");
+constexpr int kScaleRing = 4;                           // steps whose scales are kept: K runs two steps ahead of the softmax
+constexpr uint32_t kTmemCols = 512, kOut = 256;         // scores of the tiles at 0 and 128, outputs at 256 and 384
+constexpr unsigned long long kBudgetNs = 2000000000ull;
+
+__device__ unsigned int g_kv8_prompt_errors = 0;
+__device__ unsigned int g_kv8_prompt_page_errors = 0;
+
+template <int HD>
+struct PromptSmem {
+    static constexpr int kQueryBytes = 2 * kTileRows * HD * 2;
+    static constexpr int kTileBytes = kStep * HD * 2;
+    static constexpr size_t kBytes = 1024 + kQueryBytes + 4 * kTileBytes;
+};
+
+struct Item {
+    int row, kv_head, block;
+    RowSpan span;
+};
+
+// 16-byte piece `piece` of row `t` of a tile of 128: 64 dims in 128 bytes, swizzled, the next 64 a tile of rows further on
+__device__ __forceinline__ uint32_t tile_offset(int t, int piece) {
+    return (uint32_t)((piece >> 3) * kTileRows * 128 + t * 128 + (((piece & 7) ^ (t & 7)) << 4));
+}
+static_assert(kStep == kTileRows, "tile_offset");
+// B operand whose rows (dims) are contiguous: 64 of them in 128 bytes, the next 64 a tile of tokens further on, eight of K 1024 bytes
+__device__ __forceinline__ uint64_t desc_rows_contiguous(uint32_t smem) {
+    return (uint64_t)((smem >> 4) & 0x3FFFu) | ((uint64_t)(kStep * 128 / 16) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// 32 columns of this thread's lane; to be waited for
+__device__ __forceinline__ void tmem_load_32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));       // not to be used ahead of the wait
+}
+__device__ __forceinline__ void tmem_store_16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
+template <int HD, bool E4M3>
+__global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8AttentionArgs a) {
+    using Smem = PromptSmem<HD>;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* const smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    unsigned char* const queries = smem;                               // [tile]
+    unsigned char* const keys = smem + Smem::kQueryBytes;              // [step % 2]
+    unsigned char* const values = keys + 2 * Smem::kTileBytes;         // [step % 2]
+    __shared__ float4 scales[kScaleRing][kStepPages];                  // of each page: key scale, log2 and reciprocal of the value scale
+    __shared__ float row_scale[2 * kTileRows];
+    __shared__ uint64_t full_k[2], full_v[2], empty_k[2], empty_v[2], s_ready[2], p_ready[2], o_ready[2], q_ready;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_word;
+    __shared__ int warp_items[kPromptThreads / kWarp];
+    __shared__ Item found;
+    volatile int* const abort_flag = &abort_word;
+
+    const int tid = threadIdx.x, lane = tid % kWarp, warp = __shfl_sync(0xffffffffu, tid / kWarp, 0);
+    const int heads = a.cache.heads, group = a.query_heads / heads;
+
+    // ---- this CTA's columns: the rows of many columns have ceil(columns / 256) items a KV head; those of a row's last tokens, which see
+    // the most, first, all KV heads of a block together
+    if (tid == 0) found.row = -1;
+    __syncthreads();
+    int sum = 0;
+    for (int first = 0; first < a.rows; first += kPromptThreads) {
+        const int row = first + tid;
+        int mine = 0, own = 0;
+        RowSpan span{};
+        if (row < a.rows) {
+            span = row_span(a.starts, a.lengths, row, a.tokens, a.most, a.max_sequence);
+            const long long columns = (long long)span.count * group;
+            own = columns > kKv8RowColumns ? (int)((columns + 2 * kTileRows - 1) / (2 * kTileRows)) * heads : 0;
+            mine = own;
+        }
+#pragma unroll
+        for (int o = 1; o < kWarp; o <<= 1) {
+            const int other = __shfl_up_sync(0xffffffffu, mine, o);
+            if (lane >= o) mine += other;
+        }
+        if (lane == kWarp - 1) warp_items[warp] = mine;
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) mine += warp_items[w];
+        const int to = sum + mine, from = to - own, at = (int)blockIdx.x;
+        if (at >= from && at < to) found = Item{row, (at - from) % heads, own / heads - 1 - (at - from) / heads, span};
+        for (int w = 0; w < kPromptThreads / kWarp; ++w) sum += warp_items[w];
+        __syncthreads();
+    }
+    const Item item = found;
+    if (item.row < 0) return;                                          // (a grid is as large as tokens and rows may need)
+    const int column0 = item.block * 2 * kTileRows;
+    const int columns = min(2 * kTileRows, item.span.count * group - column0);
+    // tokens that the last column of each tile sees
+    auto seen_by = [&](int column) { return min(max(item.span.base + column / group + 1, 0), a.max_sequence); };
+    int steps_of[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int last = min(columns, (t + 1) * kTileRows);
+        steps_of[t] = last > t * kTileRows ? (seen_by(column0 + last - 1) + kStep - 1) / kStep : 0;
+    }
+    const int steps = max(steps_of[0], steps_of[1]);
+
+    tc::Guard guard;
+    guard.deadline = tc::now_ns() + kBudgetNs;
+    guard.abort_flag = abort_flag;
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(&full_k[i], 4);
+            tc::mbar_init(&full_v[i], 4);
+            tc::mbar_init(&empty_k[i], 1);
+            tc::mbar_init(&empty_v[i], 1);
+            tc::mbar_init(&s_ready[i], 1);
+            tc::mbar_init(&p_ready[i], 4);
+            tc::mbar_init(&o_ready[i], 1);
+        }
+        tc::mbar_init(&q_ready, 8);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kProductWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&tmem_slot)), "r"(kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = tmem_slot;
+
+    if (warp >= kKeyWarp && warp < kProductWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCopyRegisters));
+        // ---- copies: thread t takes 16 codes (8 of a head of 64) of token t / 8 of each of a step's pages
+        const bool is_value = warp >= kValueWarp;
+        const int t = tid - (is_value ? kValueWarp : kKeyWarp) * kWarp, token = t >> 3, part = t & 7;
+        constexpr int kCodes = HD / 8;                                 // bytes a thread and token
+        const uint8_t* const plane = (is_value ? a.cache.v : a.cache.k) + (size_t)item.kv_head * (kPageTokens * HD) + token * HD + part * kCodes;
+        unsigned char* const tiles = is_value ? values : keys;
+        uint64_t* const full = is_value ? full_v : full_k;
+        uint64_t* const empty = is_value ? empty_v : empty_k;
+        const int last = min(max(item.span.base + item.span.count, 0), a.max_sequence);        // what lies behind may read as NaN
+        const bool last_block = column0 + 2 * kTileRows >= item.span.count * group;
+        const int* const ids_at = a.table + (size_t)item.row * a.table_stride;
+        int ids = -1;                                                  // of 32 pages, a lane each
+        int4 code[kStepPages];
+        uint32_t good = 0u;                                            // pages of the step that are there
+        auto request = [&](int step) {
+            if (step % (kWarp / kStepPages) == 0) {
+                const int page = step * kStepPages + lane;
+                ids = page * kPageTokens < last ? ids_at[page] : -1;
+                if (ids < 0 || ids >= a.cache.pages) {
+                    if (page * kPageTokens < last && page < steps * kStepPages && t < kWarp && !is_value && item.kv_head == 0 && last_block) {
+                        atomicAdd(&g_kv8_prompt_page_errors, 1u);
+                    }
+                    ids = -1;
+                }
+            }
+            good = 0u;
+#pragma unroll
+            for (int p = 0; p < kStepPages; ++p) {
+                const int id = __shfl_sync(0xffffffffu, ids, step % (kWarp / kStepPages) * kStepPages + p);
+                code[p] = make_int4(0, 0, 0, 0);
+                if (id >= 0 && (step * kStepPages + p) * kPageTokens + token < last) {
+                    const uint8_t* const from = plane + (long long)id * a.cache.page_stride;
+                    if (kCodes == 16) {
+                        asm volatile("ld.global.L1::no_allocate.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(code[p].x), "=r"(code[p].y), "=r"(code[p].z), "=r"(code[p].w) : "l"(from));
+                    } else {
+                        const int2 half = *reinterpret_cast<const int2*>(from);
+                        code[p].x = half.x;
+                        code[p].y = half.y;
+                    }
+                }
+                good |= id >= 0 ? 1u << p : 0u;
+            }
+        };
+        float key_scale = 0.0f, value_scale = 0.0f;
+        // a page's scales, by one thread of the keys'
+        auto request_scales = [&](int step) {
+            const int id = __shfl_sync(0xffffffffu, ids, step % (kWarp / kStepPages) * kStepPages + (t & 7));
+            if (t < kStepPages && !is_value && id >= 0) {
+                const long long at = (long long)id * a.cache.scale_stride + item.kv_head;
+                key_scale = a.cache.k_scales[at];
+                value_scale = a.cache.v_scales[at];
+            }
+        };
+        if (steps > 0) {
+            request(0);
+            request_scales(0);
+        }
+        for (int step = 0; step < steps; ++step) {
+            const int buffer = step & 1;
+            if (step >= 2 && !__all_sync(0xffffffffu, guard.wait(&empty[buffer], ((step >> 1) - 1) & 1))) break;
+            if (t < kStepPages && !is_value) {
+                // a page that is not there weighs nothing: its codes are zeros, its value scale is as well
+                const float vs = fmaxf(value_scale, kKv8SmallestScale);
+                scales[step % kScaleRing][t] = (good >> t) & 1u ? make_float4(key_scale, log2_fast(vs), reciprocal_fast(vs), 0.0f)
+                                                               : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+            }
+            unsigned char* const tile = tiles + buffer * Smem::kTileBytes;
+#pragma unroll
+            for (int p = 0; p < kStepPages; ++p) {
+                const int row = p * kPageTokens + token;
+                uint32_t h[8];
+                codes_to_half<E4M3>((uint32_t)code[p].x, h[0], h[1]);
+                codes_to_half<E4M3>((uint32_t)code[p].y, h[2], h[3]);
+                if (kCodes == 16) {
+                    codes_to_half<E4M3>((uint32_t)code[p].z, h[4], h[5]);
+                    codes_to_half<E4M3>((uint32_t)code[p].w, h[6], h[7]);
+                    // (the second half of a token's threads takes its pieces the other way round: other banks)
+                    const int swap = part >> 2;
+                    const int4 lo = make_int4((int)h[0], (int)h[1], (int)h[2], (int)h[3]), hi = make_int4((int)h[4], (int)h[5], (int)h[6], (int)h[7]);
+                    *reinterpret_cast<int4*>(tile + tile_offset(row, 2 * part + swap)) = swap ? hi : lo;
+                    *reinterpret_cast<int4*>(tile + tile_offset(row, 2 * part + 1 - swap)) = swap ? lo : hi;
+                } else {
+                    *reinterpret_cast<int4*>(tile + tile_offset(row, part)) = make_int4((int)h[0], (int)h[1], (int)h[2], (int)h[3]);
+                }
+            }
+            if (step + 1 < steps) {
+                request(step + 1);
+                request_scales(step + 1);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&full[buffer]);
+        }
+    } else if (warp >= kProductWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProductRegisters));
+        if (warp == kProductWarp && steps > 0 && tc::elect_one()) {
+            // ---- products: both operands fp16, sums fp32
+            const uint32_t scores_idesc = (1u << 4) | ((uint32_t)(kStep >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
+            // B with its rows (dims) contiguous: bit 16
+            const uint32_t out_idesc = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
+            auto scores = [&](int tile, int step) {
+                const uint32_t q = tc::smem_u32(queries) + tile * kTileRows * HD * 2, k = tc::smem_u32(keys) + (step & 1) * Smem::kTileBytes;
+#pragma unroll
+                for (int j = 0; j < HD / 16; ++j) {
+                    umma_ss(tmem + tile * kStep, tc::umma_desc(q + (j / 4) * kTileRows * 128 + 32 * (j % 4)),
+                            tc::umma_desc(k + (j / 4) * kStep * 128 + 32 * (j % 4)), scores_idesc, j != 0 ? 1u : 0u);
+                }
+                tc::umma_commit(&s_ready[tile]);
+            };
+            bool ok = guard.wait(&q_ready, 0) && guard.wait(&full_k[0], 0);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (ok) {
+                if (steps_of[0] > 0) scores(0, 0);
+                if (steps_of[1] > 0) scores(1, 0);
+                tc::umma_commit(&empty_k[0]);
+            }
+            for (int step = 0; step < steps && ok; ++step) {
+                ok = guard.wait(&full_v[step & 1], (step >> 1) & 1);
+                bool keys_there = false;
+                for (int tile = 0; tile < 2 && ok; ++tile) {
+                    if (step >= steps_of[tile]) continue;
+                    ok = guard.wait(&p_ready[tile], step & 1);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t v = tc::smem_u32(values) + (step & 1) * Smem::kTileBytes;
+#pragma unroll
+                    for (int j = 0; j < kStep / 16; ++j) {
+                        tc::umma_f16_ts(tmem + kOut + tile * 128, tmem + tile * kStep + 8 * j, desc_rows_contiguous(v + j * 16 * 128), out_idesc,
+                                        (step | j) != 0 ? 1u : 0u);
+                    }
+                    tc::umma_commit(&o_ready[tile]);
+                    if (step + 1 < steps_of[tile]) {
+                        if (!keys_there) ok = guard.wait(&full_k[(step + 1) & 1], ((step + 1) >> 1) & 1);
+                        if (!ok) break;
+                        keys_there = true;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        scores(tile, step + 1);                        // (over the weights, behind the products that read them)
+                    }
+                }
+                if (!ok) break;
+                tc::umma_commit(&empty_v[step & 1]);
+                if (step + 1 < steps) tc::umma_commit(&empty_k[(step + 1) & 1]);
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
+        // ---- queries to fp16, by a power of two that brings the largest of each to 2^7..2^8
+        constexpr int kLanes = HD / 8, kAtOnce = kWarp / kLanes;       // of a row, rows of a warp
+#pragma unroll 4
+        for (int i = 0; i < 2 * kTileRows / (8 * kAtOnce); ++i) {
+            const int r = warp * (2 * kTileRows / 8) + i * kAtOnce + lane / kLanes, piece = lane % kLanes;
+            const int column = column0 + r, token = column / group;
+            int4 raw = make_int4(0, 0, 0, 0);
+            if (r < columns) {
+                raw = *reinterpret_cast<const int4*>(a.query + (size_t)(item.span.first + token) * a.query_stride
+                                                     + (size_t)(item.kv_head * group + column - token * group) * HD + piece * 8);
+            }
+            const uint32_t x[4] = {(uint32_t)raw.x, (uint32_t)raw.y, (uint32_t)raw.z, (uint32_t)raw.w};
+            uint32_t most = 0u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) most = __vmaxu2(most, x[e] & 0x7fff7fffu);
+            most = max(most & 0xffffu, most >> 16);
+#pragma unroll
+            for (int o = 1; o < kLanes; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+            const int shift = min(134 - (int)min(most >> 7, 254u), 127);
+            const float up = ldexpf(1.0f, shift);
+            int4 h;
+            h.x = (int)pack_half2(bf_lo(x[0]) * up, bf_hi(x[0]) * up);
+            h.y = (int)pack_half2(bf_lo(x[1]) * up, bf_hi(x[1]) * up);
+            h.z = (int)pack_half2(bf_lo(x[2]) * up, bf_hi(x[2]) * up);
+            h.w = (int)pack_half2(bf_lo(x[3]) * up, bf_hi(x[3]) * up);
+            *reinterpret_cast<int4*>(queries + (r / kTileRows) * kTileRows * HD * 2 + tile_offset(r % kTileRows, piece)) = h;
+            if (piece == 0) row_scale[r] = ldexpf(a.scale * 1.4426950408889634f, -shift);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&q_ready);
+        asm volatile("bar.sync 1, 256;" ::: "memory");                 // row_scale
+        // ---- softmax: a thread a row
+        const int tile = warp >> 2, quarter = warp & 3;
+        const int r = tile * kTileRows + quarter * kWarp + lane;
+        const bool real = r < columns;
+        const int seen = real ? seen_by(column0 + r) : 0;
+        const float up = row_scale[r];
+        const uint32_t lanes = tmem + ((uint32_t)(quarter * kWarp) << 16);
+        const uint32_t s_at = lanes + tile * kStep, o_at = lanes + kOut + tile * 128;
+        const int own_steps = steps_of[tile];
+        float top = -INFINITY, total = 0.0f;
+        for (int step = 0; step < own_steps; ++step) {
+            if (!__all_sync(0xffffffffu, guard.wait(&s_ready[tile], step & 1))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const float4* const page_scales = scales[step % kScaleRing];
+            const int t0 = step * kStep;
+            const bool masked = __any_sync(0xffffffffu, seen < t0 + kStep);
+            // the largest score of the step
+            float most = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < kStep / 32; ++c) {
+                uint32_t s[32];
+                tmem_load_32(s_at + 32 * c, s);
+                tmem_wait_load(s);
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    float m = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const float x = __uint_as_float(s[16 * p + j]);
+                        m = fmaxf(m, masked && t0 + 32 * c + 16 * p + j >= seen ? -INFINITY : x);
+                    }
+                    const float4 f = page_scales[2 * c + p];
+                    most = fmaxf(most, m == -INFINITY ? m : fmaf(m, f.x * up, f.y));
+                }
+            }
+            if (__any_sync(0xffffffffu, most > top + kKv8Slack)) {
+                const float moved = most > top + kKv8Slack ? most : top;
+                const float keep = moved == top ? 1.0f : exp2_ftz(top - moved);
+                top = moved;
+                total *= keep;
+                if (step > 0) {
+                    if (!__all_sync(0xffffffffu, guard.wait(&o_ready[tile], (step - 1) & 1))) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+                    for (int c = 0; c < HD; c += 16) {
+                        float o[16];
+                        uint32_t bits[16];
+                        tc::tmem_load_row<16>(o_at + c, o);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) bits[j] = __float_as_uint(o[j] * keep);
+                        tmem_store_16(o_at + c, bits);
+                    }
+                }
+            }
+            // (nothing but -inf so far: weights of zero)
+            const float reference = top == -INFINITY ? 0.0f : top - kKv8Lift;
+#pragma unroll
+            for (int c = 0; c < kStep / 32; ++c) {
+                uint32_t s[32], w[16];
+                tmem_load_32(s_at + 32 * c, s);
+                tmem_wait_load(s);
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const float4 f = page_scales[2 * c + p];
+                    const float slope = f.x * up, shift = f.y - reference;
+                    const unsigned long long slope2 = pack2(slope, slope), shift2 = pack2(shift, shift);
+                    unsigned long long sums = pack2(0.0f, 0.0f);
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) {
+                        float x, y;
+                        unpack2(fma2(pack2(__uint_as_float(s[16 * p + j]), __uint_as_float(s[16 * p + j + 1])), slope2, shift2), x, y);
+                        if (masked) {
+                            if (t0 + 32 * c + 16 * p + j >= seen) x = -INFINITY;
+                            if (t0 + 32 * c + 16 * p + j + 1 >= seen) y = -INFINITY;
+                        }
+                        x = exp2_ftz(x);
+                        y = exp2_ftz(y);
+                        sums = add2(sums, pack2(x, y));
+                        w[8 * p + j / 2] = pack_half2(x, y);
+                    }
+                    float x, y;
+                    unpack2(sums, x, y);
+                    total = fmaf(x + y, f.z, total);
+                }
+                tmem_store_16(s_at + 16 * c, w);
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&p_ready[tile]);
+        }
+        if (own_steps > 0) guard.wait(&o_ready[tile], (own_steps - 1) & 1);
+        __syncwarp();
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+        const int column = column0 + min(r, columns - 1), i = column / group;
+        const size_t token = item.span.first + i, at = (size_t)(item.kv_head * group + column - i * group) * HD;
+#pragma unroll 1
+        for (int c = 0; c < HD; c += 16) {
+            float o[16];
+            if (own_steps > 0) {
+                tc::tmem_load_row<16>(o_at + c, o);
+            }
+            if (!real || *abort_flag != 0) continue;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[j] = own_steps > 0 ? o[j] * inverse : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 16; j += 8) {
+                __nv_bfloat162 x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = __floats2bfloat162_rn(o[j + 2 * e], o[j + 2 * e + 1]);
+                *reinterpret_cast<int4*>(a.out + token * a.out_stride + at + c + j) = *reinterpret_cast<const int4*>(x);
+            }
+            if (a.out32 != nullptr) {
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                    *reinterpret_cast<float4*>(a.out32 + token * a.query_heads * HD + at + c + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                }
+            }
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    }
+    __syncwarp();
+    __syncthreads();
+    if (*abort_flag != 0) {
+        if (tid == 0) {
+            atomicAdd(&g_kv8_prompt_errors, 1u);
+            const unsigned long long until = tc::now_ns() + 200000ull;       // products that are still under way
+            while (tc::now_ns() < until) __nanosleep(1000);
+        }
+        __syncthreads();
+    }
+    if (warp == kProductWarp) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    }
+    pdl_wait();
+    pdl_trigger();
+}
+
+template <int HD, bool E4M3>
+cudaError_t launch_prompts(const Kv8AttentionArgs& a, cudaStream_t stream) {
+    static std::atomic<unsigned long long> allowed{0};
+    static std::atomic<bool> looked{false};
+    if (!looked.load(std::memory_order_acquire)) {
+        cudaFuncAttributes built;
+        const cudaError_t e = cudaFuncGetAttributes(&built, kv8_prompt_kernel<HD, E4M3>);
+        if (e != cudaSuccess) return e;
+        if (built.numRegs < kLaunchRegisters) return cudaErrorInvalidConfiguration;     // what setmaxnreg hands out has to be there
+        looked.store(true, std::memory_order_release);
+    }
+    const cudaError_t e = kv8_allow_smem(allowed, kv8_prompt_kernel<HD, E4M3>, (int)PromptSmem<HD>::kBytes);
+    if (e != cudaSuccess) return e;
+    // as many items as any split of the tokens over the rows can make
+    const long long columns = (long long)a.tokens * (a.query_heads / a.cache.heads);
+    const long long rows = columns / (kKv8RowColumns + 1) < a.rows ? columns / (kKv8RowColumns + 1) : a.rows;
+    const long long items = (columns / (2 * kTileRows) + rows) * a.cache.heads;
+    if (items > 0x7fffffffll) return cudaErrorInvalidValue;
+    return launch_pdl(kv8_prompt_kernel<HD, E4M3>, dim3((unsigned)(items > 0 ? items : 1)), dim3(kPromptThreads), PromptSmem<HD>::kBytes, stream, a);
+}
+
+}  // namespace
+
+cudaError_t launch_kv8_prompts(const Kv8AttentionArgs& a, int head_dim, bool e4m3, cudaStream_t stream) {
+    if (head_dim == 128) return e4m3 ? launch_prompts<128, true>(a, stream) : launch_prompts<128, false>(a, stream);
+    return e4m3 ? launch_prompts<64, true>(a, stream) : launch_prompts<64, false>(a, stream);
+}
+
+unsigned int kv8_prompt_error_count() {
+    unsigned int v = 0;
+    return cudaMemcpyFromSymbol(&v, g_kv8_prompt_errors, sizeof(v)) == cudaSuccess ? v : ~0u;
+}
+unsigned int kv8_prompt_page_error_count() {
+    unsigned int v = 0;
+    return cudaMemcpyFromSymbol(&v, g_kv8_prompt_page_errors, sizeof(v)) == cudaSuccess ? v : ~0u;
+}
+
+}  // namespace q3t

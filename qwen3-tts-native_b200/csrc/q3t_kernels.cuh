@@ -214,6 +214,7 @@ cudaError_t launch_attention_reference_order(const AttentionArgs& args, cudaStre
 // then attends in the reference's order.
 // rows seen so far whose position lay outside what the launch was sized for (clamped and counted)
 unsigned int kv8_range_error_count();          // kv8_attention.cu
+unsigned int kv8_prompt_error_count();         // kv8_prompt.cu
 unsigned int attention_range_error_count();
 cudaError_t set_attention_error_sink(unsigned int* device_visible_word);
 int set_attention_mode(int mode);
