@@ -15,6 +15,8 @@
 #include "q3t_kernels.cuh"
 #include "q3t_tcgen05.cuh"
 
+#include <type_traits>
+
 namespace q3t {
 namespace {
 
@@ -24,10 +26,11 @@ constexpr int kStepPages = kStep / kPageTokens;
 constexpr int kPromptThreads = 640;                     // warps 0..7 softmax (a tile each four), 8..11 K, 12..15 V, 16 products
 constexpr int kKeyWarp = 8, kValueWarp = 12, kProductWarp = 16;
 // What setmaxnreg hands out is what the block was launched with
-constexpr int kLaunchRegisters = 96, kSoftmaxRegisters = 152, kCopyRegisters = 64, kProductRegisters = 48;
+constexpr int kLaunchRegisters = 96, kSoftmaxRegisters = 144, kCopyRegisters = 72, kProductRegisters = 48;
 static_assert(2 * kSoftmaxRegisters + 2 * kCopyRegisters + kProductRegisters <= 5 * kLaunchRegisters, "registers of the five warpgroups");
 constexpr int kScaleRing = 4;                           // steps whose scales are kept: K runs two steps ahead of the softmax
 constexpr uint32_t kTmemCols = 512, kOut = 256;         // scores of the tiles at 0 and 128, outputs at 256 and 384
+constexpr float kMostWeight = 32768.0f;                 // of a page's weights together
 constexpr unsigned long long kBudgetNs = 2000000000ull;
 
 __device__ unsigned int g_kv8_prompt_errors = 0;
@@ -177,10 +180,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
 
     if (warp >= kKeyWarp && warp < kProductWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCopyRegisters));
-        // ---- copies: thread t takes 16 codes (8 of a head of 64) of token t / 8 of each of a step's pages
+        // ---- copies: a thread takes 16 codes (8 of a head of 64) of one token of each of a step's pages.  Eight threads that store side by
+        // side have half of the parts of two tokens, which the swizzle puts into all of the banks
         const bool is_value = warp >= kValueWarp;
-        const int t = tid - (is_value ? kValueWarp : kKeyWarp) * kWarp, token = t >> 3, part = t & 7;
+        const int t = tid - (is_value ? kValueWarp : kKeyWarp) * kWarp;
+        const int token = ((t >> 2) & 1) | ((t >> 4) << 1), part = (t & 3) | (((t >> 3) & 1) << 2);
         constexpr int kCodes = HD / 8;                                 // bytes a thread and token
+        const int store_at = (int)tile_offset(token, kCodes == 16 ? 2 * part : part);
+        const int store_more = (int)tile_offset(token, 2 * part + 1) - store_at;
         const uint8_t* const plane = (is_value ? a.cache.v : a.cache.k) + (size_t)item.kv_head * (kPageTokens * HD) + token * HD + part * kCodes;
         unsigned char* const tiles = is_value ? values : keys;
         uint64_t* const full = is_value ? full_v : full_k;
@@ -243,23 +250,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
                 scales[step % kScaleRing][t] = (good >> t) & 1u ? make_float4(key_scale, log2_fast(vs), reciprocal_fast(vs), 0.0f)
                                                                : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
             }
-            unsigned char* const tile = tiles + buffer * Smem::kTileBytes;
+            unsigned char* const tile = tiles + buffer * Smem::kTileBytes + store_at;
 #pragma unroll
             for (int p = 0; p < kStepPages; ++p) {
-                const int row = p * kPageTokens + token;
                 uint32_t h[8];
                 codes_to_half<E4M3>((uint32_t)code[p].x, h[0], h[1]);
                 codes_to_half<E4M3>((uint32_t)code[p].y, h[2], h[3]);
+                *reinterpret_cast<int4*>(tile + p * (kPageTokens * 128)) = make_int4((int)h[0], (int)h[1], (int)h[2], (int)h[3]);
                 if (kCodes == 16) {
                     codes_to_half<E4M3>((uint32_t)code[p].z, h[4], h[5]);
                     codes_to_half<E4M3>((uint32_t)code[p].w, h[6], h[7]);
-                    // (the second half of a token's threads takes its pieces the other way round: other banks)
-                    const int swap = part >> 2;
-                    const int4 lo = make_int4((int)h[0], (int)h[1], (int)h[2], (int)h[3]), hi = make_int4((int)h[4], (int)h[5], (int)h[6], (int)h[7]);
-                    *reinterpret_cast<int4*>(tile + tile_offset(row, 2 * part + swap)) = swap ? hi : lo;
-                    *reinterpret_cast<int4*>(tile + tile_offset(row, 2 * part + 1 - swap)) = swap ? lo : hi;
-                } else {
-                    *reinterpret_cast<int4*>(tile + tile_offset(row, part)) = make_int4((int)h[0], (int)h[1], (int)h[2], (int)h[3]);
+                    *reinterpret_cast<int4*>(tile + store_more + p * (kPageTokens * 128)) = make_int4((int)h[4], (int)h[5], (int)h[6], (int)h[7]);
                 }
             }
             if (step + 1 < steps) {
@@ -364,82 +365,100 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         const uint32_t lanes = tmem + ((uint32_t)(quarter * kWarp) << 16);
         const uint32_t s_at = lanes + tile * kStep, o_at = lanes + kOut + tile * 128;
         const int own_steps = steps_of[tile];
-        float top = -INFINITY, total = 0.0f;
+        float top = real ? -INFINITY : 0.0f, total = 0.0f;
         for (int step = 0; step < own_steps; ++step) {
             if (!__all_sync(0xffffffffu, guard.wait(&s_ready[tile], step & 1))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const float4* const page_scales = scales[step % kScaleRing];
-            const int t0 = step * kStep;
-            const bool masked = __any_sync(0xffffffffu, seen < t0 + kStep);
-            // the largest score of the step
-            float most = -INFINITY;
+            const int visible = seen - step * kStep;                   // of the step's tokens
+            const bool masked = __any_sync(0xffffffffu, visible < kStep);
+            // the reference becomes the largest score so far
+            auto measure = [&]() {
+                float most = -INFINITY;
+#pragma unroll 1
+                for (int c = 0; c < kStep / 32; ++c) {
+                    uint32_t s[32];
+                    tmem_load_32(s_at + 32 * c, s);
+                    tmem_wait_load(s);
 #pragma unroll
-            for (int c = 0; c < kStep / 32; ++c) {
-                uint32_t s[32];
-                tmem_load_32(s_at + 32 * c, s);
-                tmem_wait_load(s);
+                    for (int p = 0; p < 2; ++p) {
+                        float m = -INFINITY;
 #pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    float m = -INFINITY;
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float x = __uint_as_float(s[16 * p + j]);
-                        m = fmaxf(m, masked && t0 + 32 * c + 16 * p + j >= seen ? -INFINITY : x);
+                        for (int j = 0; j < 16; ++j) m = fmaxf(m, 32 * c + 16 * p + j >= visible ? -INFINITY : __uint_as_float(s[16 * p + j]));
+                        const float4 f = page_scales[2 * c + p];
+                        most = fmaxf(most, m == -INFINITY ? m : fmaf(m, f.x * up, f.y));
                     }
-                    const float4 f = page_scales[2 * c + p];
-                    most = fmaxf(most, m == -INFINITY ? m : fmaf(m, f.x * up, f.y));
                 }
-            }
-            if (__any_sync(0xffffffffu, most > top + kKv8Slack)) {
-                const float moved = most > top + kKv8Slack ? most : top;
+                const float moved = fmaxf(top, most);
                 const float keep = moved == top ? 1.0f : exp2_ftz(top - moved);
                 top = moved;
                 total *= keep;
-                if (step > 0) {
-                    if (!__all_sync(0xffffffffu, guard.wait(&o_ready[tile], (step - 1) & 1))) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (step == 0) return;
+                // (the products of the steps before are done: the scores came behind them)
 #pragma unroll 1
-                    for (int c = 0; c < HD; c += 16) {
-                        float o[16];
-                        uint32_t bits[16];
-                        tc::tmem_load_row<16>(o_at + c, o);
+                for (int c = 0; c < HD; c += 16) {
+                    float o[16];
+                    uint32_t bits[16];
+                    tc::tmem_load_row<16>(o_at + c, o);
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) bits[j] = __float_as_uint(o[j] * keep);
-                        tmem_store_16(o_at + c, bits);
+                    for (int j = 0; j < 16; ++j) bits[j] = __float_as_uint(o[j] * keep);
+                    tmem_store_16(o_at + c, bits);
+                }
+            };
+            uint32_t w[kStep / 2];
+            float added, largest;
+            auto weigh = [&](auto mask) {
+                // (nothing but -inf so far: weights of zero)
+                const float reference = top == -INFINITY ? 0.0f : top - kKv8Lift;
+                added = 0.0f;
+                largest = 0.0f;
+#pragma unroll
+                for (int c = 0; c < kStep / 32; ++c) {
+                    uint32_t s[32];
+                    tmem_load_32(s_at + 32 * c, s);
+                    tmem_wait_load(s);
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        const float4 f = page_scales[2 * c + p];
+                        const float slope = f.x * up, shift = f.y - reference;
+                        const unsigned long long slope2 = pack2(slope, slope), shift2 = pack2(shift, shift);
+                        unsigned long long sums = pack2(0.0f, 0.0f);
+#pragma unroll
+                        for (int j = 0; j < 16; j += 2) {
+                            float x, y;
+                            unpack2(fma2(pack2(__uint_as_float(s[16 * p + j]), __uint_as_float(s[16 * p + j + 1])), slope2, shift2), x, y);
+                            if (mask.value) {
+                                if (32 * c + 16 * p + j >= visible) x = -INFINITY;
+                                if (32 * c + 16 * p + j + 1 >= visible) y = -INFINITY;
+                            }
+                            x = exp2_ftz(x);
+                            y = exp2_ftz(y);
+                            sums = add2(sums, pack2(x, y));
+                            w[16 * c + 8 * p + j / 2] = pack_half2(x, y);
+                        }
+                        float x, y;
+                        unpack2(sums, x, y);
+                        x += y;
+                        largest = fmaxf(largest, x);
+                        added = fmaf(x, f.z, added);
                     }
                 }
+            };
+            // No maximum is looked for at first: a weight is at most its page's sum, which says whether one may have outgrown fp16
+            if (__any_sync(0xffffffffu, top == -INFINITY)) measure();
+            for (int again = 0;; ++again) {
+                if (masked) weigh(std::true_type{});
+                else weigh(std::false_type{});
+                if (again != 0 || !__any_sync(0xffffffffu, largest > kMostWeight)) break;
+                measure();
             }
-            // (nothing but -inf so far: weights of zero)
-            const float reference = top == -INFINITY ? 0.0f : top - kKv8Lift;
+            total += added;
 #pragma unroll
             for (int c = 0; c < kStep / 32; ++c) {
-                uint32_t s[32], w[16];
-                tmem_load_32(s_at + 32 * c, s);
-                tmem_wait_load(s);
+                uint32_t part_of[16];
 #pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    const float4 f = page_scales[2 * c + p];
-                    const float slope = f.x * up, shift = f.y - reference;
-                    const unsigned long long slope2 = pack2(slope, slope), shift2 = pack2(shift, shift);
-                    unsigned long long sums = pack2(0.0f, 0.0f);
-#pragma unroll
-                    for (int j = 0; j < 16; j += 2) {
-                        float x, y;
-                        unpack2(fma2(pack2(__uint_as_float(s[16 * p + j]), __uint_as_float(s[16 * p + j + 1])), slope2, shift2), x, y);
-                        if (masked) {
-                            if (t0 + 32 * c + 16 * p + j >= seen) x = -INFINITY;
-                            if (t0 + 32 * c + 16 * p + j + 1 >= seen) y = -INFINITY;
-                        }
-                        x = exp2_ftz(x);
-                        y = exp2_ftz(y);
-                        sums = add2(sums, pack2(x, y));
-                        w[8 * p + j / 2] = pack_half2(x, y);
-                    }
-                    float x, y;
-                    unpack2(sums, x, y);
-                    total = fmaf(x + y, f.z, total);
-                }
-                tmem_store_16(s_at + 16 * c, w);
+                for (int j = 0; j < 16; ++j) part_of[j] = w[16 * c + j];
+                tmem_store_16(s_at + 16 * c, part_of);
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
