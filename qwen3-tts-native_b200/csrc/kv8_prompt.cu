@@ -2,14 +2,14 @@
 // value scale an addend of the exponent, are in kv8_attention.cu.
 //
 // A CTA takes 256 columns ((new token, query head) pairs of a KV head, two tiles of 128 rows of the tensor cores) of a row and walks
-// what they see of its cache once, 128 tokens a step:
+// what they see of its cache once, 128 tokens a step, two halves of 64:
 //   copies    codes from their pages to registers, to fp16 (exact) and into shared memory, swizzled: K by four warps, V by four; the
 //             next step's are requested before the present one's are stored
-//   scores    S = Q K^T, tcgen05.mma from shared memory into 128 columns of tensor memory a tile
+//   scores    S = Q K^T, tcgen05.mma from shared memory into 64 columns of tensor memory a tile and half
 //   softmax   a thread a row: w = exp2(s * key scale + log2(value scale) - reference) as fp16 over the scores' place
 //   output    O += W V, the weights from tensor memory
-// While one tile's scores are in the softmax the other's products run: the tiles take turns.  A row's reference follows its scores
-// only when they exceed it by 2^8, so that the output in tensor memory is rescaled almost never.
+// While a tile's half is in the softmax the products of its other half and of the other tile run.  A row's reference follows its scores
+// only when its weights outgrow fp16, so that the output in tensor memory is rescaled almost never.
 
 #include "kv8.cuh"
 #include "q3t_kernels.cuh"
@@ -22,6 +22,7 @@ namespace {
 
 constexpr int kTileRows = 128;
 constexpr int kStep = 128;                              // tokens
+constexpr int kHalf = kStep / 2;
 constexpr int kStepPages = kStep / kPageTokens;
 constexpr int kPromptThreads = 640;                     // warps 0..7 softmax (a tile each four), 8..11 K, 12..15 V, 16 products
 constexpr int kKeyWarp = 8, kValueWarp = 12, kProductWarp = 16;
@@ -100,7 +101,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
     unsigned char* const values = keys + 2 * Smem::kTileBytes;         // [step % 2]
     __shared__ float4 scales[kScaleRing][kStepPages];                  // of each page: key scale, log2 and reciprocal of the value scale
     __shared__ float row_scale[2 * kTileRows];
-    __shared__ uint64_t full_k[2], full_v[2], empty_k[2], empty_v[2], s_ready[2], p_ready[2], o_ready[2], q_ready;
+    __shared__ uint64_t full_k[2], full_v[2], empty_k[2], empty_v[2], s_ready[2][2], p_ready[2][2], o_ready[2], q_ready;     // [tile][half]
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     __shared__ int warp_items[kPromptThreads / kWarp];
@@ -144,13 +145,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
     const int columns = min(2 * kTileRows, item.span.count * group - column0);
     // tokens that the last column of each tile sees
     auto seen_by = [&](int column) { return min(max(item.span.base + column / group + 1, 0), a.max_sequence); };
-    int steps_of[2];
+    int halves_of[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         const int last = min(columns, (t + 1) * kTileRows);
-        steps_of[t] = last > t * kTileRows ? (seen_by(column0 + last - 1) + kStep - 1) / kStep : 0;
+        halves_of[t] = last > t * kTileRows ? (seen_by(column0 + last - 1) + kHalf - 1) / kHalf : 0;
     }
-    const int steps = max(steps_of[0], steps_of[1]);
+    const int halves = max(halves_of[0], halves_of[1]), steps = (halves + 1) / 2;
 
     tc::Guard guard;
     guard.deadline = tc::now_ns() + kBudgetNs;
@@ -161,8 +162,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
             tc::mbar_init(&full_v[i], 4);
             tc::mbar_init(&empty_k[i], 1);
             tc::mbar_init(&empty_v[i], 1);
-            tc::mbar_init(&s_ready[i], 1);
-            tc::mbar_init(&p_ready[i], 4);
+            for (int h = 0; h < 2; ++h) {
+                tc::mbar_init(&s_ready[i][h], 1);
+                tc::mbar_init(&p_ready[i][h], 4);
+            }
             tc::mbar_init(&o_ready[i], 1);
         }
         tc::mbar_init(&q_ready, 8);
@@ -275,51 +278,57 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProductRegisters));
         if (warp == kProductWarp && steps > 0 && tc::elect_one()) {
             // ---- products: both operands fp16, sums fp32
-            const uint32_t scores_idesc = (1u << 4) | ((uint32_t)(kStep >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
+            const uint32_t scores_idesc = (1u << 4) | ((uint32_t)(kHalf >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
             // B with its rows (dims) contiguous: bit 16
             const uint32_t out_idesc = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
-            auto scores = [&](int tile, int step) {
-                const uint32_t q = tc::smem_u32(queries) + tile * kTileRows * HD * 2, k = tc::smem_u32(keys) + (step & 1) * Smem::kTileBytes;
+            auto scores = [&](int tile, int n) {                       // n: half of a step, counted through
+                const uint32_t q = tc::smem_u32(queries) + tile * kTileRows * HD * 2;
+                const uint32_t k = tc::smem_u32(keys) + ((n >> 1) & 1) * Smem::kTileBytes + (n & 1) * kHalf * 128;
 #pragma unroll
                 for (int j = 0; j < HD / 16; ++j) {
-                    umma_ss(tmem + tile * kStep, tc::umma_desc(q + (j / 4) * kTileRows * 128 + 32 * (j % 4)),
+                    umma_ss(tmem + tile * kStep + (n & 1) * kHalf, tc::umma_desc(q + (j / 4) * kTileRows * 128 + 32 * (j % 4)),
                             tc::umma_desc(k + (j / 4) * kStep * 128 + 32 * (j % 4)), scores_idesc, j != 0 ? 1u : 0u);
                 }
-                tc::umma_commit(&s_ready[tile]);
+                tc::umma_commit(&s_ready[tile][n & 1]);
             };
             bool ok = guard.wait(&q_ready, 0) && guard.wait(&full_k[0], 0);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (ok) {
-                if (steps_of[0] > 0) scores(0, 0);
-                if (steps_of[1] > 0) scores(1, 0);
-                tc::umma_commit(&empty_k[0]);
-            }
-            for (int step = 0; step < steps && ok; ++step) {
-                ok = guard.wait(&full_v[step & 1], (step >> 1) & 1);
-                bool keys_there = false;
-                for (int tile = 0; tile < 2 && ok; ++tile) {
-                    if (step >= steps_of[tile]) continue;
-                    ok = guard.wait(&p_ready[tile], step & 1);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t v = tc::smem_u32(values) + (step & 1) * Smem::kTileBytes;
-#pragma unroll
-                    for (int j = 0; j < kStep / 16; ++j) {
-                        tc::umma_f16_ts(tmem + kOut + tile * 128, tmem + tile * kStep + 8 * j, desc_rows_contiguous(v + j * 16 * 128), out_idesc,
-                                        (step | j) != 0 ? 1u : 0u);
-                    }
-                    tc::umma_commit(&o_ready[tile]);
-                    if (step + 1 < steps_of[tile]) {
-                        if (!keys_there) ok = guard.wait(&full_k[(step + 1) & 1], ((step + 1) >> 1) & 1);
-                        if (!ok) break;
-                        keys_there = true;
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        scores(tile, step + 1);                        // (over the weights, behind the products that read them)
+                for (int n = 0; n < 2; ++n) {
+                    for (int tile = 0; tile < 2; ++tile) {
+                        if (n < halves_of[tile]) scores(tile, n);
                     }
                 }
+                tc::umma_commit(&empty_k[0]);
+            }
+            for (int n = 0; n < halves && ok; ++n) {
+                const int step = n >> 1;
+                const bool ahead = n + 2 < halves;                     // scores of the next step
+                if ((n & 1) == 0) ok = guard.wait(&full_v[step & 1], (step >> 1) & 1);
+                for (int tile = 0; tile < 2 && ok; ++tile) {
+                    if (n >= halves_of[tile]) continue;
+                    ok = guard.wait(&p_ready[tile][n & 1], step & 1);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t v = tc::smem_u32(values) + (step & 1) * Smem::kTileBytes + (n & 1) * kHalf * 128;
+#pragma unroll
+                    for (int j = 0; j < kHalf / 16; ++j) {
+                        tc::umma_f16_ts(tmem + kOut + tile * 128, tmem + tile * kStep + (n & 1) * kHalf + 8 * j, desc_rows_contiguous(v + j * 16 * 128),
+                                        out_idesc, (n | j) != 0 ? 1u : 0u);
+                    }
+                    tc::umma_commit(&o_ready[tile]);
+                }
+                if (ahead && (n & 1) == 0) ok = ok && guard.wait(&full_k[(step + 1) & 1], ((step + 1) >> 1) & 1);
+                // the next scores of this half lie over the weights: products of other accumulators are in no order of their own
+                for (int tile = 0; tile < 2 && ok; ++tile) {
+                    if (n + 2 >= halves_of[tile]) continue;
+                    ok = guard.wait(&o_ready[tile], n & 1);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (ok) scores(tile, n + 2);
+                }
                 if (!ok) break;
-                tc::umma_commit(&empty_v[step & 1]);
-                if (step + 1 < steps) tc::umma_commit(&empty_k[(step + 1) & 1]);
+                if ((n & 1) != 0 || n + 1 == halves) tc::umma_commit(&empty_v[step & 1]);
+                if (ahead && ((n & 1) != 0 || n + 3 == halves)) tc::umma_commit(&empty_k[(step + 1) & 1]);
             }
         }
     } else {
@@ -363,20 +372,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         const int seen = real ? seen_by(column0 + r) : 0;
         const float up = row_scale[r];
         const uint32_t lanes = tmem + ((uint32_t)(quarter * kWarp) << 16);
-        const uint32_t s_at = lanes + tile * kStep, o_at = lanes + kOut + tile * 128;
-        const int own_steps = steps_of[tile];
+        const uint32_t o_at = lanes + kOut + tile * 128;
+        const int own = halves_of[tile];
         float top = real ? -INFINITY : 0.0f, total = 0.0f;
-        for (int step = 0; step < own_steps; ++step) {
-            if (!__all_sync(0xffffffffu, guard.wait(&s_ready[tile], step & 1))) break;
+        for (int n = 0; n < own; ++n) {
+            if (!__all_sync(0xffffffffu, guard.wait(&s_ready[tile][n & 1], (n >> 1) & 1))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const float4* const page_scales = scales[step % kScaleRing];
-            const int visible = seen - step * kStep;                   // of the step's tokens
-            const bool masked = __any_sync(0xffffffffu, visible < kStep);
+            const uint32_t s_at = lanes + tile * kStep + (n & 1) * kHalf;
+            const float4* const page_scales = scales[(n >> 1) % kScaleRing] + (n & 1) * (kStepPages / 2);
+            const int visible = seen - n * kHalf;                      // of the half's tokens
+            const bool masked = __any_sync(0xffffffffu, visible < kHalf);
             // the reference becomes the largest score so far
             auto measure = [&]() {
                 float most = -INFINITY;
 #pragma unroll 1
-                for (int c = 0; c < kStep / 32; ++c) {
+                for (int c = 0; c < kHalf / 32; ++c) {
                     uint32_t s[32];
                     tmem_load_32(s_at + 32 * c, s);
                     tmem_wait_load(s);
@@ -393,8 +403,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
                 const float keep = moved == top ? 1.0f : exp2_ftz(top - moved);
                 top = moved;
                 total *= keep;
-                if (step == 0) return;
-                // (the products of the steps before are done: the scores came behind them)
+                if (n == 0 || !__all_sync(0xffffffffu, guard.wait(&o_ready[tile], (n - 1) & 1))) return;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
                 for (int c = 0; c < HD; c += 16) {
                     float o[16];
@@ -405,7 +415,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
                     tmem_store_16(o_at + c, bits);
                 }
             };
-            uint32_t w[kStep / 2];
+            uint32_t w[kHalf / 2];
             float added, largest;
             auto weigh = [&](auto mask) {
                 // (nothing but -inf so far: weights of zero)
@@ -413,7 +423,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
                 added = 0.0f;
                 largest = 0.0f;
 #pragma unroll
-                for (int c = 0; c < kStep / 32; ++c) {
+                for (int c = 0; c < kHalf / 32; ++c) {
                     uint32_t s[32];
                     tmem_load_32(s_at + 32 * c, s);
                     tmem_wait_load(s);
@@ -454,7 +464,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
             }
             total += added;
 #pragma unroll
-            for (int c = 0; c < kStep / 32; ++c) {
+            for (int c = 0; c < kHalf / 32; ++c) {
                 uint32_t part_of[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j) part_of[j] = w[16 * c + j];
@@ -463,9 +473,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&p_ready[tile]);
+            if (lane == 0) tc::mbar_arrive(&p_ready[tile][n & 1]);
         }
-        if (own_steps > 0) guard.wait(&o_ready[tile], (own_steps - 1) & 1);
+        // (the last two halves' products; those before them came ahead of the last scores)
+        for (int n = max(own - 2, 0); n < own; ++n) guard.wait(&o_ready[tile], n & 1);
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
@@ -474,12 +485,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
 #pragma unroll 1
         for (int c = 0; c < HD; c += 16) {
             float o[16];
-            if (own_steps > 0) {
+            if (own > 0) {
                 tc::tmem_load_row<16>(o_at + c, o);
             }
             if (!real || *abort_flag != 0) continue;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) o[j] = own_steps > 0 ? o[j] * inverse : 0.0f;
+            for (int j = 0; j < 16; ++j) o[j] = own > 0 ? o[j] * inverse : 0.0f;
 #pragma unroll
             for (int j = 0; j < 16; j += 8) {
                 __nv_bfloat162 x[4];
