@@ -143,7 +143,10 @@ __global__ void __launch_bounds__(kRowThreads, 2) kv8_rows_kernel(const Kv8Atten
     }
     const long long units = sum;
     const int ctas = (int)min((long long)gridDim.x, (units + kRowWarps - 1) / kRowWarps);
-    if ((int)blockIdx.x >= ctas) return;
+    if ((int)blockIdx.x >= ctas) {
+        pdl_wait();
+        return;
+    }
     const long long cta_first = units * blockIdx.x / ctas, cta_end = units * (blockIdx.x + 1) / ctas;
     long long unit = cta_first + (cta_end - cta_first) * warp / kRowWarps;
     const long long unit_end = cta_first + (cta_end - cta_first) * (warp + 1) / kRowWarps;

@@ -44,6 +44,32 @@ struct PromptSmem {
     static constexpr size_t kBytes = 1024 + kQueryBytes + 4 * kTileBytes;
 };
 
+// As tc::Guard, with a limit to each look at a barrier: a look of the whole warp may be suspended for milliseconds otherwise, a thousand of
+// which are no bound
+struct Guard {
+    unsigned long long deadline;
+    volatile int* abort_flag;
+    __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) const {
+        uint32_t polls = 0;
+        for (;;) {
+            uint32_t ok;
+            asm volatile(
+                "{\n\t.reg .pred p;\n\t"
+                "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+                "selp.u32 %0, 1, 0, p;\n\t}"
+                : "=r"(ok)
+                : "r"(tc::smem_u32(bar)), "r"(parity), "r"(20000u)
+                : "memory");
+            if (ok != 0) return true;
+            if (*abort_flag != 0) return false;
+            if ((++polls & 31u) == 0 && tc::now_ns() > deadline) {
+                *abort_flag = 1;
+                return false;
+            }
+        }
+    }
+};
+
 struct Item {
     int row, kv_head, block;
     RowSpan span;
@@ -101,7 +127,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
     unsigned char* const values = keys + 2 * Smem::kTileBytes;         // [step % 2]
     __shared__ float4 scales[kScaleRing][kStepPages];                  // of each page: key scale, log2 and reciprocal of the value scale
     __shared__ float row_scale[2 * kTileRows];
-    __shared__ uint64_t full_k[2], full_v[2], empty_k[2], empty_v[2], s_ready[2][2], p_ready[2][2], o_ready[2], q_ready;     // [tile][half]
+    __shared__ uint64_t full_k[2], full_v[2], empty_k[2], empty_v[2], s_ready[2][2], p_ready[2][2], o_ready[2][2], q_ready;     // [tile][half]
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     __shared__ int warp_items[kPromptThreads / kWarp];
@@ -140,7 +166,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         __syncthreads();
     }
     const Item item = found;
-    if (item.row < 0) return;                                          // (a grid is as large as tokens and rows may need)
+    if (item.row < 0) {                                                // (a grid is as large as tokens and rows may need)
+        pdl_wait();                                                    // what follows relies on this launch to be behind the one before
+        return;
+    }
     const int column0 = item.block * 2 * kTileRows;
     const int columns = min(2 * kTileRows, item.span.count * group - column0);
     // tokens that the last column of each tile sees
@@ -153,7 +182,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
     }
     const int halves = max(halves_of[0], halves_of[1]), steps = (halves + 1) / 2;
 
-    tc::Guard guard;
+    Guard guard;
     guard.deadline = tc::now_ns() + kBudgetNs;
     guard.abort_flag = abort_flag;
     if (tid == 0) {
@@ -165,8 +194,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
             for (int h = 0; h < 2; ++h) {
                 tc::mbar_init(&s_ready[i][h], 1);
                 tc::mbar_init(&p_ready[i][h], 4);
+                tc::mbar_init(&o_ready[i][h], 1);
             }
-            tc::mbar_init(&o_ready[i], 1);
         }
         tc::mbar_init(&q_ready, 8);
         *abort_flag = 0;
@@ -316,13 +345,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
                         tc::umma_f16_ts(tmem + kOut + tile * 128, tmem + tile * kStep + (n & 1) * kHalf + 8 * j, desc_rows_contiguous(v + j * 16 * 128),
                                         out_idesc, (n | j) != 0 ? 1u : 0u);
                     }
-                    tc::umma_commit(&o_ready[tile]);
+                    tc::umma_commit(&o_ready[tile][n & 1]);
                 }
                 if (ahead && (n & 1) == 0) ok = ok && guard.wait(&full_k[(step + 1) & 1], ((step + 1) >> 1) & 1);
                 // the next scores of this half lie over the weights: products of other accumulators are in no order of their own
                 for (int tile = 0; tile < 2 && ok; ++tile) {
                     if (n + 2 >= halves_of[tile]) continue;
-                    ok = guard.wait(&o_ready[tile], n & 1);
+                    ok = guard.wait(&o_ready[tile][n & 1], step & 1);
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     if (ok) scores(tile, n + 2);
                 }
@@ -403,7 +432,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
                 const float keep = moved == top ? 1.0f : exp2_ftz(top - moved);
                 top = moved;
                 total *= keep;
-                if (n == 0 || !__all_sync(0xffffffffu, guard.wait(&o_ready[tile], (n - 1) & 1))) return;
+                if (n == 0 || !__all_sync(0xffffffffu, guard.wait(&o_ready[tile][(n - 1) & 1], ((n - 1) >> 1) & 1))) return;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
                 for (int c = 0; c < HD; c += 16) {
@@ -475,8 +504,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(&p_ready[tile][n & 1]);
         }
-        // (the last two halves' products; those before them came ahead of the last scores)
-        for (int n = max(own - 2, 0); n < own; ++n) guard.wait(&o_ready[tile], n & 1);
+        // (A barrier a half: of the one that is waited for here all completions but the last are known to be past, so that its parity says
+        // which.  With one barrier for both halves a late reader would take two completions for none.)
+        if (own > 0) guard.wait(&o_ready[tile][(own - 1) & 1], ((own - 1) >> 1) & 1);
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
