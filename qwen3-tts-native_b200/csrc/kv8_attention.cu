@@ -1,7 +1,7 @@
 // Causal attention over an 8-bit paged cache (q3t_launch_kv8_attention): rows of few new tokens.  kv8_prompt.cu has the others.
 //
 // out = sum_j p_j v_j / sum_j p_j, p_j = exp(scale * q . k_j - max), over the positions up to the token's own; k_j and v_j are codes times the
-// scale of their page and head.  A (new token, query head) of a KV head is a column; a warp takes pages of 16 tokens for 8 columns:
+// scale of their page and head.  A (new token, query head) of a KV head is a column; a warp takes pages of 16 tokens for 8 or 16 columns:
 //   scores    S^T = K Q^T, mma.sync m16n8k16 in fp16: tokens are rows of A (a row's 16-byte loads give whole fragments once the
 //             contraction index is permuted alike in Q), columns those of B
 //   weights   w_j = exp2(s_j * key scale + log2(value scale) - reference): the value's scale is an addend of the exponent, so that
@@ -11,7 +11,7 @@
 // maximum until a score exceeds it by 2^8, so that outputs are rescaled almost never; weights are kept 2^6 times larger than that
 // needs, which leaves fp16 its 11 bits down to 2^-20 of the largest.
 //
-// The batch's work, the pages of every (row, KV head, 8 columns), is cut into as many equal ranges as there are warps, wherever
+// The batch's work, the pages of every (row, KV head, block of columns), is cut into as many equal ranges as there are warps, wherever
 // that falls.  A warp writes what it has whole; what is cut is merged by the CTA in shared memory, and of what its range cuts
 // the CTA leaves (reference, sum, output) and the one with the last ticket folds them in order, so a result depends on
 // the batch's lengths, not on timing.
@@ -30,7 +30,7 @@ namespace {
 constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / kWarp;
 constexpr int kRowCtas = 2 * 148;
-constexpr int kColumns = 8;
+constexpr int kTileColumns = 8;                        // of a product
 constexpr int kCounterBytes = (kRowCtas * 4 + 255) / 256 * 256;
 
 __device__ unsigned int g_kv8_range_errors = 0;
@@ -44,7 +44,7 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // an 8 x 8 tile of fp16 across the warp, rows for columns
-__device__ __forceinline__ uint32_t transposkv8_allow_smem(uint32_t x) {
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t r;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
     return r;
@@ -55,34 +55,38 @@ __device__ __forceinline__ int4 load16(const uint8_t* p) {
     return v;
 }
 
-__device__ __forceinline__ void add8(float (&v)[8], float f, const float4& lo, const float4& hi) {
-    v[0] = fmaf(f, lo.x, v[0]);
-    v[1] = fmaf(f, lo.y, v[1]);
-    v[2] = fmaf(f, lo.z, v[2]);
-    v[3] = fmaf(f, lo.w, v[3]);
-    v[4] = fmaf(f, hi.x, v[4]);
-    v[5] = fmaf(f, hi.y, v[5]);
-    v[6] = fmaf(f, hi.z, v[6]);
-    v[7] = fmaf(f, hi.w, v[7]);
-}
+// 8 dims of the pieces of a column: their sum in terms of the largest reference
+struct Merged {
+    float top = -INFINITY, total = 0.0f, sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    // stats: reference and total of a piece
+    __device__ __forceinline__ void add(const float2& stats, const float4& lo, const float4& hi) {
+        const float most = fmaxf(top, stats.x);
+        const float keep = top == -INFINITY ? 0.0f : exp2_ftz(top - most), f = stats.x == -INFINITY ? 0.0f : exp2_ftz(stats.x - most);
+        const float more[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        top = most;
+        total = fmaf(f, stats.y, total * keep);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] = fmaf(f, more[e], sum[e] * keep);
+    }
+};
 
 // What a row asks of the kernel
 struct RowWork {
     RowSpan span;
     int last;          // tokens that some new token of the row sees
-    int blocks;        // of 8 columns; none where the row is kv8_prompt.cu's
+    int blocks;        // of 8 or 16 columns; none where the row is kv8_prompt.cu's
     int pages;         // at least one: rows that see nothing have zeros to write
 };
-__device__ __forceinline__ RowWork row_work(const Kv8AttentionArgs& a, int row, int group) {
+__device__ __forceinline__ RowWork row_work(const Kv8AttentionArgs& a, int row, int group, int block_columns) {
     RowWork w;
     w.span = row_span(a.starts, a.lengths, row, a.tokens, a.most, a.max_sequence);
     w.last = min(max(w.span.base + w.span.count, 0), a.max_sequence);
-    w.blocks = w.span.count * group > kKv8RowColumns ? 0 : (w.span.count * group + kColumns - 1) / kColumns;
+    w.blocks = w.span.count * group > kKv8RowColumns ? 0 : (w.span.count * group + block_columns - 1) / block_columns;
     w.pages = max(1, (w.last + kPageTokens - 1) / kPageTokens);
     return w;
 }
 
-// A part of a segment, (row, KV head, 8 columns): whose it is
+// A part of a segment, (row, KV head, block of columns): whose it is
 struct Piece {
     long long start;   // first unit of the segment, -1: none
     int pages;         // of the segment
@@ -92,13 +96,19 @@ struct Piece {
     int columns;       // of the segment
 };
 
-template <int HD>
+template <int HD, int TILES>
 constexpr size_t rows_smem(int rows) {
-    return (size_t)rows * sizeof(long long) + (size_t)2 * kRowWarps * kColumns * (HD + 4) * sizeof(float);
+    return (size_t)rows * sizeof(long long) + (size_t)2 * kRowWarps * TILES * kTileColumns * (HD + 4) * sizeof(float);
+}
+// CTAs of an SM: a warp of two tiles of columns and heads of 128 holds twice the outputs and queries
+template <int HD, int TILES>
+constexpr int rows_residency() {
+    return HD == 128 && TILES == 2 ? 1 : 2;
 }
 
-template <int HD, bool E4M3>
-__global__ void __launch_bounds__(kRowThreads, 2) kv8_rows_kernel(const Kv8AttentionArgs a) {
+template <int HD, bool E4M3, int TILES>
+__global__ void __launch_bounds__(kRowThreads, rows_residency<HD, TILES>()) kv8_rows_kernel(const Kv8AttentionArgs a) {
+    constexpr int kColumns = TILES * kTileColumns;
     constexpr int kParts = HD / 64;                    // 16-byte pieces of a key that a lane holds
     constexpr int kTiles = HD / 16;                    // of 16 dims
     constexpr int kWords = HD / 32;                    // of a value's dims that a lane holds
@@ -108,9 +118,8 @@ __global__ void __launch_bounds__(kRowThreads, 2) kv8_rows_kernel(const Kv8Atten
     float* const parts = reinterpret_cast<float*>(smem);                                    // [warp][2] pieces
     long long* const before = reinterpret_cast<long long*>(parts + 2 * kRowWarps * kPiece);  // [rows]: units of the rows up to each
     __shared__ Piece held[2 * kRowWarps];
-    __shared__ float fold_scale[2][kRowCtas][kColumns];
     __shared__ long long scan[kRowWarps];
-    __shared__ int beyond[2], tickets[2];              // segments that go beyond the CTA at its start and its end
+    __shared__ int folds[2];                           // of the segments that go beyond the CTA at its start and its end: the piece, if it is up to this CTA
     const int tid = threadIdx.x, lane = tid % kWarp, warp = __shfl_sync(0xffffffffu, tid / kWarp, 0);
     const int g = lane >> 2, q4 = lane & 3;
     const int heads = a.cache.heads, group = a.query_heads / heads;
@@ -125,7 +134,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) kv8_rows_kernel(const Kv8Atten
         const int row = first + tid;
         long long mine = 0;
         if (row < a.rows) {
-            const RowWork w = row_work(a, row, group);
+            const RowWork w = row_work(a, row, group, kColumns);
             mine = (long long)w.blocks * heads * w.pages;
             if (w.span.cut && blockIdx.x == 0) atomicAdd(&g_kv8_range_errors, 1u);
         }
@@ -174,14 +183,14 @@ __global__ void __launch_bounds__(kRowThreads, 2) kv8_rows_kernel(const Kv8Atten
             *reinterpret_cast<float4*>(to + 4) = make_float4(v[4], v[5], v[6], v[7]);
         }
     };
-    if (tid < 2) beyond[tid] = -1;
+    if (tid < 2) folds[tid] = -1;
     if (lane < 2) held[2 * warp + lane].start = -1;
     __syncwarp();
 
     int pieces_held = 0;
     while (unit < unit_end) {
         while (before[row] <= unit) ++row;
-        const RowWork w = row_work(a, row, group);
+        const RowWork w = row_work(a, row, group, kColumns);
         const long long row_first = row > 0 ? before[row - 1] : 0;
         const int segment = (int)((unit - row_first) / w.pages);              // (KV head, block of columns)
         const long long start = row_first + (long long)segment * w.pages;
@@ -196,22 +205,23 @@ __global__ void __launch_bounds__(kRowThreads, 2) kv8_rows_kernel(const Kv8Atten
         auto ids_from = [&](int first) { return first + lane < page_end && (first + lane) * kPageTokens < w.last ? ids_at[first + lane] : -1; };
         int ids = ids_from(page_first);
 
-        // ---- queries: this lane's column and dims, to fp16 by a power of two that brings the largest to 2^7..2^8
-        uint32_t qf[kParts][4][2];
-        float column_scale;
-        int column_seen;
-        int4 raw[kParts][2];
-        {
-            const int column = block * kColumns + g;
-            const bool real = g < columns;
+        // ---- queries: this lane's columns and dims, to fp16 by a power of two that brings the largest to 2^7..2^8
+        uint32_t qf[TILES][kParts][4][2];
+        float column_scale[TILES];
+        int column_seen[TILES];
+        int4 raw[TILES][kParts][2];
+#pragma unroll
+        for (int n = 0; n < TILES; ++n) {
+            const int of_block = n * kTileColumns + g, column = block * kColumns + of_block;
+            const bool real = of_block < columns;
             const int i = real ? column / group : 0;
             const bf16* q = a.query + (size_t)(w.span.first + i) * a.query_stride + (size_t)(kv_head * group + column % group) * HD + q4 * 16;
 #pragma unroll
             for (int j = 0; j < kParts; ++j) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) raw[j][h] = real ? *reinterpret_cast<const int4*>(q + 64 * j + 8 * h) : make_int4(0, 0, 0, 0);
+                for (int h = 0; h < 2; ++h) raw[n][j][h] = real ? *reinterpret_cast<const int4*>(q + 64 * j + 8 * h) : make_int4(0, 0, 0, 0);
             }
-            column_seen = real ? min(max(w.span.base + i + 1, 0), a.max_sequence) : 0;
+            column_seen[n] = real ? min(max(w.span.base + i + 1, 0), a.max_sequence) : 0;
         }
         int4 kr[kParts][2], vr[4];
         float key_scale, value_scale;
@@ -244,13 +254,14 @@ __global__ void __launch_bounds__(kRowThreads, 2) kv8_rows_kernel(const Kv8Atten
         int raw_id = __shfl_sync(0xffffffffu, ids, 0);
         load_keys(usable(raw_id) ? raw_id : 0);
         load_values(usable(raw_id) ? raw_id : 0);
-        {
+#pragma unroll
+        for (int n = 0; n < TILES; ++n) {
             uint32_t most = 0u;
 #pragma unroll
             for (int j = 0; j < kParts; ++j) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const uint32_t x[4] = {(uint32_t)raw[j][h].x, (uint32_t)raw[j][h].y, (uint32_t)raw[j][h].z, (uint32_t)raw[j][h].w};
+                    const uint32_t x[4] = {(uint32_t)raw[n][j][h].x, (uint32_t)raw[n][j][h].y, (uint32_t)raw[n][j][h].z, (uint32_t)raw[n][j][h].w};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) most = __vmaxu2(most, x[e] & 0x7fff7fffu);
                 }
@@ -260,25 +271,32 @@ __global__ void __launch_bounds__(kRowThreads, 2) kv8_rows_kernel(const Kv8Atten
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
             const int shift = min(134 - (int)min(most >> 7, 254u), 127);
             const float up = ldexpf(1.0f, shift);
-            column_scale = ldexpf(a.scale * 1.4426950408889634f, -shift);
+            column_scale[n] = ldexpf(a.scale * 1.4426950408889634f, -shift);
 #pragma unroll
             for (int j = 0; j < kParts; ++j) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const uint32_t x[4] = {(uint32_t)raw[j][h].x, (uint32_t)raw[j][h].y, (uint32_t)raw[j][h].z, (uint32_t)raw[j][h].w};
+                    const uint32_t x[4] = {(uint32_t)raw[n][j][h].x, (uint32_t)raw[n][j][h].y, (uint32_t)raw[n][j][h].z, (uint32_t)raw[n][j][h].w};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) qf[j][2 * h + e / 2][e & 1] = pack_half2(bf_lo(x[e]) * up, bf_hi(x[e]) * up);
+                    for (int e = 0; e < 4; ++e) qf[n][j][2 * h + e / 2][e & 1] = pack_half2(bf_lo(x[e]) * up, bf_hi(x[e]) * up);
                 }
             }
         }
-        // of the columns whose scores this lane gets
-        const float scale0 = __shfl_sync(0xffffffffu, column_scale, 8 * q4), scale1 = __shfl_sync(0xffffffffu, column_scale, 8 * q4 + 4);
-        const int seen0 = __shfl_sync(0xffffffffu, column_seen, 8 * q4), seen1 = __shfl_sync(0xffffffffu, column_seen, 8 * q4 + 4);
-
-        float o[kTiles][4];
+        // of the columns whose scores this lane gets, 2 q4 and + 1 of each tile
+        float scale_of[TILES][2], top[TILES][2], sum_of[TILES][2], o[TILES][kTiles][4];
+        int seen[TILES][2];
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.0f;
-        float top0 = -INFINITY, top1 = -INFINITY, sum0 = 0.0f, sum1 = 0.0f;
+        for (int n = 0; n < TILES; ++n) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                scale_of[n][c] = __shfl_sync(0xffffffffu, column_scale[n], 8 * q4 + 4 * c);
+                seen[n][c] = __shfl_sync(0xffffffffu, column_seen[n], 8 * q4 + 4 * c);
+                top[n][c] = -INFINITY;
+                sum_of[n][c] = 0.0f;
+            }
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) o[n][t][0] = o[n][t][1] = o[n][t][2] = o[n][t][3] = 0.0f;
+        }
 
         for (int page = page_first; page < page_end; ++page) {
             const bool there = usable(raw_id);
@@ -290,7 +308,9 @@ __global__ void __launch_bounds__(kRowThreads, 2) kv8_rows_kernel(const Kv8Atten
             const bool more = page + 1 < page_end;
 
             // ---- scores
-            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float s[TILES][4];
+#pragma unroll
+            for (int n = 0; n < TILES; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
 #pragma unroll
             for (int j = 0; j < kParts; ++j) {
                 const uint32_t x[4] = {(uint32_t)kr[j][0].x, (uint32_t)kr[j][0].y, (uint32_t)kr[j][0].z, (uint32_t)kr[j][0].w};
@@ -300,46 +320,56 @@ __global__ void __launch_bounds__(kRowThreads, 2) kv8_rows_kernel(const Kv8Atten
                     uint32_t a0, a1, a2, a3;
                     codes_to_half<E4M3>(x[e], a0, a2);
                     codes_to_half<E4M3>(y[e], a1, a3);
-                    mma_f16(s, a0, a1, a2, a3, qf[j][e][0], qf[j][e][1]);
+#pragma unroll
+                    for (int n = 0; n < TILES; ++n) mma_f16(s[n], a0, a1, a2, a3, qf[n][j][e][0], qf[n][j][e][1]);
                 }
             }
             const float ks = key_scale, vs = fmaxf(value_scale, kKv8SmallestScale);
             if (more) load_keys(next_id);
             // ---- weights of the codes
-            const float lv = log2_fast(vs), f0 = ks * scale0, f1 = ks * scale1;
+            const float lv = log2_fast(vs), inverse = reciprocal_fast(vs);
             const int t_low = page * kPageTokens + g, t_high = t_low + 8;
-            s[0] = there && t_low < seen0 ? fmaf(s[0], f0, lv) : -INFINITY;
-            s[1] = there && t_low < seen1 ? fmaf(s[1], f1, lv) : -INFINITY;
-            s[2] = there && t_high < seen0 ? fmaf(s[2], f0, lv) : -INFINITY;
-            s[3] = there && t_high < seen1 ? fmaf(s[3], f1, lv) : -INFINITY;
-            float m0 = fmaxf(s[0], s[2]), m1 = fmaxf(s[1], s[3]);
-            if (__any_sync(0xffffffffu, m0 > top0 + kKv8Slack || m1 > top1 + kKv8Slack)) {
+            uint32_t b0[TILES], b1[TILES];
 #pragma unroll
-                for (int x = 4; x < kWarp; x <<= 1) {
-                    m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, x));
-                    m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, x));
-                }
-                const float keep0 = m0 > top0 + kKv8Slack ? exp2_ftz(top0 - m0) : 1.0f;
-                const float keep1 = m1 > top1 + kKv8Slack ? exp2_ftz(top1 - m1) : 1.0f;
-                top0 = m0 > top0 + kKv8Slack ? m0 : top0;
-                top1 = m1 > top1 + kKv8Slack ? m1 : top1;
-                sum0 *= keep0;
-                sum1 *= keep1;
+            for (int n = 0; n < TILES; ++n) {
+                float m[2];
+                bool moves = false;
 #pragma unroll
-                for (int t = 0; t < kTiles; ++t) {
-                    o[t][0] *= keep0;
-                    o[t][1] *= keep1;
-                    o[t][2] *= keep0;
-                    o[t][3] *= keep1;
+                for (int c = 0; c < 2; ++c) {
+                    const float f = ks * scale_of[n][c];
+                    s[n][c] = there && t_low < seen[n][c] ? fmaf(s[n][c], f, lv) : -INFINITY;
+                    s[n][2 + c] = there && t_high < seen[n][c] ? fmaf(s[n][2 + c], f, lv) : -INFINITY;
+                    m[c] = fmaxf(s[n][c], s[n][2 + c]);
+                    moves |= m[c] > top[n][c] + kKv8Slack;
                 }
+                if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                        for (int x = 4; x < kWarp; x <<= 1) m[c] = fmaxf(m[c], __shfl_xor_sync(0xffffffffu, m[c], x));
+                        const bool up = m[c] > top[n][c] + kKv8Slack;
+                        const float keep = up ? exp2_ftz(top[n][c] - m[c]) : 1.0f;
+                        top[n][c] = up ? m[c] : top[n][c];
+                        sum_of[n][c] *= keep;
+#pragma unroll
+                        for (int t = 0; t < kTiles; ++t) {
+                            o[n][t][c] *= keep;
+                            o[n][t][2 + c] *= keep;
+                        }
+                    }
+                }
+                float low[2], high[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    // (nothing but -inf so far: weights of zero)
+                    const float reference = top[n][c] == -INFINITY ? 0.0f : top[n][c] - kKv8Lift;
+                    low[c] = exp2_ftz(s[n][c] - reference);
+                    high[c] = exp2_ftz(s[n][2 + c] - reference);
+                    sum_of[n][c] = fmaf(low[c] + high[c], inverse, sum_of[n][c]);
+                }
+                b0[n] = transpose8(pack_half2(low[0], low[1]));
+                b1[n] = transpose8(pack_half2(high[0], high[1]));
             }
-            // (nothing but -inf so far: weights of zero)
-            const float r0 = top0 == -INFINITY ? 0.0f : top0 - kKv8Lift, r1 = top1 == -INFINITY ? 0.0f : top1 - kKv8Lift;
-            const float w0 = exp2_ftz(s[0] - r0), w1 = exp2_ftz(s[1] - r1), w2 = exp2_ftz(s[2] - r0), w3 = exp2_ftz(s[3] - r1);
-            const float inverse = reciprocal_fast(vs);
-            sum0 = fmaf(w0 + w2, inverse, sum0);
-            sum1 = fmaf(w1 + w3, inverse, sum1);
-            const uint32_t b0 = transposkv8_allow_smem(pack_half2(w0, w1)), b1 = transposkv8_allow_smem(pack_half2(w2, w3));
             // ---- output; what lies behind the row's last token may read as NaN, which no weight of zero removes
             if (E4M3 && (page + 1) * kPageTokens > w.last) {
 #pragma unroll
@@ -357,40 +387,40 @@ __global__ void __launch_bounds__(kRowThreads, 2) kv8_rows_kernel(const Kv8Atten
                     uint32_t a0, a1, a2, a3;
                     codes_to_half<E4M3>(__byte_perm(word(vr[0]), word(vr[1]), h == 0 ? 0x5140 : 0x7362), a0, a1);
                     codes_to_half<E4M3>(__byte_perm(word(vr[2]), word(vr[3]), h == 0 ? 0x5140 : 0x7362), a2, a3);
-                    mma_f16(o[2 * e + h], a0, a1, a2, a3, b0, b1);
+#pragma unroll
+                    for (int n = 0; n < TILES; ++n) mma_f16(o[n][2 * e + h], a0, a1, a2, a3, b0[n], b1[n]);
                 }
             }
             if (more) load_values(next_id);
             raw_id = next_raw;
         }
-#pragma unroll
-        for (int x = 4; x < kWarp; x <<= 1) {
-            sum0 += __shfl_xor_sync(0xffffffffu, sum0, x);
-            sum1 += __shfl_xor_sync(0xffffffffu, sum1, x);
-        }
         // ---- whole: written; cut: into shared memory
         const bool whole = page_first == 0 && page_end == w.pages;
         float* const piece = parts + (size_t)(2 * warp + pieces_held) * kPiece;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            if (2 * q4 + c >= columns) continue;
-            if (whole) {
-                const float total = c == 0 ? sum0 : sum1, inverse = total == 0.0f ? 0.0f : 1.0f / total;
+        for (int n = 0; n < TILES; ++n) {
 #pragma unroll
-                for (int t = 0; t < kTiles; t += 4) {
-                    const float v[8] = {o[t][c] * inverse, o[t][c + 2] * inverse, o[t + 1][c] * inverse, o[t + 1][c + 2] * inverse,
-                                        o[t + 2][c] * inverse, o[t + 2][c + 2] * inverse, o[t + 3][c] * inverse, o[t + 3][c + 2] * inverse};
-                    write8(w.span.first, kv_head, block * kColumns + 2 * q4 + c, g * (HD / 8) + 2 * t, v);
-                }
-            } else {
-                float* const at = piece + (2 * q4 + c) * kPitch;
+            for (int c = 0; c < 2; ++c) {
+                float total = sum_of[n][c];
 #pragma unroll
-                for (int t = 0; t < kTiles; t += 2) {
-                    *reinterpret_cast<float4*>(at + g * (HD / 8) + 2 * t) = make_float4(o[t][c], o[t][c + 2], o[t + 1][c], o[t + 1][c + 2]);
-                }
-                if (g == 0) {
-                    at[HD] = c == 0 ? top0 : top1;
-                    at[HD + 1] = c == 0 ? sum0 : sum1;
+                for (int x = 4; x < kWarp; x <<= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
+                const int column = n * kTileColumns + 2 * q4 + c;
+                if (column >= columns) continue;
+                if (whole) {
+                    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+                    for (int t = 0; t < kTiles; t += 4) {
+                        const float v[8] = {o[n][t][c] * inverse, o[n][t][c + 2] * inverse, o[n][t + 1][c] * inverse, o[n][t + 1][c + 2] * inverse,
+                                            o[n][t + 2][c] * inverse, o[n][t + 2][c + 2] * inverse, o[n][t + 3][c] * inverse, o[n][t + 3][c + 2] * inverse};
+                        write8(w.span.first, kv_head, block * kColumns + column, g * (HD / 8) + 2 * t, v);
+                    }
+                } else {
+                    float* const at = piece + column * kPitch;
+#pragma unroll
+                    for (int t = 0; t < kTiles; t += 2) {
+                        *reinterpret_cast<float4*>(at + g * (HD / 8) + 2 * t) = make_float4(o[n][t][c], o[n][t][c + 2], o[n][t + 1][c], o[n][t + 1][c + 2]);
+                    }
+                    if (g == 0) *reinterpret_cast<float2*>(at + HD) = make_float2(top[n][c], total);
                 }
             }
         }
@@ -405,6 +435,13 @@ __global__ void __launch_bounds__(kRowThreads, 2) kv8_rows_kernel(const Kv8Atten
     // ---- pieces of a segment that lie in this CTA stand in order; a warp a segment merges them
     float* const left = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + kCounterBytes);
     auto left_by = [&](int cta, int which) { return left + (size_t)(2 * cta + which) * kPiece; };
+    auto owner = [&](long long u) { return (int)(((u + 1) * ctas - 1) / units); };
+    auto finish = [&](const Piece& p, int column, int d, Merged& v) {
+        const float inverse = v.total == 0.0f ? 0.0f : 1.0f / v.total;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v.sum[e] *= inverse;
+        write8(p.first, p.kv_head, p.column + column, d, v.sum);
+    };
     {
         const long long mine = lane < 2 * kRowWarps ? held[lane].start : -1;
         const unsigned int real = __ballot_sync(0xffffffffu, mine >= 0);
@@ -423,111 +460,96 @@ __global__ void __launch_bounds__(kRowThreads, 2) kv8_rows_kernel(const Kv8Atten
             for (int x = lane; x < p.columns * (HD / 8); x += kWarp) {
                 const int column = x / (HD / 8), d = x % (HD / 8) * 8;
                 const float* const at = parts + column * kPitch;
-                float top = -INFINITY, total = 0.0f, v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-                for (unsigned int left_over = parts_here; left_over != 0u; left_over &= left_over - 1) {
-                    top = fmaxf(top, at[(__ffs(left_over) - 1) * kPiece + HD]);
-                }
-                for (unsigned int left_over = parts_here; left_over != 0u; left_over &= left_over - 1) {
-                    const float* const from = at + (__ffs(left_over) - 1) * kPiece;
-                    const float f = from[HD] == -INFINITY ? 0.0f : exp2_ftz(from[HD] - top);
-                    total = fmaf(f, from[HD + 1], total);
-                    const float4 lo = *reinterpret_cast<const float4*>(from + d), hi = *reinterpret_cast<const float4*>(from + d + 4);
-                    add8(v, f, lo, hi);
+                Merged v;
+                for (unsigned int rest = parts_here; rest != 0u; rest &= rest - 1) {
+                    const float* const from = at + (__ffs(rest) - 1) * kPiece;
+                    v.add(*reinterpret_cast<const float2*>(from + HD), *reinterpret_cast<const float4*>(from + d), *reinterpret_cast<const float4*>(from + d + 4));
                 }
                 if (whole) {
-                    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] *= inverse;
-                    write8(p.first, p.kv_head, p.column + column, d, v);
+                    finish(p, column, d, v);
                 } else {
-                    *reinterpret_cast<float4*>(to + column * kPitch + d) = make_float4(v[0], v[1], v[2], v[3]);
-                    *reinterpret_cast<float4*>(to + column * kPitch + d + 4) = make_float4(v[4], v[5], v[6], v[7]);
-                    if (d == 0) *reinterpret_cast<float2*>(to + column * kPitch + HD) = make_float2(top, total);
+                    *reinterpret_cast<float4*>(to + column * kPitch + d) = make_float4(v.sum[0], v.sum[1], v.sum[2], v.sum[3]);
+                    *reinterpret_cast<float4*>(to + column * kPitch + d + 4) = make_float4(v.sum[4], v.sum[5], v.sum[6], v.sum[7]);
+                    if (d == 0) *reinterpret_cast<float2*>(to + column * kPitch + HD) = make_float2(v.top, v.total);
                 }
             }
             if (!whole) {
+                // of the CTAs that share the segment the last one folds what they left
+                const int first_cta = owner(p.start), count = owner(p.start + p.pages - 1) - first_cta + 1;
+                pdl_wait();                                // the counters are zero
                 __threadfence();
-                if (lane == 0) beyond[which] = first;
+                __syncwarp();
+                if (lane == 0 && atomicAdd(static_cast<unsigned int*>(a.scratch) + first_cta, 1u) == (unsigned int)(count - 1)) folds[which] = first;
             }
         }
     }
-    pdl_wait();                                            // the counters are zero
+    pdl_wait();
     __syncthreads();
-    if (beyond[0] < 0 && beyond[1] < 0) {
-        pdl_trigger();
-        return;
-    }
-    // ---- of the CTAs that share a segment the last one folds what they left: half of the CTA for each of the two
-    constexpr int kHalf = kRowWarps / 2;
-    const int which = warp / kHalf, in_half = tid % (kRowThreads / 2);
-    const Piece p = held[max(beyond[which], 0)];
-    auto owner = [&](long long u) { return (int)(((u + 1) * ctas - 1) / units); };
-    const int first_cta = owner(p.start), count = owner(p.start + p.pages - 1) - first_cta + 1;
-    if (in_half == 0) tickets[which] = beyond[which] >= 0 ? (int)atomicAdd(static_cast<unsigned int*>(a.scratch) + first_cta, 1u) : -1;
-    __syncthreads();
-    const bool folds[2] = {tickets[0] >= 0, tickets[1] >= 0};
-    const bool mine = folds[which] && tickets[which] == count - 1;
-    if (!__syncthreads_or(mine)) {
+    const int folding = (folds[0] >= 0 ? 1 : 0) + (folds[1] >= 0 ? 1 : 0);
+    if (folding == 0) {
         pdl_trigger();
         return;
     }
     __threadfence();
-    // the segment begins in the first CTA's range, whose second piece it is
-    auto piece_of = [&](int n) { return left_by(first_cta + n, n == 0 ? 1 : 0); };
-    if (mine) {
-        for (int x = in_half; x < count * p.columns; x += kRowThreads / 2) {
-            fold_scale[which][x / p.columns][x % p.columns] = __ldcg(piece_of(x / p.columns) + x % p.columns * kPitch + HD);
-        }
-    }
-    __syncthreads();
-    const int share = warp % kHalf;                        // pieces share, share + kHalf, ...
-    if (mine) {
+    // all warps for one segment, half of them each for two; a warp takes pieces share, share + shares, ...
+    const int shares = kRowWarps / folding, share = warp % shares, which = folding == 2 ? warp / shares : (folds[0] >= 0 ? 0 : 1);
+    const Piece p = held[folds[which]];
+    {
+        const int first_cta = owner(p.start), count = owner(p.start + p.pages - 1) - first_cta + 1;
         for (int x = lane; x < p.columns * (HD / 8); x += kWarp) {
             const int column = x / (HD / 8), d = x % (HD / 8) * 8;
-            float top = -INFINITY, total = 0.0f, v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-            for (int n = 0; n < count; ++n) top = fmaxf(top, fold_scale[which][n][column]);
-#pragma unroll 4
-            for (int n = share; n < count; n += kHalf) {
-                const float* const from = piece_of(n) + column * kPitch;
-                const float piece_top = fold_scale[which][n][column], f = piece_top == -INFINITY ? 0.0f : exp2_ftz(piece_top - top);
-                const float4 lo = __ldcg(reinterpret_cast<const float4*>(from + d)), hi = __ldcg(reinterpret_cast<const float4*>(from + d + 4));
-                total = fmaf(f, __ldcg(from + HD + 1), total);
-                add8(v, f, lo, hi);
+            Merged v;
+            constexpr int kAtOnce = 4;
+            for (int n0 = share; n0 < count; n0 += kAtOnce * shares) {
+                float2 stats[kAtOnce];
+                float4 lo[kAtOnce], hi[kAtOnce];
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    const int n = n0 + i * shares;
+                    // (the segment begins in the first CTA's range, whose second piece it is)
+                    const float* const from = left_by(first_cta + min(n, count - 1), n == 0 ? 1 : 0) + column * kPitch;
+                    stats[i] = __ldcg(reinterpret_cast<const float2*>(from + HD));
+                    lo[i] = __ldcg(reinterpret_cast<const float4*>(from + d));
+                    hi[i] = __ldcg(reinterpret_cast<const float4*>(from + d + 4));
+                }
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    if (n0 + i * shares < count) v.add(stats[i], lo[i], hi[i]);
+                }
             }
             float* const to = parts + (size_t)warp * kPiece + column * kPitch;
-            *reinterpret_cast<float4*>(to + d) = make_float4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<float4*>(to + d + 4) = make_float4(v[4], v[5], v[6], v[7]);
-            if (d == 0) to[HD] = total;
+            *reinterpret_cast<float4*>(to + d) = make_float4(v.sum[0], v.sum[1], v.sum[2], v.sum[3]);
+            *reinterpret_cast<float4*>(to + d + 4) = make_float4(v.sum[4], v.sum[5], v.sum[6], v.sum[7]);
+            if (d == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(v.top, v.total);
         }
     }
     __syncthreads();
-    if (mine) {
-        for (int x = in_half; x < p.columns * (HD / 8); x += kRowThreads / 2) {
-            const int column = x / (HD / 8), d = x % (HD / 8) * 8;
-            float total = 0.0f, v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int n = 0; n < kHalf; ++n) {
-                const float* const from = parts + (size_t)(which * kHalf + n) * kPiece + column * kPitch;
-                total += from[HD];
-                add8(v, 1.0f, *reinterpret_cast<const float4*>(from + d), *reinterpret_cast<const float4*>(from + d + 4));
-            }
-            const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= inverse;
-            write8(p.first, p.kv_head, p.column + column, d, v);
+    for (int x = share * kWarp + lane; x < p.columns * (HD / 8); x += shares * kWarp) {
+        const int column = x / (HD / 8), d = x % (HD / 8) * 8;
+        Merged v;
+        for (int n = 0; n < shares; ++n) {
+            const float* const from = parts + (size_t)((folding == 2 ? which * shares : 0) + n) * kPiece + column * kPitch;
+            v.add(*reinterpret_cast<const float2*>(from + HD), *reinterpret_cast<const float4*>(from + d), *reinterpret_cast<const float4*>(from + d + 4));
         }
+        finish(p, column, d, v);
     }
     pdl_trigger();
 }
 
-template <int HD, bool E4M3>
+template <int HD, bool E4M3, int TILES>
 cudaError_t launch_rows(const Kv8AttentionArgs& a, cudaStream_t stream) {
     static std::atomic<unsigned long long> allowed{0};
-    cudaError_t e = kv8_allow_smem(allowed, kv8_rows_kernel<HD, E4M3>, (int)rows_smem<HD>(Q3T_MAX_TABLE_ROWS));
+    cudaError_t e = kv8_allow_smem(allowed, kv8_rows_kernel<HD, E4M3, TILES>, (int)rows_smem<HD, TILES>(Q3T_MAX_TABLE_ROWS));
     if (e == cudaSuccess) e = launch_zero_counters(static_cast<unsigned int*>(a.scratch), kRowCtas, stream);
     if (e != cudaSuccess) return e;
-    e = launch_pdl(kv8_rows_kernel<HD, E4M3>, dim3(kRowCtas), dim3(kRowThreads), rows_smem<HD>(a.rows), stream, a);
+    e = launch_pdl(kv8_rows_kernel<HD, E4M3, TILES>, dim3(148 * rows_residency<HD, TILES>()), dim3(kRowThreads), rows_smem<HD, TILES>(a.rows), stream, a);
     return e != cudaSuccess || !a.prompts ? e : launch_kv8_prompts(a, HD, E4M3, stream);
+}
+
+template <int HD, bool E4M3>
+cudaError_t launch_attention(const Kv8AttentionArgs& a, cudaStream_t stream) {
+    // two tiles of columns a warp where rows may have more than one: what a page costs to read and to convert is paid once
+    return (long long)a.most * (a.query_heads / a.cache.heads) > kTileColumns ? launch_rows<HD, E4M3, 2>(a, stream) : launch_rows<HD, E4M3, 1>(a, stream);
 }
 
 // false: refused
@@ -584,7 +606,7 @@ extern "C" uint32_t q3t_kv8_page_error_count(void) {
 extern "C" size_t q3t_kv8_attention_scratch_bytes(const Q3tKv8AttentionDesc* desc) {
     q3t::Kv8AttentionArgs a;
     if (!q3t::attention_args(desc, &a)) return 0;
-    return q3t::kCounterBytes + (size_t)q3t::kRowCtas * 2 * q3t::kColumns * (desc->cache->head_dimension + 4) * sizeof(float);
+    return q3t::kCounterBytes + (size_t)q3t::kRowCtas * 2 * 2 * q3t::kTileColumns * (desc->cache->head_dimension + 4) * sizeof(float);
 }
 
 extern "C" int32_t q3t_launch_kv8_attention(const Q3tKv8AttentionDesc* desc, void* stream) {
@@ -599,6 +621,6 @@ extern "C" int32_t q3t_launch_kv8_attention(const Q3tKv8AttentionDesc* desc, voi
     a.prompts = (long long)a.most * (a.query_heads / a.cache.heads) > kKv8RowColumns ? 1 : 0;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool e4m3 = desc->cache->format == Q3T_KV8_E4M3;
-    if (desc->cache->head_dimension == 128) return static_cast<int32_t>(e4m3 ? launch_rows<128, true>(a, s) : launch_rows<128, false>(a, s));
-    return static_cast<int32_t>(e4m3 ? launch_rows<64, true>(a, s) : launch_rows<64, false>(a, s));
+    if (desc->cache->head_dimension == 128) return static_cast<int32_t>(e4m3 ? launch_attention<128, true>(a, s) : launch_attention<128, false>(a, s));
+    return static_cast<int32_t>(e4m3 ? launch_attention<64, true>(a, s) : launch_attention<64, false>(a, s));
 }
