@@ -31,6 +31,7 @@ constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / kWarp;
 constexpr int kRowCtas = 2 * 148;
 constexpr int kTileColumns = 8;                        // of a product
+constexpr int kStartUnits = 2;                         // what the start of a segment counts for in the cut, in pages
 constexpr int kCounterBytes = (kRowCtas * 4 + 255) / 256 * 256;
 
 __device__ unsigned int g_kv8_range_errors = 0;
@@ -86,9 +87,15 @@ __device__ __forceinline__ RowWork row_work(const Kv8AttentionArgs& a, int row, 
     return w;
 }
 
+// 64-bit divisions take hundreds of instructions, where a CTA has nothing else to do; most fit 32 bits
+__device__ __forceinline__ long long quotient(long long x, long long y) {
+    return ((x | y) >> 32) == 0 ? (long long)((unsigned int)x / (unsigned int)y) : x / y;
+}
+__device__ __forceinline__ long long share_of(long long units, int n, int of) { return quotient(units * n, of); }
+
 // A part of a segment, (row, KV head, block of columns): whose it is
 struct Piece {
-    long long start;   // first unit of the segment, -1: none
+    long long start;   // unit of the segment's first page, -1: none
     int pages;         // of the segment
     int first;         // number of the row's first new token
     int kv_head;
@@ -128,14 +135,14 @@ __global__ void __launch_bounds__(kRowThreads, rows_residency<HD, TILES>()) kv8_
         pdl_wait();
         pdl_trigger();
     }
-    // ---- the batch's units (pages of a segment), as prefix sums over the rows; the first CTA counts what lies outside the host's bounds
+    // ---- the batch's units (of a segment its start, then its pages), as prefix sums over the rows; the first CTA counts what lies outside the host's bounds
     long long sum = 0;
     for (int first = 0; first < a.rows; first += kRowThreads) {
         const int row = first + tid;
         long long mine = 0;
         if (row < a.rows) {
             const RowWork w = row_work(a, row, group, kColumns);
-            mine = (long long)w.blocks * heads * w.pages;
+            mine = (long long)w.blocks * heads * (w.pages + kStartUnits);
             if (w.span.cut && blockIdx.x == 0) atomicAdd(&g_kv8_range_errors, 1u);
         }
 #pragma unroll
@@ -156,7 +163,7 @@ __global__ void __launch_bounds__(kRowThreads, rows_residency<HD, TILES>()) kv8_
         pdl_wait();
         return;
     }
-    const long long cta_first = units * blockIdx.x / ctas, cta_end = units * (blockIdx.x + 1) / ctas;
+    const long long cta_first = share_of(units, (int)blockIdx.x, ctas), cta_end = share_of(units, (int)blockIdx.x + 1, ctas);
     long long unit = cta_first + (cta_end - cta_first) * warp / kRowWarps;
     const long long unit_end = cta_first + (cta_end - cta_first) * (warp + 1) / kRowWarps;
     int row;
@@ -192,10 +199,12 @@ __global__ void __launch_bounds__(kRowThreads, rows_residency<HD, TILES>()) kv8_
         while (before[row] <= unit) ++row;
         const RowWork w = row_work(a, row, group, kColumns);
         const long long row_first = row > 0 ? before[row - 1] : 0;
-        const int segment = (int)((unit - row_first) / w.pages);              // (KV head, block of columns)
-        const long long start = row_first + (long long)segment * w.pages;
-        const int page_first = (int)(unit - start);
-        const int page_end = (int)min((long long)w.pages, page_first + (unit_end - unit));
+        const int segment = (int)quotient(unit - row_first, w.pages + kStartUnits);          // (KV head, block of columns)
+        const long long start = row_first + (long long)segment * (w.pages + kStartUnits) + kStartUnits;
+        const int page_first = (int)max(unit - start, 0ll);
+        const int page_end = (int)min((long long)w.pages, unit_end - start);
+        unit = start + w.pages;
+        if (page_end <= page_first) continue;
         const int kv_head = segment / w.blocks, block = segment - kv_head * w.blocks;
         const int columns = min(kColumns, w.span.count * group - block * kColumns);
 
@@ -428,14 +437,14 @@ __global__ void __launch_bounds__(kRowThreads, rows_residency<HD, TILES>()) kv8_
             if (lane == 0) held[2 * warp + pieces_held] = Piece{start, w.pages, w.span.first, kv_head, block * kColumns, columns};
             ++pieces_held;
         }
-        unit += page_end - page_first;
     }
     __syncthreads();
 
     // ---- pieces of a segment that lie in this CTA stand in order; a warp a segment merges them
     float* const left = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + kCounterBytes);
     auto left_by = [&](int cta, int which) { return left + (size_t)(2 * cta + which) * kPiece; };
-    auto owner = [&](long long u) { return (int)(((u + 1) * ctas - 1) / units); };
+    // the CTA whose range has a unit
+    auto owner = [&](long long u) { return u >= cta_first && u < cta_end ? (int)blockIdx.x : (int)quotient((u + 1) * ctas - 1, units); };
     auto finish = [&](const Piece& p, int column, int d, Merged& v) {
         const float inverse = v.total == 0.0f ? 0.0f : 1.0f / v.total;
 #pragma unroll
