@@ -18,6 +18,7 @@
 
 #include "kv8.cuh"
 #include "q3t_kernels.cuh"
+#include "q3t_tcgen05.cuh"
 
 #include <climits>
 
@@ -32,6 +33,8 @@ constexpr int kRowWarps = kRowThreads / kWarp;
 constexpr int kRowCtas = 2 * 148;
 constexpr int kTileColumns = 8;                        // of a product
 constexpr int kStartUnits = 2;                         // what the start of a segment counts for in the cut, in pages
+constexpr int kClusterCtas = 8;
+constexpr int kFewTokens = 8192;                       // of a row, up to which a cluster a segment is the shortest way
 constexpr int kCounterBytes = (kRowCtas * 4 + 255) / 256 * 256;
 
 __device__ unsigned int g_kv8_range_errors = 0;
@@ -53,6 +56,18 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 __device__ __forceinline__ int4 load16(const uint8_t* p) {
     int4 v;
     asm volatile("ld.global.L1::no_allocate.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// of another CTA's shared memory
+__device__ __forceinline__ float2 peer_float2(uint32_t at) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 peer_float4(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
     return v;
 }
 
@@ -87,128 +102,57 @@ __device__ __forceinline__ RowWork row_work(const Kv8AttentionArgs& a, int row, 
     return w;
 }
 
-// 64-bit divisions take hundreds of instructions, where a CTA has nothing else to do; most fit 32 bits
-__device__ __forceinline__ long long quotient(long long x, long long y) {
-    return ((x | y) >> 32) == 0 ? (long long)((unsigned int)x / (unsigned int)y) : x / y;
-}
-__device__ __forceinline__ long long share_of(long long units, int n, int of) { return quotient(units * n, of); }
-
-// A part of a segment, (row, KV head, block of columns): whose it is
-struct Piece {
-    long long start;   // unit of the segment's first page, -1: none
-    int pages;         // of the segment
-    int first;         // number of the row's first new token
-    int kv_head;
-    int column;        // of the row and KV head: the segment's first
-    int columns;       // of the segment
+// A segment, (row, KV head, block of columns), of which a warp takes some pages
+struct Segment {
+    int row, kv_head;
+    int column;        // of the row and KV head: the first
+    int columns;
+    bool counts;       // its pages that are not there
 };
 
-template <int HD, int TILES>
-constexpr size_t rows_smem(int rows) {
-    return (size_t)rows * sizeof(long long) + (size_t)2 * kRowWarps * TILES * kTileColumns * (HD + 4) * sizeof(float);
-}
-// CTAs of an SM: a warp of two tiles of columns and heads of 128 holds twice the outputs and queries
-template <int HD, int TILES>
-constexpr int rows_residency() {
-    return HD == 128 && TILES == 2 ? 1 : 2;
+// 8 dims of a column of a row and KV head, from where its new tokens begin
+template <int HD>
+__device__ __forceinline__ void write8(const Kv8AttentionArgs& a, int first, int kv_head, int column, int d, const float (&v)[8]) {
+    const int group = a.query_heads / a.cache.heads, i = column / group;
+    const size_t token = first + i, at = (size_t)(kv_head * group + column - i * group) * HD + d;
+    __nv_bfloat162 x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+    *reinterpret_cast<int4*>(a.out + token * a.out_stride + at) = *reinterpret_cast<const int4*>(x);
+    if (a.out32 != nullptr) {
+        float* const to = a.out32 + token * a.query_heads * HD + at;
+        *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(to + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    }
 }
 
+// A warp's way through pages of a segment.  Lane 4 g + q4 holds dims g * HD / 8 and on of columns 2 q4 and + 1 of each tile.
 template <int HD, bool E4M3, int TILES>
-__global__ void __launch_bounds__(kRowThreads, rows_residency<HD, TILES>()) kv8_rows_kernel(const Kv8AttentionArgs a) {
-    constexpr int kColumns = TILES * kTileColumns;
-    constexpr int kParts = HD / 64;                    // 16-byte pieces of a key that a lane holds
-    constexpr int kTiles = HD / 16;                    // of 16 dims
-    constexpr int kWords = HD / 32;                    // of a value's dims that a lane holds
-    constexpr int kPitch = HD + 4;                     // of a column of a piece: its output, then top and sum
-    constexpr int kPiece = kColumns * kPitch;
-    extern __shared__ __align__(16) unsigned char smem[];
-    float* const parts = reinterpret_cast<float*>(smem);                                    // [warp][2] pieces
-    long long* const before = reinterpret_cast<long long*>(parts + 2 * kRowWarps * kPiece);  // [rows]: units of the rows up to each
-    __shared__ Piece held[2 * kRowWarps];
-    __shared__ long long scan[kRowWarps];
-    __shared__ int folds[2];                           // of the segments that go beyond the CTA at its start and its end: the piece, if it is up to this CTA
-    const int tid = threadIdx.x, lane = tid % kWarp, warp = __shfl_sync(0xffffffffu, tid / kWarp, 0);
-    const int g = lane >> 2, q4 = lane & 3;
-    const int heads = a.cache.heads, group = a.query_heads / heads;
+struct Walk {
+    static constexpr int kColumns = TILES * kTileColumns;
+    static constexpr int kParts = HD / 64;             // 16-byte pieces of a key that a lane holds
+    static constexpr int kTiles = HD / 16;             // of 16 dims
+    static constexpr int kWords = HD / 32;             // of a value's dims that a lane holds
+    static constexpr int kPitch = HD + 4;              // of a column of a piece: its output, then reference and sum
+    static constexpr int kPiece = kColumns * kPitch;
+    float o[TILES][kTiles][4], top[TILES][2], sum_of[TILES][2];
 
-    if (a.prompts) {                                   // (they may run beside this one)
-        pdl_wait();
-        pdl_trigger();
-    }
-    // ---- the batch's units (of a segment its start, then its pages), as prefix sums over the rows; the first CTA counts what lies outside the host's bounds
-    long long sum = 0;
-    for (int first = 0; first < a.rows; first += kRowThreads) {
-        const int row = first + tid;
-        long long mine = 0;
-        if (row < a.rows) {
-            const RowWork w = row_work(a, row, group, kColumns);
-            mine = (long long)w.blocks * heads * (w.pages + kStartUnits);
-            if (w.span.cut && blockIdx.x == 0) atomicAdd(&g_kv8_range_errors, 1u);
-        }
+    __device__ __forceinline__ Walk() {
 #pragma unroll
-        for (int o = 1; o < kWarp; o <<= 1) {
-            const long long other = __shfl_up_sync(0xffffffffu, mine, o);
-            if (lane >= o) mine += other;
-        }
-        if (lane == kWarp - 1) scan[warp] = mine;
-        __syncthreads();
-        for (int w = 0; w < warp; ++w) mine += scan[w];
-        if (row < a.rows) before[row] = sum + mine;
-        for (int w = 0; w < kRowWarps; ++w) sum += scan[w];
-        __syncthreads();
-    }
-    const long long units = sum;
-    const int ctas = (int)min((long long)gridDim.x, (units + kRowWarps - 1) / kRowWarps);
-    if ((int)blockIdx.x >= ctas) {
-        pdl_wait();
-        return;
-    }
-    const long long cta_first = share_of(units, (int)blockIdx.x, ctas), cta_end = share_of(units, (int)blockIdx.x + 1, ctas);
-    long long unit = cta_first + (cta_end - cta_first) * warp / kRowWarps;
-    const long long unit_end = cta_first + (cta_end - cta_first) * (warp + 1) / kRowWarps;
-    int row;
-    {
-        int low = 0, high = a.rows - 1;
-        while (low < high) {
-            const int middle = (low + high) >> 1;
-            if (before[middle] > unit) high = middle;
-            else low = middle + 1;
-        }
-        row = low;
-    }
-    // 8 dims of a column
-    auto write8 = [&](int first, int kv_head, int column, int d, const float (&v)[8]) {
-        const int i = column / group;
-        const size_t token = first + i, at = (size_t)(kv_head * group + column - i * group) * HD + d;
-        __nv_bfloat162 x[4];
+        for (int n = 0; n < TILES; ++n) {
+            top[n][0] = top[n][1] = -INFINITY;
+            sum_of[n][0] = sum_of[n][1] = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
-        *reinterpret_cast<int4*>(a.out + token * a.out_stride + at) = *reinterpret_cast<const int4*>(x);
-        if (a.out32 != nullptr) {
-            float* const to = a.out32 + token * a.query_heads * HD + at;
-            *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<float4*>(to + 4) = make_float4(v[4], v[5], v[6], v[7]);
+            for (int t = 0; t < kTiles; ++t) o[n][t][0] = o[n][t][1] = o[n][t][2] = o[n][t][3] = 0.0f;
         }
-    };
-    if (tid < 2) folds[tid] = -1;
-    if (lane < 2) held[2 * warp + lane].start = -1;
-    __syncwarp();
+    }
 
-    int pieces_held = 0;
-    while (unit < unit_end) {
-        while (before[row] <= unit) ++row;
-        const RowWork w = row_work(a, row, group, kColumns);
-        const long long row_first = row > 0 ? before[row - 1] : 0;
-        const int segment = (int)quotient(unit - row_first, w.pages + kStartUnits);          // (KV head, block of columns)
-        const long long start = row_first + (long long)segment * (w.pages + kStartUnits) + kStartUnits;
-        const int page_first = (int)max(unit - start, 0ll);
-        const int page_end = (int)min((long long)w.pages, unit_end - start);
-        unit = start + w.pages;
-        if (page_end <= page_first) continue;
-        const int kv_head = segment / w.blocks, block = segment - kv_head * w.blocks;
-        const int columns = min(kColumns, w.span.count * group - block * kColumns);
-
+    // pages page_first .. page_end - 1, at least one
+    __device__ __forceinline__ void run(const Kv8AttentionArgs& a, const RowWork& w, const Segment& of, int page_first, int page_end) {
+        const int row = of.row, kv_head = of.kv_head, columns = of.columns;
+        const bool counts = of.counts;
         // ---- pages: their ids a lane each, 32 at a time (one that is not there is read as page 0 and masked)
+        const int lane = threadIdx.x % kWarp, g = lane >> 2, q4 = lane & 3, group = a.query_heads / a.cache.heads;
         const int* const ids_at = a.table + (size_t)row * a.table_stride;
         auto usable = [&](int id) { return id >= 0 && id < a.cache.pages; };
         auto ids_from = [&](int first) { return first + lane < page_end && (first + lane) * kPageTokens < w.last ? ids_at[first + lane] : -1; };
@@ -221,7 +165,7 @@ __global__ void __launch_bounds__(kRowThreads, rows_residency<HD, TILES>()) kv8_
         int4 raw[TILES][kParts][2];
 #pragma unroll
         for (int n = 0; n < TILES; ++n) {
-            const int of_block = n * kTileColumns + g, column = block * kColumns + of_block;
+            const int of_block = n * kTileColumns + g, column = of.column + of_block;
             const bool real = of_block < columns;
             const int i = real ? column / group : 0;
             const bf16* q = a.query + (size_t)(w.span.first + i) * a.query_stride + (size_t)(kv_head * group + column % group) * HD + q4 * 16;
@@ -292,7 +236,7 @@ __global__ void __launch_bounds__(kRowThreads, rows_residency<HD, TILES>()) kv8_
             }
         }
         // of the columns whose scores this lane gets, 2 q4 and + 1 of each tile
-        float scale_of[TILES][2], top[TILES][2], sum_of[TILES][2], o[TILES][kTiles][4];
+        float scale_of[TILES][2];
         int seen[TILES][2];
 #pragma unroll
         for (int n = 0; n < TILES; ++n) {
@@ -300,16 +244,12 @@ __global__ void __launch_bounds__(kRowThreads, rows_residency<HD, TILES>()) kv8_
             for (int c = 0; c < 2; ++c) {
                 scale_of[n][c] = __shfl_sync(0xffffffffu, column_scale[n], 8 * q4 + 4 * c);
                 seen[n][c] = __shfl_sync(0xffffffffu, column_seen[n], 8 * q4 + 4 * c);
-                top[n][c] = -INFINITY;
-                sum_of[n][c] = 0.0f;
             }
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t) o[n][t][0] = o[n][t][1] = o[n][t][2] = o[n][t][3] = 0.0f;
         }
 
         for (int page = page_first; page < page_end; ++page) {
             const bool there = usable(raw_id);
-            if (!there && segment == 0 && lane == 0 && page * kPageTokens < w.last) atomicAdd(&g_kv8_page_errors, 1u);
+            if (!there && counts && lane == 0 && page * kPageTokens < w.last) atomicAdd(&g_kv8_page_errors, 1u);
             const int next = page + 1 - page_first;
             if ((next & 31) == 0) ids = ids_from(page + 1);
             const int next_raw = __shfl_sync(0xffffffffu, ids, next & 31);
@@ -403,9 +343,11 @@ __global__ void __launch_bounds__(kRowThreads, rows_residency<HD, TILES>()) kv8_
             if (more) load_values(next_id);
             raw_id = next_raw;
         }
-        // ---- whole: written; cut: into shared memory
-        const bool whole = page_first == 0 && page_end == w.pages;
-        float* const piece = parts + (size_t)(2 * warp + pieces_held) * kPiece;
+    }
+
+    // into shared memory
+    __device__ __forceinline__ void keep(float* piece, int columns) const {
+        const int lane = threadIdx.x % kWarp, g = lane >> 2, q4 = lane & 3;
 #pragma unroll
         for (int n = 0; n < TILES; ++n) {
 #pragma unroll
@@ -415,25 +357,152 @@ __global__ void __launch_bounds__(kRowThreads, rows_residency<HD, TILES>()) kv8_
                 for (int x = 4; x < kWarp; x <<= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
                 const int column = n * kTileColumns + 2 * q4 + c;
                 if (column >= columns) continue;
-                if (whole) {
-                    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+                float* const at = piece + column * kPitch;
 #pragma unroll
-                    for (int t = 0; t < kTiles; t += 4) {
-                        const float v[8] = {o[n][t][c] * inverse, o[n][t][c + 2] * inverse, o[n][t + 1][c] * inverse, o[n][t + 1][c + 2] * inverse,
-                                            o[n][t + 2][c] * inverse, o[n][t + 2][c + 2] * inverse, o[n][t + 3][c] * inverse, o[n][t + 3][c + 2] * inverse};
-                        write8(w.span.first, kv_head, block * kColumns + column, g * (HD / 8) + 2 * t, v);
-                    }
-                } else {
-                    float* const at = piece + column * kPitch;
+                for (int t = 0; t < kTiles; t += 2) {
+                    *reinterpret_cast<float4*>(at + g * (HD / 8) + 2 * t) = make_float4(o[n][t][c], o[n][t][c + 2], o[n][t + 1][c], o[n][t + 1][c + 2]);
+                }
+                if (g == 0) *reinterpret_cast<float2*>(at + HD) = make_float2(top[n][c], total);
+            }
+        }
+    }
+
+    // a whole segment
+    __device__ __forceinline__ void write(const Kv8AttentionArgs& a, int first, const Segment& of) const {
+        const int lane = threadIdx.x % kWarp, g = lane >> 2, q4 = lane & 3;
 #pragma unroll
-                    for (int t = 0; t < kTiles; t += 2) {
-                        *reinterpret_cast<float4*>(at + g * (HD / 8) + 2 * t) = make_float4(o[n][t][c], o[n][t][c + 2], o[n][t + 1][c], o[n][t + 1][c + 2]);
-                    }
-                    if (g == 0) *reinterpret_cast<float2*>(at + HD) = make_float2(top[n][c], total);
+        for (int n = 0; n < TILES; ++n) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float total = sum_of[n][c];
+#pragma unroll
+                for (int x = 4; x < kWarp; x <<= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
+                const int column = n * kTileColumns + 2 * q4 + c;
+                if (column >= of.columns) continue;
+                const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+                for (int t = 0; t < kTiles; t += 4) {
+                    const float v[8] = {o[n][t][c] * inverse, o[n][t][c + 2] * inverse, o[n][t + 1][c] * inverse, o[n][t + 1][c + 2] * inverse,
+                                        o[n][t + 2][c] * inverse, o[n][t + 2][c + 2] * inverse, o[n][t + 3][c] * inverse, o[n][t + 3][c + 2] * inverse};
+                    write8<HD>(a, first, of.kv_head, of.column + column, g * (HD / 8) + 2 * t, v);
                 }
             }
         }
-        if (!whole) {
+    }
+};
+
+// 64-bit divisions take hundreds of instructions, where a CTA has nothing else to do; most fit 32 bits
+__device__ __forceinline__ long long quotient(long long x, long long y) {
+    return ((x | y) >> 32) == 0 ? (long long)((unsigned int)x / (unsigned int)y) : x / y;
+}
+__device__ __forceinline__ long long share_of(long long units, int n, int of) { return quotient(units * n, of); }
+
+// The tickets of the launch behind it, which is let in at once and waits for this one before anything else: it lies in wait on the SMs
+// while the launch ahead of both ends
+__global__ void kv8_zero_tickets_kernel(unsigned int* tickets) {
+    pdl_trigger();
+    pdl_wait();
+    tickets[threadIdx.x] = 0u;
+}
+
+// A part of a segment, (row, KV head, block of columns): whose it is
+struct Piece {
+    long long start;   // unit of the segment's first page, -1: none
+    int pages;         // of the segment
+    int first;         // number of the row's first new token
+    int kv_head;
+    int column;        // of the row and KV head: the segment's first
+    int columns;       // of the segment
+};
+
+template <int HD, int TILES>
+constexpr size_t rows_smem(int rows) {
+    return (size_t)rows * sizeof(long long) + (size_t)2 * kRowWarps * TILES * kTileColumns * (HD + 4) * sizeof(float);
+}
+// CTAs of an SM: a warp of two tiles of columns and heads of 128 holds twice the outputs and queries
+template <int HD, int TILES>
+constexpr int rows_residency() {
+    return HD == 128 && TILES == 2 ? 1 : 2;
+}
+
+template <int HD, bool E4M3, int TILES>
+__global__ void __launch_bounds__(kRowThreads, rows_residency<HD, TILES>()) kv8_rows_kernel(const Kv8AttentionArgs a) {
+    constexpr int kColumns = TILES * kTileColumns, kPitch = Walk<HD, E4M3, TILES>::kPitch, kPiece = Walk<HD, E4M3, TILES>::kPiece;
+    extern __shared__ __align__(16) unsigned char smem[];
+    float* const parts = reinterpret_cast<float*>(smem);                                    // [warp][2] pieces
+    long long* const before = reinterpret_cast<long long*>(parts + 2 * kRowWarps * kPiece);  // [rows]: units of the rows up to each
+    __shared__ Piece held[2 * kRowWarps];
+    __shared__ long long scan[kRowWarps];
+    __shared__ int folds[2];                           // of the segments that go beyond the CTA at its start and its end: the piece, if it is up to this CTA
+    const int tid = threadIdx.x, lane = tid % kWarp, warp = __shfl_sync(0xffffffffu, tid / kWarp, 0);
+    const int heads = a.cache.heads, group = a.query_heads / heads;
+
+    pdl_wait();
+    if (a.prompts) pdl_trigger();                      // (they may run beside this one)
+    // ---- the batch's units (of a segment its start, then its pages), as prefix sums over the rows; the first CTA counts what lies outside the host's bounds
+    long long sum = 0;
+    for (int first = 0; first < a.rows; first += kRowThreads) {
+        const int row = first + tid;
+        long long mine = 0;
+        if (row < a.rows) {
+            const RowWork w = row_work(a, row, group, kColumns);
+            mine = (long long)w.blocks * heads * (w.pages + kStartUnits);
+            if (w.span.cut && blockIdx.x == 0) atomicAdd(&g_kv8_range_errors, 1u);
+        }
+#pragma unroll
+        for (int o = 1; o < kWarp; o <<= 1) {
+            const long long other = __shfl_up_sync(0xffffffffu, mine, o);
+            if (lane >= o) mine += other;
+        }
+        if (lane == kWarp - 1) scan[warp] = mine;
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) mine += scan[w];
+        if (row < a.rows) before[row] = sum + mine;
+        for (int w = 0; w < kRowWarps; ++w) sum += scan[w];
+        __syncthreads();
+    }
+    const long long units = sum;
+    const int ctas = (int)min((long long)gridDim.x, (units + kRowWarps - 1) / kRowWarps);
+    if ((int)blockIdx.x >= ctas) return;
+    const long long cta_first = share_of(units, (int)blockIdx.x, ctas), cta_end = share_of(units, (int)blockIdx.x + 1, ctas);
+    long long unit = cta_first + (cta_end - cta_first) * warp / kRowWarps;
+    const long long unit_end = cta_first + (cta_end - cta_first) * (warp + 1) / kRowWarps;
+    int row;
+    {
+        int low = 0, high = a.rows - 1;
+        while (low < high) {
+            const int middle = (low + high) >> 1;
+            if (before[middle] > unit) high = middle;
+            else low = middle + 1;
+        }
+        row = low;
+    }
+    if (tid < 2) folds[tid] = -1;
+    if (lane < 2) held[2 * warp + lane].start = -1;
+    __syncwarp();
+
+    int pieces_held = 0;
+    while (unit < unit_end) {
+        while (before[row] <= unit) ++row;
+        const RowWork w = row_work(a, row, group, kColumns);
+        const long long row_first = row > 0 ? before[row - 1] : 0;
+        const int segment = (int)quotient(unit - row_first, w.pages + kStartUnits);          // (KV head, block of columns)
+        const long long start = row_first + (long long)segment * (w.pages + kStartUnits) + kStartUnits;
+        const int page_first = (int)max(unit - start, 0ll);
+        const int page_end = (int)min((long long)w.pages, unit_end - start);
+        unit = start + w.pages;
+        if (page_end <= page_first) continue;
+        const int kv_head = segment / w.blocks, block = segment - kv_head * w.blocks;
+        const int columns = min(kColumns, w.span.count * group - block * kColumns);
+
+        const Segment of{row, kv_head, block * kColumns, columns, segment == 0};
+        Walk<HD, E4M3, TILES> walk;
+        walk.run(a, w, of, page_first, page_end);
+        // ---- whole: written; cut: into shared memory
+        if (page_first == 0 && page_end == w.pages) {
+            walk.write(a, w.span.first, of);
+        } else {
+            walk.keep(parts + (size_t)(2 * warp + pieces_held) * kPiece, columns);
             if (lane == 0) held[2 * warp + pieces_held] = Piece{start, w.pages, w.span.first, kv_head, block * kColumns, columns};
             ++pieces_held;
         }
@@ -449,7 +518,7 @@ __global__ void __launch_bounds__(kRowThreads, rows_residency<HD, TILES>()) kv8_
         const float inverse = v.total == 0.0f ? 0.0f : 1.0f / v.total;
 #pragma unroll
         for (int e = 0; e < 8; ++e) v.sum[e] *= inverse;
-        write8(p.first, p.kv_head, p.column + column, d, v.sum);
+        write8<HD>(a, p.first, p.kv_head, p.column + column, d, v.sum);
     };
     {
         const long long mine = lane < 2 * kRowWarps ? held[lane].start : -1;
@@ -485,14 +554,12 @@ __global__ void __launch_bounds__(kRowThreads, rows_residency<HD, TILES>()) kv8_
             if (!whole) {
                 // of the CTAs that share the segment the last one folds what they left
                 const int first_cta = owner(p.start), count = owner(p.start + p.pages - 1) - first_cta + 1;
-                pdl_wait();                                // the counters are zero
                 __threadfence();
                 __syncwarp();
                 if (lane == 0 && atomicAdd(static_cast<unsigned int*>(a.scratch) + first_cta, 1u) == (unsigned int)(count - 1)) folds[which] = first;
             }
         }
     }
-    pdl_wait();
     __syncthreads();
     const int folding = (folds[0] >= 0 ? 1 : 0) + (folds[1] >= 0 ? 1 : 0);
     if (folding == 0) {
@@ -545,11 +612,79 @@ __global__ void __launch_bounds__(kRowThreads, rows_residency<HD, TILES>()) kv8_
     pdl_trigger();
 }
 
+// Few segments (one listener, or a few): a cluster each, whose 64 warps share its pages.  What they leave is merged through distributed
+// shared memory: no sums over the batch, no tickets, no way through the L2 and back.
+template <int HD, bool E4M3, int TILES>
+__global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kRowThreads, rows_residency<HD, TILES>()) kv8_few_rows_kernel(const Kv8AttentionArgs a, int blocks) {
+    using W = Walk<HD, E4M3, TILES>;
+    constexpr int kWarpsOf = kClusterCtas * kRowWarps, kItems = HD / 8;                    // of a segment; of a column
+    extern __shared__ __align__(16) unsigned char smem[];
+    float* const parts = reinterpret_cast<float*>(smem);                                    // a piece a warp, then the CTA's
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid / kWarp, 0);
+    const int heads = a.cache.heads, group = a.query_heads / heads;
+    const int rank = (int)(blockIdx.x % kClusterCtas), number = (int)(blockIdx.x / kClusterCtas), block = number % blocks;
+    const int kv_head = number / blocks % heads, row = number / blocks / heads;
+    pdl_wait();
+    pdl_trigger();
+    const RowWork w = row_work(a, row, group, W::kColumns);
+    if (w.span.cut && tid == 0 && rank == 0 && block == 0 && kv_head == 0) atomicAdd(&g_kv8_range_errors, 1u);
+    if (block >= w.blocks) return;                                                          // the whole cluster
+    const Segment of{row, kv_head, block * W::kColumns, min(W::kColumns, w.span.count * group - block * W::kColumns), kv_head == 0 && block == 0};
+    const int which = rank * kRowWarps + warp;
+    const int page_first = (int)((long long)w.pages * which / kWarpsOf), page_end = (int)((long long)w.pages * (which + 1) / kWarpsOf);
+    {
+        W walk;
+        if (page_first < page_end) walk.run(a, w, of, page_first, page_end);
+        walk.keep(parts + (size_t)warp * W::kPiece, of.columns);
+    }
+    __syncthreads();
+    float* const own = parts + (size_t)kRowWarps * W::kPiece;
+    for (int x = tid; x < of.columns * kItems; x += kRowThreads) {
+        const int column = x / kItems, d = x % kItems * 8;
+        Merged v;
+#pragma unroll
+        for (int n = 0; n < kRowWarps; ++n) {
+            const float* const from = parts + (size_t)n * W::kPiece + column * W::kPitch;
+            v.add(*reinterpret_cast<const float2*>(from + HD), *reinterpret_cast<const float4*>(from + d), *reinterpret_cast<const float4*>(from + d + 4));
+        }
+        float* const to = own + column * W::kPitch;
+        *reinterpret_cast<float4*>(to + d) = make_float4(v.sum[0], v.sum[1], v.sum[2], v.sum[3]);
+        *reinterpret_cast<float4*>(to + d + 4) = make_float4(v.sum[4], v.sum[5], v.sum[6], v.sum[7]);
+        if (d == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(v.top, v.total);
+    }
+    tc::cluster_sync();
+    for (int x = tid * kClusterCtas + rank; x < of.columns * kItems; x += kRowThreads * kClusterCtas) {
+        const int column = x / kItems, d = x % kItems * 8;
+        Merged v;
+#pragma unroll
+        for (int n = 0; n < kClusterCtas; ++n) {
+            const uint32_t from = tc::peer_smem(tc::smem_u32(own + column * W::kPitch), (uint32_t)n);
+            v.add(peer_float2(from + HD * 4), peer_float4(from + d * 4), peer_float4(from + d * 4 + 16));
+        }
+        const float inverse = v.total == 0.0f ? 0.0f : 1.0f / v.total;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v.sum[e] *= inverse;
+        write8<HD>(a, w.span.first, kv_head, of.column + column, d, v.sum);
+    }
+    tc::cluster_sync();                                                                     // no CTA leaves while another reads its memory
+}
+
 template <int HD, bool E4M3, int TILES>
 cudaError_t launch_rows(const Kv8AttentionArgs& a, cudaStream_t stream) {
+    constexpr int kPiece = Walk<HD, E4M3, TILES>::kPiece;
+    // segments: as many clusters as are resident at once, and pages of 8 to a warp at most
+    const long long blocks = ((long long)a.most * (a.query_heads / a.cache.heads) + TILES * kTileColumns - 1) / (TILES * kTileColumns);
+    const long long clusters = blocks * a.cache.heads * a.rows;
+    if (!a.prompts && clusters * kClusterCtas <= 148 * rows_residency<HD, TILES>() && a.max_sequence <= kFewTokens) {
+        static std::atomic<unsigned long long> allowed{0};
+        constexpr int kBytes = (kRowWarps + 1) * kPiece * (int)sizeof(float);
+        const cudaError_t e = kv8_allow_smem(allowed, kv8_few_rows_kernel<HD, E4M3, TILES>, kBytes);
+        return e != cudaSuccess ? e : launch_pdl(kv8_few_rows_kernel<HD, E4M3, TILES>, dim3((unsigned)(clusters * kClusterCtas)), dim3(kRowThreads), kBytes, stream,
+                                                 a, (int)blocks);
+    }
     static std::atomic<unsigned long long> allowed{0};
     cudaError_t e = kv8_allow_smem(allowed, kv8_rows_kernel<HD, E4M3, TILES>, (int)rows_smem<HD, TILES>(Q3T_MAX_TABLE_ROWS));
-    if (e == cudaSuccess) e = launch_zero_counters(static_cast<unsigned int*>(a.scratch), kRowCtas, stream);
+    if (e == cudaSuccess) e = launch_pdl(kv8_zero_tickets_kernel, dim3(1), dim3(kRowCtas), 0, stream, static_cast<unsigned int*>(a.scratch));
     if (e != cudaSuccess) return e;
     e = launch_pdl(kv8_rows_kernel<HD, E4M3, TILES>, dim3(148 * rows_residency<HD, TILES>()), dim3(kRowThreads), rows_smem<HD, TILES>(a.rows), stream, a);
     return e != cudaSuccess || !a.prompts ? e : launch_kv8_prompts(a, HD, E4M3, stream);
