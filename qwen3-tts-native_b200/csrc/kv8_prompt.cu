@@ -2,14 +2,14 @@
 // value scale an addend of the exponent, are in kv8_attention.cu.
 //
 // A CTA takes 256 columns ((new token, query head) pairs of a KV head, two tiles of 128 rows of the tensor cores) of a row and walks
-// what they see of its cache once, 128 tokens a step, two halves of 64:
+// what they see of its cache once, 128 tokens a step:
 //   copies    codes from their pages to registers, to fp16 (exact) and into shared memory, swizzled: K by four warps, V by four; the
 //             next step's are requested before the present one's are stored
-//   scores    S = Q K^T, tcgen05.mma from shared memory into 64 columns of tensor memory a tile and half
+//   scores    S = Q K^T, tcgen05.mma from shared memory into 128 columns of tensor memory a tile
 //   softmax   a thread a row: w = exp2(s * key scale + log2(value scale) - reference) as fp16 over the scores' place
 //   output    O += W V, the weights from tensor memory
-// While a tile's half is in the softmax the products of its other half and of the other tile run.  A row's reference follows its scores
-// only when its weights outgrow fp16, so that the output in tensor memory is rescaled almost never.
+// The tiles take turns: one's products run while the other is in the softmax.  A row's reference follows its scores only when its
+// weights outgrow fp16, so that the output in tensor memory is rescaled almost never.
 
 #include "kv8.cuh"
 #include "q3t_kernels.cuh"
@@ -22,12 +22,11 @@ namespace {
 
 constexpr int kTileRows = 128;
 constexpr int kStep = 128;                              // tokens
-constexpr int kHalf = kStep / 2;
 constexpr int kStepPages = kStep / kPageTokens;
 constexpr int kPromptThreads = 640;                     // warps 0..7 softmax (a tile each four), 8..11 K, 12..15 V, 16 products
-constexpr int kKeyWarp = 8, kValueWarp = 12, kProductWarp = 16;
+constexpr int kSoftmaxWarps = 8, kKeyWarp = 8, kValueWarp = 12, kProductWarp = 16;
 // What setmaxnreg hands out is what the block was launched with
-constexpr int kLaunchRegisters = 96, kSoftmaxRegisters = 144, kCopyRegisters = 72, kProductRegisters = 48;
+constexpr int kLaunchRegisters = 96, kSoftmaxRegisters = 136, kCopyRegisters = 72, kProductRegisters = 64;
 static_assert(2 * kSoftmaxRegisters + 2 * kCopyRegisters + kProductRegisters <= 5 * kLaunchRegisters, "registers of the five warpgroups");
 constexpr int kScaleRing = 4;                           // steps whose scales are kept: K runs two steps ahead of the softmax
 constexpr uint32_t kTmemCols = 512, kOut = 256;         // scores of the tiles at 0 and 128, outputs at 256 and 384
@@ -92,7 +91,15 @@ __device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint
         ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// 32 columns of this thread's lane; to be waited for
+// 16 or 32 columns of this thread's lane, to be waited for
+__device__ __forceinline__ void tmem_load_16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
 __device__ __forceinline__ void tmem_load_32(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
@@ -103,10 +110,22 @@ __device__ __forceinline__ void tmem_load_32(uint32_t taddr, uint32_t (&r)[32]) 
           "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[32]) {
+template <int N>
+__device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[N]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));       // not to be used ahead of the wait
+    for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));        // not to be used ahead of the wait
+}
+__device__ __forceinline__ void tmem_load_8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_store_8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_store_16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
@@ -127,7 +146,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
     unsigned char* const values = keys + 2 * Smem::kTileBytes;         // [step % 2]
     __shared__ float4 scales[kScaleRing][kStepPages];                  // of each page: key scale, log2 and reciprocal of the value scale
     __shared__ float row_scale[2 * kTileRows];
-    __shared__ uint64_t full_k[2], full_v[2], empty_k[2], empty_v[2], s_ready[2][2], p_ready[2][2], o_ready[2][2], q_ready;     // [tile][half]
+    __shared__ uint64_t full_k[2], full_v[2], empty_k[2], empty_v[2], s_ready[2], p_ready[2], o_ready[2], q_ready;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     __shared__ int warp_items[kPromptThreads / kWarp];
@@ -174,13 +193,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
     const int columns = min(2 * kTileRows, item.span.count * group - column0);
     // tokens that the last column of each tile sees
     auto seen_by = [&](int column) { return min(max(item.span.base + column / group + 1, 0), a.max_sequence); };
-    int halves_of[2];
+    int steps_of[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         const int last = min(columns, (t + 1) * kTileRows);
-        halves_of[t] = last > t * kTileRows ? (seen_by(column0 + last - 1) + kHalf - 1) / kHalf : 0;
+        steps_of[t] = last > t * kTileRows ? (seen_by(column0 + last - 1) + kStep - 1) / kStep : 0;
     }
-    const int halves = max(halves_of[0], halves_of[1]), steps = (halves + 1) / 2;
+    const int steps = max(steps_of[0], steps_of[1]);
 
     Guard guard;
     guard.deadline = tc::now_ns() + kBudgetNs;
@@ -191,13 +210,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
             tc::mbar_init(&full_v[i], 4);
             tc::mbar_init(&empty_k[i], 1);
             tc::mbar_init(&empty_v[i], 1);
-            for (int h = 0; h < 2; ++h) {
-                tc::mbar_init(&s_ready[i][h], 1);
-                tc::mbar_init(&p_ready[i][h], 4);
-                tc::mbar_init(&o_ready[i][h], 1);
-            }
+            tc::mbar_init(&s_ready[i], 1);
+            tc::mbar_init(&p_ready[i], 4);
+            tc::mbar_init(&o_ready[i], 1);
         }
-        tc::mbar_init(&q_ready, 8);
+        tc::mbar_init(&q_ready, kSoftmaxWarps);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -295,69 +312,62 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
                     *reinterpret_cast<int4*>(tile + store_more + p * (kPageTokens * 128)) = make_int4((int)h[4], (int)h[5], (int)h[6], (int)h[7]);
                 }
             }
+            // (ahead of the next requests: the fence would wait for them)
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&full[buffer]);
             if (step + 1 < steps) {
                 request(step + 1);
                 request_scales(step + 1);
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&full[buffer]);
         }
     } else if (warp >= kProductWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProductRegisters));
         if (warp == kProductWarp && steps > 0 && tc::elect_one()) {
             // ---- products: both operands fp16, sums fp32
-            const uint32_t scores_idesc = (1u << 4) | ((uint32_t)(kHalf >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
+            const uint32_t scores_idesc = (1u << 4) | ((uint32_t)(kStep >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
             // B with its rows (dims) contiguous: bit 16
             const uint32_t out_idesc = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
-            auto scores = [&](int tile, int n) {                       // n: half of a step, counted through
-                const uint32_t q = tc::smem_u32(queries) + tile * kTileRows * HD * 2;
-                const uint32_t k = tc::smem_u32(keys) + ((n >> 1) & 1) * Smem::kTileBytes + (n & 1) * kHalf * 128;
+            auto scores = [&](int tile, int step) {
+                const uint32_t q = tc::smem_u32(queries) + tile * kTileRows * HD * 2, k = tc::smem_u32(keys) + (step & 1) * Smem::kTileBytes;
 #pragma unroll
                 for (int j = 0; j < HD / 16; ++j) {
-                    umma_ss(tmem + tile * kStep + (n & 1) * kHalf, tc::umma_desc(q + (j / 4) * kTileRows * 128 + 32 * (j % 4)),
+                    umma_ss(tmem + tile * kStep, tc::umma_desc(q + (j / 4) * kTileRows * 128 + 32 * (j % 4)),
                             tc::umma_desc(k + (j / 4) * kStep * 128 + 32 * (j % 4)), scores_idesc, j != 0 ? 1u : 0u);
                 }
-                tc::umma_commit(&s_ready[tile][n & 1]);
+                tc::umma_commit(&s_ready[tile]);
             };
             bool ok = guard.wait(&q_ready, 0) && guard.wait(&full_k[0], 0);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (ok) {
-                for (int n = 0; n < 2; ++n) {
-                    for (int tile = 0; tile < 2; ++tile) {
-                        if (n < halves_of[tile]) scores(tile, n);
-                    }
-                }
+                if (steps_of[0] > 0) scores(0, 0);
+                if (steps_of[1] > 0) scores(1, 0);
                 tc::umma_commit(&empty_k[0]);
             }
-            for (int n = 0; n < halves && ok; ++n) {
-                const int step = n >> 1;
-                const bool ahead = n + 2 < halves;                     // scores of the next step
-                if ((n & 1) == 0) ok = guard.wait(&full_v[step & 1], (step >> 1) & 1);
+            for (int step = 0; step < steps && ok; ++step) {
+                ok = guard.wait(&full_v[step & 1], (step >> 1) & 1) && (step + 1 == steps || guard.wait(&full_k[(step + 1) & 1], ((step + 1) >> 1) & 1));
                 for (int tile = 0; tile < 2 && ok; ++tile) {
-                    if (n >= halves_of[tile]) continue;
-                    ok = guard.wait(&p_ready[tile][n & 1], step & 1);
+                    if (step >= steps_of[tile]) continue;
+                    ok = guard.wait(&p_ready[tile], step & 1);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t v = tc::smem_u32(values) + (step & 1) * Smem::kTileBytes + (n & 1) * kHalf * 128;
+                    const uint32_t v = tc::smem_u32(values) + (step & 1) * Smem::kTileBytes;
 #pragma unroll
-                    for (int j = 0; j < kHalf / 16; ++j) {
-                        tc::umma_f16_ts(tmem + kOut + tile * 128, tmem + tile * kStep + (n & 1) * kHalf + 8 * j, desc_rows_contiguous(v + j * 16 * 128),
-                                        out_idesc, (n | j) != 0 ? 1u : 0u);
+                    for (int j = 0; j < kStep / 16; ++j) {
+                        tc::umma_f16_ts(tmem + kOut + tile * 128, tmem + tile * kStep + 8 * j, desc_rows_contiguous(v + j * 16 * 128), out_idesc,
+                                        (step | j) != 0 ? 1u : 0u);
                     }
-                    tc::umma_commit(&o_ready[tile][n & 1]);
-                }
-                if (ahead && (n & 1) == 0) ok = ok && guard.wait(&full_k[(step + 1) & 1], ((step + 1) >> 1) & 1);
-                // the next scores of this half lie over the weights: products of other accumulators are in no order of their own
-                for (int tile = 0; tile < 2 && ok; ++tile) {
-                    if (n + 2 >= halves_of[tile]) continue;
-                    ok = guard.wait(&o_ready[tile][n & 1], step & 1);
+                    tc::umma_commit(&o_ready[tile]);
+                    if (step + 1 >= steps_of[tile]) continue;
+                    // the next scores lie over the weights: products of other accumulators are in no order of their own
+                    ok = guard.wait(&o_ready[tile], step & 1);
+                    if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (ok) scores(tile, n + 2);
+                    scores(tile, step + 1);
                 }
                 if (!ok) break;
-                if ((n & 1) != 0 || n + 1 == halves) tc::umma_commit(&empty_v[step & 1]);
-                if (ahead && ((n & 1) != 0 || n + 3 == halves)) tc::umma_commit(&empty_k[(step + 1) & 1]);
+                tc::umma_commit(&empty_v[step & 1]);
+                if (step + 1 < steps) tc::umma_commit(&empty_k[(step + 1) & 1]);
             }
         }
     } else {
@@ -365,8 +375,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         // ---- queries to fp16, by a power of two that brings the largest of each to 2^7..2^8
         constexpr int kLanes = HD / 8, kAtOnce = kWarp / kLanes;       // of a row, rows of a warp
 #pragma unroll 4
-        for (int i = 0; i < 2 * kTileRows / (8 * kAtOnce); ++i) {
-            const int r = warp * (2 * kTileRows / 8) + i * kAtOnce + lane / kLanes, piece = lane % kLanes;
+        for (int i = 0; i < 2 * kTileRows / (kSoftmaxWarps * kAtOnce); ++i) {
+            const int r = warp * (2 * kTileRows / kSoftmaxWarps) + i * kAtOnce + lane / kLanes, piece = lane % kLanes;
             const int column = column0 + r, token = column / group;
             int4 raw = make_int4(0, 0, 0, 0);
             if (r < columns) {
@@ -399,114 +409,141 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         const int r = tile * kTileRows + quarter * kWarp + lane;
         const bool real = r < columns;
         const int seen = real ? seen_by(column0 + r) : 0;
+        const int unmasked = (int)__reduce_min_sync(0xffffffffu, (unsigned int)seen) / kStep;      // steps all of which every row of the warp sees
         const float up = row_scale[r];
         const uint32_t lanes = tmem + ((uint32_t)(quarter * kWarp) << 16);
-        const uint32_t o_at = lanes + kOut + tile * 128;
-        const int own = halves_of[tile];
+        const uint32_t o_at = lanes + kOut + tile * 128, s_at = lanes + tile * kStep;
+        const int own = steps_of[tile];
         float top = real ? -INFINITY : 0.0f, total = 0.0f;
-        for (int n = 0; n < own; ++n) {
-            if (!__all_sync(0xffffffffu, guard.wait(&s_ready[tile][n & 1], (n >> 1) & 1))) break;
+        bool open = true;                                              // some row of the warp has no reference yet
+        // (the products of the steps before are done: the scores came behind them)
+        auto rescale_output = [&](float keep) {
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 16) {
+                float o[16];
+                uint32_t bits[16];
+                tc::tmem_load_row<16>(o_at + c, o);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) bits[j] = __float_as_uint(o[j] * keep);
+                tmem_store_16(o_at + c, bits);
+            }
+        };
+        for (int step = 0; step < own; ++step) {
+            if (!__all_sync(0xffffffffu, guard.wait(&s_ready[tile], step & 1))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t s_at = lanes + tile * kStep + (n & 1) * kHalf;
-            const float4* const page_scales = scales[(n >> 1) % kScaleRing] + (n & 1) * (kStepPages / 2);
-            const int visible = seen - n * kHalf;                      // of the half's tokens
-            const bool masked = __any_sync(0xffffffffu, visible < kHalf);
-            // the reference becomes the largest score so far
-            auto measure = [&]() {
+            const float4* const page_scales = scales[step % kScaleRing];
+            const int visible = seen - step * kStep;                   // of the step's tokens
+            if (open) {
+                // the reference becomes the largest score so far
                 float most = -INFINITY;
 #pragma unroll 1
-                for (int c = 0; c < kHalf / 32; ++c) {
-                    uint32_t s[32];
-                    tmem_load_32(s_at + 32 * c, s);
+                for (int p = 0; p < kStepPages; ++p) {
+                    uint32_t s[16];
+                    tmem_load_16(s_at + 16 * p, s);
                     tmem_wait_load(s);
+                    float m = -INFINITY;
 #pragma unroll
-                    for (int p = 0; p < 2; ++p) {
-                        float m = -INFINITY;
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) m = fmaxf(m, 32 * c + 16 * p + j >= visible ? -INFINITY : __uint_as_float(s[16 * p + j]));
-                        const float4 f = page_scales[2 * c + p];
-                        most = fmaxf(most, m == -INFINITY ? m : fmaf(m, f.x * up, f.y));
-                    }
+                    for (int j = 0; j < 16; ++j) m = fmaxf(m, 16 * p + j >= visible ? -INFINITY : __uint_as_float(s[j]));
+                    const float4 f = page_scales[p];
+                    most = fmaxf(most, m == -INFINITY ? m : fmaf(m, f.x * up, f.y));
                 }
-                const float moved = fmaxf(top, most);
-                const float keep = moved == top ? 1.0f : exp2_ftz(top - moved);
+                const float moved = fmaxf(top, most), keep = moved == top ? 1.0f : exp2_ftz(top - moved);
                 top = moved;
                 total *= keep;
-                if (n == 0 || !__all_sync(0xffffffffu, guard.wait(&o_ready[tile][(n - 1) & 1], ((n - 1) >> 1) & 1))) return;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll 1
-                for (int c = 0; c < HD; c += 16) {
-                    float o[16];
-                    uint32_t bits[16];
-                    tc::tmem_load_row<16>(o_at + c, o);
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) bits[j] = __float_as_uint(o[j] * keep);
-                    tmem_store_16(o_at + c, bits);
-                }
-            };
-            uint32_t w[kHalf / 2];
-            float added, largest;
+                if (step > 0) rescale_output(keep);
+                open = __any_sync(0xffffffffu, top == -INFINITY);
+            }
             auto weigh = [&](auto mask) {
                 // (nothing but -inf so far: weights of zero)
-                const float reference = top == -INFINITY ? 0.0f : top - kKv8Lift;
-                added = 0.0f;
-                largest = 0.0f;
+                float reference = top == -INFINITY ? 0.0f : top - kKv8Lift;
+                // scores of 32 tokens, three buffers: the loads of the last two chunks run under the arithmetic of the first two
+                uint32_t s[3][32];
+                tmem_load_32(s_at, s[0]);
+                tmem_load_32(s_at + 32, s[1]);
 #pragma unroll
-                for (int c = 0; c < kHalf / 32; ++c) {
-                    uint32_t s[32];
-                    tmem_load_32(s_at + 32 * c, s);
-                    tmem_wait_load(s);
-#pragma unroll
-                    for (int p = 0; p < 2; ++p) {
-                        const float4 f = page_scales[2 * c + p];
-                        const float slope = f.x * up, shift = f.y - reference;
-                        const unsigned long long slope2 = pack2(slope, slope), shift2 = pack2(shift, shift);
-                        unsigned long long sums = pack2(0.0f, 0.0f);
-#pragma unroll
-                        for (int j = 0; j < 16; j += 2) {
-                            float x, y;
-                            unpack2(fma2(pack2(__uint_as_float(s[16 * p + j]), __uint_as_float(s[16 * p + j + 1])), slope2, shift2), x, y);
-                            if (mask.value) {
-                                if (32 * c + 16 * p + j >= visible) x = -INFINITY;
-                                if (32 * c + 16 * p + j + 1 >= visible) y = -INFINITY;
-                            }
-                            x = exp2_ftz(x);
-                            y = exp2_ftz(y);
-                            sums = add2(sums, pack2(x, y));
-                            w[16 * c + 8 * p + j / 2] = pack_half2(x, y);
-                        }
-                        float x, y;
-                        unpack2(sums, x, y);
-                        x += y;
-                        largest = fmaxf(largest, x);
-                        added = fmaf(x, f.z, added);
+                for (int c = 0; c < kStep / 32; ++c) {
+                    if (c == 0 || c == 2) {
+                        tmem_wait_load(s[c % 3]);
+                        tmem_wait_load(s[(c + 1) % 3]);
                     }
+                    if (c < 2) tmem_load_32(s_at + 32 * (c + 2), s[(c + 2) % 3]);
+                    uint32_t w[16];
+                    float largest, added;
+                    auto pages = [&]() {
+                        largest = added = 0.0f;
+#pragma unroll
+                        for (int p = 0; p < 2; ++p) {
+                            const float4 f = page_scales[2 * c + p];
+                            const float slope = f.x * up, shift = f.y - reference;
+                            const unsigned long long slope2 = pack2(slope, slope), shift2 = pack2(shift, shift);
+                            unsigned long long sums[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
+#pragma unroll
+                            for (int j = 0; j < 16; j += 2) {
+                                const uint32_t* const at = &s[c % 3][16 * p + j];
+                                float x, y;
+                                unpack2(fma2(pack2(__uint_as_float(at[0]), __uint_as_float(at[1])), slope2, shift2), x, y);
+                                if (mask.value) {
+                                    if (32 * c + 16 * p + j >= visible) x = -INFINITY;
+                                    if (32 * c + 16 * p + j + 1 >= visible) y = -INFINITY;
+                                }
+                                x = exp2_ftz(x);
+                                y = exp2_ftz(y);
+                                sums[(j >> 1) & 1] = add2(sums[(j >> 1) & 1], pack2(x, y));
+                                w[8 * p + j / 2] = pack_half2(x, y);
+                            }
+                            float x, y;
+                            unpack2(add2(sums[0], sums[1]), x, y);
+                            x += y;
+                            largest = fmaxf(largest, x);
+                            added = fmaf(x, f.z, added);
+                        }
+                    };
+                    // No maximum is looked for: a weight is at most its page's sum, which says whether one may have outgrown fp16.  The
+                    // reference then rises by a whole number, so that the weights that are stored already shrink exactly.
+                    pages();
+                    if (__any_sync(0xffffffffu, largest > kMostWeight)) {
+                        float rise = 0.0f;
+#pragma unroll
+                        for (int p = 0; p < 2; ++p) {
+                            const float4 f = page_scales[2 * c + p];
+                            float most = -INFINITY;
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) most = fmaxf(most, mask.value && 32 * c + 16 * p + j >= visible ? -INFINITY : __uint_as_float(s[c % 3][16 * p + j]));
+                            if (most > -INFINITY) rise = fmaxf(rise, ceilf(fmaf(most, f.x * up, f.y - reference) - kKv8Lift));
+                        }
+                        if (!(largest > kMostWeight)) rise = 0.0f;
+                        const float keep = exp2_ftz(-rise);
+                        top += rise;
+                        reference += rise;
+                        total *= keep;
+                        if (step > 0) rescale_output(keep);
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+#pragma unroll 1
+                        for (int before = 0; before < 2 * c; ++before) {
+                            uint32_t h[8];
+                            tmem_load_8(s_at + 8 * before, h);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+                                h[j] = pack_half2(x.x * keep, x.y * keep);
+                            }
+                            tmem_store_8(s_at + 8 * before, h);
+                        }
+                        pages();
+                    }
+                    total += added;
+                    tmem_store_16(s_at + 16 * c, w);
                 }
             };
-            // No maximum is looked for at first: a weight is at most its page's sum, which says whether one may have outgrown fp16
-            if (__any_sync(0xffffffffu, top == -INFINITY)) measure();
-            for (int again = 0;; ++again) {
-                if (masked) weigh(std::true_type{});
-                else weigh(std::false_type{});
-                if (again != 0 || !__any_sync(0xffffffffu, largest > kMostWeight)) break;
-                measure();
-            }
-            total += added;
-#pragma unroll
-            for (int c = 0; c < kHalf / 32; ++c) {
-                uint32_t part_of[16];
-#pragma unroll
-                for (int j = 0; j < 16; ++j) part_of[j] = w[16 * c + j];
-                tmem_store_16(s_at + 16 * c, part_of);
-            }
+            if (step < unmasked) weigh(std::false_type{});
+            else weigh(std::true_type{});
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&p_ready[tile][n & 1]);
+            if (lane == 0) tc::mbar_arrive(&p_ready[tile]);
         }
-        // (A barrier a half: of the one that is waited for here all completions but the last are known to be past, so that its parity says
-        // which.  With one barrier for both halves a late reader would take two completions for none.)
-        if (own > 0) guard.wait(&o_ready[tile][(own - 1) & 1], ((own - 1) >> 1) & 1);
+        // (all completions but the last are known to be past, so that the parity says which is)
+        if (own > 0) guard.wait(&o_ready[tile], (own - 1) & 1);
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
