@@ -2,14 +2,14 @@
 // value scale an addend of the exponent, are in kv8_attention.cu.
 //
 // A CTA takes 256 columns ((new token, query head) pairs of a KV head, two tiles of 128 rows of the tensor cores) of a row and walks
-// what they see of its cache once, 128 tokens a step:
+// what they see of its cache once, 128 tokens a step, two halves of 64:
 //   copies    codes from their pages to registers, to fp16 (exact) and into shared memory, swizzled: K by four warps, V by four; the
 //             next step's are requested before the present one's are stored
-//   scores    S = Q K^T, tcgen05.mma from shared memory into 128 columns of tensor memory a tile
+//   scores    S = Q K^T, tcgen05.mma from shared memory into 64 columns of tensor memory a tile and half
 //   softmax   a thread a row: w = exp2(s * key scale + log2(value scale) - reference) as fp16 over the scores' place
 //   output    O += W V, the weights from tensor memory
-// The tiles take turns: one's products run while the other is in the softmax.  A row's reference follows its scores only when its
-// weights outgrow fp16, so that the output in tensor memory is rescaled almost never.
+// While a tile's half is in the softmax the products of its other half and of the other tile run.  A row's reference follows its scores
+// only when its weights outgrow fp16, so that the output in tensor memory is rescaled almost never.
 
 #include "kv8.cuh"
 #include "q3t_kernels.cuh"
@@ -23,7 +23,8 @@ namespace {
 constexpr int kTileRows = 128;
 constexpr int kStep = 128;                              // tokens
 constexpr int kStepPages = kStep / kPageTokens;
-constexpr int kPromptThreads = 640;                     // warps 0..7 softmax (a tile each four), 8..11 K, 12..15 V, 16 products
+constexpr int kHalf = kStep / 2, kHalfPages = kStepPages / 2;
+constexpr int kPromptThreads = 640;                     // warps 0..7 softmax (a tile each four), 8..11 K, 12..15 V, 16 and 17 products (a tile each)
 constexpr int kSoftmaxWarps = 8, kKeyWarp = 8, kValueWarp = 12, kProductWarp = 16;
 // What setmaxnreg hands out is what the block was launched with
 constexpr int kLaunchRegisters = 96, kSoftmaxRegisters = 136, kCopyRegisters = 72, kProductRegisters = 64;
@@ -31,7 +32,7 @@ static_assert(2 * kSoftmaxRegisters + 2 * kCopyRegisters + kProductRegisters <= 
 constexpr int kScaleRing = 4;                           // steps whose scales are kept: K runs two steps ahead of the softmax
 constexpr uint32_t kTmemCols = 512, kOut = 256;         // scores of the tiles at 0 and 128, outputs at 256 and 384
 constexpr float kMostWeight = 32768.0f;                 // of a page's weights together
-constexpr unsigned long long kBudgetNs = 2000000000ull;
+constexpr long long kBudgetCycles = 4000000000ll;        // about two seconds
 
 __device__ unsigned int g_kv8_prompt_errors = 0;
 __device__ unsigned int g_kv8_prompt_page_errors = 0;
@@ -43,29 +44,20 @@ struct PromptSmem {
     static constexpr size_t kBytes = 1024 + kQueryBytes + 4 * kTileBytes;
 };
 
-// As tc::Guard, with a limit to each look at a barrier: a look of the whole warp may be suspended for milliseconds otherwise, a thousand of
-// which are no bound
+// As tc::Guard, but the clock is looked at whenever a look at a barrier ends: one of a whole warp may be suspended for milliseconds, a
+// thousand of which are no bound.  (With a limit to the suspension, 20 us, a chunk of 4096 at 16k took 6 % longer.)
 struct Guard {
-    unsigned long long deadline;
+    long long deadline;                                                // of clock64()
     volatile int* abort_flag;
     __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) const {
-        uint32_t polls = 0;
-        for (;;) {
-            uint32_t ok;
-            asm volatile(
-                "{\n\t.reg .pred p;\n\t"
-                "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-                "selp.u32 %0, 1, 0, p;\n\t}"
-                : "=r"(ok)
-                : "r"(tc::smem_u32(bar)), "r"(parity), "r"(20000u)
-                : "memory");
-            if (ok != 0) return true;
+        while (!tc::mbar_try_wait(bar, parity)) {
             if (*abort_flag != 0) return false;
-            if ((++polls & 31u) == 0 && tc::now_ns() > deadline) {
+            if (clock64() > deadline) {
                 *abort_flag = 1;
                 return false;
             }
         }
+        return true;
     }
 };
 
@@ -146,7 +138,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
     unsigned char* const values = keys + 2 * Smem::kTileBytes;         // [step % 2]
     __shared__ float4 scales[kScaleRing][kStepPages];                  // of each page: key scale, log2 and reciprocal of the value scale
     __shared__ float row_scale[2 * kTileRows];
-    __shared__ uint64_t full_k[2], full_v[2], empty_k[2], empty_v[2], s_ready[2], p_ready[2], o_ready[2], q_ready;
+    // full: V of a step and K of the next one
+    __shared__ uint64_t first_k, full[2], empty_k[2], empty_v[2], s_ready[2][2], p_ready[2][2], o_ready[2][2], q_ready;     // [tile][half]
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     __shared__ int warp_items[kPromptThreads / kWarp];
@@ -193,27 +186,25 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
     const int columns = min(2 * kTileRows, item.span.count * group - column0);
     // tokens that the last column of each tile sees
     auto seen_by = [&](int column) { return min(max(item.span.base + column / group + 1, 0), a.max_sequence); };
-    int steps_of[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const int last = min(columns, (t + 1) * kTileRows);
-        steps_of[t] = last > t * kTileRows ? (seen_by(column0 + last - 1) + kStep - 1) / kStep : 0;
-    }
-    const int steps = max(steps_of[0], steps_of[1]);
+    // (both tiles go as far as the second one's last column sees; one that is empty not at all)
+    const int tiles = columns > kTileRows ? 2 : 1;
+    const int halves = (seen_by(column0 + columns - 1) + kHalf - 1) / kHalf, steps = (halves + 1) / 2;
 
     Guard guard;
-    guard.deadline = tc::now_ns() + kBudgetNs;
+    guard.deadline = clock64() + kBudgetCycles;
     guard.abort_flag = abort_flag;
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            tc::mbar_init(&full_k[i], 4);
-            tc::mbar_init(&full_v[i], 4);
-            tc::mbar_init(&empty_k[i], 1);
-            tc::mbar_init(&empty_v[i], 1);
-            tc::mbar_init(&s_ready[i], 1);
-            tc::mbar_init(&p_ready[i], 4);
-            tc::mbar_init(&o_ready[i], 1);
+            tc::mbar_init(&full[i], 8);
+            tc::mbar_init(&empty_k[i], tiles);
+            tc::mbar_init(&empty_v[i], tiles);
+            for (int h = 0; h < 2; ++h) {
+                tc::mbar_init(&s_ready[i][h], 1);
+                tc::mbar_init(&p_ready[i][h], 4);
+                tc::mbar_init(&o_ready[i][h], 1);
+            }
         }
+        tc::mbar_init(&first_k, 4);
         tc::mbar_init(&q_ready, kSoftmaxWarps);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -238,8 +229,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         const int store_at = (int)tile_offset(token, kCodes == 16 ? 2 * part : part);
         const int store_more = (int)tile_offset(token, 2 * part + 1) - store_at;
         const uint8_t* const plane = (is_value ? a.cache.v : a.cache.k) + (size_t)item.kv_head * (kPageTokens * HD) + token * HD + part * kCodes;
-        unsigned char* const tiles = is_value ? values : keys;
-        uint64_t* const full = is_value ? full_v : full_k;
+        unsigned char* const buffers = is_value ? values : keys;
         uint64_t* const empty = is_value ? empty_v : empty_k;
         const int last = min(max(item.span.base + item.span.count, 0), a.max_sequence);        // what lies behind may read as NaN
         const bool last_block = column0 + 2 * kTileRows >= item.span.count * group;
@@ -299,7 +289,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
                 scales[step % kScaleRing][t] = (good >> t) & 1u ? make_float4(key_scale, log2_fast(vs), reciprocal_fast(vs), 0.0f)
                                                                : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
             }
-            unsigned char* const tile = tiles + buffer * Smem::kTileBytes + store_at;
+            unsigned char* const tile = buffers + buffer * Smem::kTileBytes + store_at;
 #pragma unroll
             for (int p = 0; p < kStepPages; ++p) {
                 uint32_t h[8];
@@ -315,59 +305,62 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
             // (ahead of the next requests: the fence would wait for them)
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&full[buffer]);
+            if (lane == 0) tc::mbar_arrive(is_value ? &full[buffer] : step == 0 ? &first_k : &full[buffer ^ 1]);
             if (step + 1 < steps) {
                 request(step + 1);
                 request_scales(step + 1);
             }
         }
+        // the last step has no next K; its barrier's phase before is past when the scores of the step before last are there
+        if (!is_value && steps > 0) {
+            if (steps > 1) guard.wait(&empty_k[steps & 1], ((steps - 2) >> 1) & 1);
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&full[(steps - 1) & 1]);
+        }
     } else if (warp >= kProductWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProductRegisters));
-        if (warp == kProductWarp && steps > 0 && tc::elect_one()) {
-            // ---- products: both operands fp16, sums fp32
-            const uint32_t scores_idesc = (1u << 4) | ((uint32_t)(kStep >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
+        const int tile = warp - kProductWarp;
+        if (tile < tiles && steps > 0 && tc::elect_one()) {
+            // ---- products of a tile: both operands fp16, sums fp32.  What a step takes here is the looks at barriers, 350 cycles each beside the
+            // copies' stores: hence a thread a tile (one for both: a chunk of 4096 at 16k 645 us), and one barrier for V and the next K.
+            const uint32_t scores_idesc = (1u << 4) | ((uint32_t)(kHalf >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
             // B with its rows (dims) contiguous: bit 16
             const uint32_t out_idesc = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
-            auto scores = [&](int tile, int step) {
-                const uint32_t q = tc::smem_u32(queries) + tile * kTileRows * HD * 2, k = tc::smem_u32(keys) + (step & 1) * Smem::kTileBytes;
+            const uint32_t q = tc::smem_u32(queries) + tile * kTileRows * HD * 2;
+            auto scores = [&](int n) {                                 // n: half of a step, counted through
+                const uint32_t k = tc::smem_u32(keys) + ((n >> 1) & 1) * Smem::kTileBytes + (n & 1) * kHalf * 128;
 #pragma unroll
                 for (int j = 0; j < HD / 16; ++j) {
-                    umma_ss(tmem + tile * kStep, tc::umma_desc(q + (j / 4) * kTileRows * 128 + 32 * (j % 4)),
+                    umma_ss(tmem + tile * kStep + (n & 1) * kHalf, tc::umma_desc(q + (j / 4) * kTileRows * 128 + 32 * (j % 4)),
                             tc::umma_desc(k + (j / 4) * kStep * 128 + 32 * (j % 4)), scores_idesc, j != 0 ? 1u : 0u);
                 }
-                tc::umma_commit(&s_ready[tile]);
+                tc::umma_commit(&s_ready[tile][n & 1]);
+                if ((n & 1) != 0 || n + 1 == halves) tc::umma_commit(&empty_k[(n >> 1) & 1]);
             };
-            bool ok = guard.wait(&q_ready, 0) && guard.wait(&full_k[0], 0);
+            bool ok = guard.wait(&q_ready, 0) && guard.wait(&first_k, 0);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (ok) {
-                if (steps_of[0] > 0) scores(0, 0);
-                if (steps_of[1] > 0) scores(1, 0);
-                tc::umma_commit(&empty_k[0]);
+                scores(0);
+                if (halves > 1) scores(1);
             }
-            for (int step = 0; step < steps && ok; ++step) {
-                ok = guard.wait(&full_v[step & 1], (step >> 1) & 1) && (step + 1 == steps || guard.wait(&full_k[(step + 1) & 1], ((step + 1) >> 1) & 1));
-                for (int tile = 0; tile < 2 && ok; ++tile) {
-                    if (step >= steps_of[tile]) continue;
-                    ok = guard.wait(&p_ready[tile], step & 1);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t v = tc::smem_u32(values) + (step & 1) * Smem::kTileBytes;
-#pragma unroll
-                    for (int j = 0; j < kStep / 16; ++j) {
-                        tc::umma_f16_ts(tmem + kOut + tile * 128, tmem + tile * kStep + 8 * j, desc_rows_contiguous(v + j * 16 * 128), out_idesc,
-                                        (step | j) != 0 ? 1u : 0u);
-                    }
-                    tc::umma_commit(&o_ready[tile]);
-                    if (step + 1 >= steps_of[tile]) continue;
-                    // the next scores lie over the weights: products of other accumulators are in no order of their own
-                    ok = guard.wait(&o_ready[tile], step & 1);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    scores(tile, step + 1);
-                }
+            for (int n = 0; n < halves && ok; ++n) {
+                const int step = n >> 1, h = n & 1;
+                ok = (h != 0 || guard.wait(&full[step & 1], (step >> 1) & 1)) && guard.wait(&p_ready[tile][h], step & 1);
                 if (!ok) break;
-                tc::umma_commit(&empty_v[step & 1]);
-                if (step + 1 < steps) tc::umma_commit(&empty_k[(step + 1) & 1]);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t v = tc::smem_u32(values) + (step & 1) * Smem::kTileBytes + h * kHalf * 128;
+#pragma unroll
+                for (int j = 0; j < kHalf / 16; ++j) {
+                    tc::umma_f16_ts(tmem + kOut + tile * 128, tmem + tile * kStep + h * kHalf + 8 * j, desc_rows_contiguous(v + j * 16 * 128), out_idesc,
+                                    (n | j) != 0 ? 1u : 0u);
+                }
+                tc::umma_commit(&o_ready[tile][h]);
+                if (h != 0 || n + 1 == halves) tc::umma_commit(&empty_v[step & 1]);
+                if (n + 2 >= halves) continue;
+                // the next scores of this half lie over the weights: products of other accumulators are in no order of their own
+                ok = guard.wait(&o_ready[tile][h], step & 1);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (ok) scores(n + 2);
             }
         }
     } else {
@@ -409,15 +402,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         const int r = tile * kTileRows + quarter * kWarp + lane;
         const bool real = r < columns;
         const int seen = real ? seen_by(column0 + r) : 0;
-        const int unmasked = (int)__reduce_min_sync(0xffffffffu, (unsigned int)seen) / kStep;      // steps all of which every row of the warp sees
+        const int unmasked = (int)__reduce_min_sync(0xffffffffu, (unsigned int)seen) / kHalf;      // halves all of which every row of the warp sees
         const float up = row_scale[r];
         const uint32_t lanes = tmem + ((uint32_t)(quarter * kWarp) << 16);
-        const uint32_t o_at = lanes + kOut + tile * 128, s_at = lanes + tile * kStep;
-        const int own = steps_of[tile];
+        const uint32_t o_at = lanes + kOut + tile * 128;
+        const int own = tile < tiles ? halves : 0;
         float top = real ? -INFINITY : 0.0f, total = 0.0f;
         bool open = true;                                              // some row of the warp has no reference yet
-        // (the products of the steps before are done: the scores came behind them)
-        auto rescale_output = [&](float keep) {
+        auto rescale_output = [&](float keep, int n) {                 // when the products of the halves before are done
+            if (!__all_sync(0xffffffffu, guard.wait(&o_ready[tile][(n - 1) & 1], ((n - 1) >> 1) & 1))) return;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
             for (int c = 0; c < HD; c += 16) {
                 float o[16];
@@ -428,16 +422,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
                 tmem_store_16(o_at + c, bits);
             }
         };
-        for (int step = 0; step < own; ++step) {
-            if (!__all_sync(0xffffffffu, guard.wait(&s_ready[tile], step & 1))) break;
+        for (int n = 0; n < own; ++n) {
+            if (!__all_sync(0xffffffffu, guard.wait(&s_ready[tile][n & 1], (n >> 1) & 1))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const float4* const page_scales = scales[step % kScaleRing];
-            const int visible = seen - step * kStep;                   // of the step's tokens
+            const uint32_t s_at = lanes + tile * kStep + (n & 1) * kHalf;
+            const float4* const page_scales = scales[(n >> 1) % kScaleRing] + (n & 1) * kHalfPages;
+            const int visible = seen - n * kHalf;                      // of the half's tokens
             if (open) {
                 // the reference becomes the largest score so far
                 float most = -INFINITY;
 #pragma unroll 1
-                for (int p = 0; p < kStepPages; ++p) {
+                for (int p = 0; p < kHalfPages; ++p) {
                     uint32_t s[16];
                     tmem_load_16(s_at + 16 * p, s);
                     tmem_wait_load(s);
@@ -450,23 +445,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
                 const float moved = fmaxf(top, most), keep = moved == top ? 1.0f : exp2_ftz(top - moved);
                 top = moved;
                 total *= keep;
-                if (step > 0) rescale_output(keep);
+                if (n > 0) rescale_output(keep, n);
                 open = __any_sync(0xffffffffu, top == -INFINITY);
             }
             auto weigh = [&](auto mask) {
                 // (nothing but -inf so far: weights of zero)
                 float reference = top == -INFINITY ? 0.0f : top - kKv8Lift;
-                // scores of 32 tokens, three buffers: the loads of the last two chunks run under the arithmetic of the first two
-                uint32_t s[3][32];
+                uint32_t s[2][32];
                 tmem_load_32(s_at, s[0]);
                 tmem_load_32(s_at + 32, s[1]);
 #pragma unroll
-                for (int c = 0; c < kStep / 32; ++c) {
-                    if (c == 0 || c == 2) {
-                        tmem_wait_load(s[c % 3]);
-                        tmem_wait_load(s[(c + 1) % 3]);
+                for (int c = 0; c < kHalf / 32; ++c) {
+                    if (c == 0) {
+                        tmem_wait_load(s[0]);
+                        tmem_wait_load(s[1]);
                     }
-                    if (c < 2) tmem_load_32(s_at + 32 * (c + 2), s[(c + 2) % 3]);
                     uint32_t w[16];
                     float largest, added;
                     auto pages = [&]() {
@@ -479,7 +472,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
                             unsigned long long sums[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
 #pragma unroll
                             for (int j = 0; j < 16; j += 2) {
-                                const uint32_t* const at = &s[c % 3][16 * p + j];
+                                const uint32_t* const at = &s[c][16 * p + j];
                                 float x, y;
                                 unpack2(fma2(pack2(__uint_as_float(at[0]), __uint_as_float(at[1])), slope2, shift2), x, y);
                                 if (mask.value) {
@@ -508,7 +501,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
                             const float4 f = page_scales[2 * c + p];
                             float most = -INFINITY;
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) most = fmaxf(most, mask.value && 32 * c + 16 * p + j >= visible ? -INFINITY : __uint_as_float(s[c % 3][16 * p + j]));
+                            for (int j = 0; j < 16; ++j) most = fmaxf(most, mask.value && 32 * c + 16 * p + j >= visible ? -INFINITY : __uint_as_float(s[c][16 * p + j]));
                             if (most > -INFINITY) rise = fmaxf(rise, ceilf(fmaf(most, f.x * up, f.y - reference) - kKv8Lift));
                         }
                         if (!(largest > kMostWeight)) rise = 0.0f;
@@ -516,7 +509,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
                         top += rise;
                         reference += rise;
                         total *= keep;
-                        if (step > 0) rescale_output(keep);
+                        if (n > 0) rescale_output(keep, n);
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 #pragma unroll 1
                         for (int before = 0; before < 2 * c; ++before) {
@@ -535,15 +528,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
                     tmem_store_16(s_at + 16 * c, w);
                 }
             };
-            if (step < unmasked) weigh(std::false_type{});
+            if (n < unmasked) weigh(std::false_type{});
             else weigh(std::true_type{});
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&p_ready[tile]);
+            if (lane == 0) tc::mbar_arrive(&p_ready[tile][n & 1]);
         }
-        // (all completions but the last are known to be past, so that the parity says which is)
-        if (own > 0) guard.wait(&o_ready[tile], (own - 1) & 1);
+        // (A barrier a half: of the one that is waited for here all completions but the last are known to be past, so that its parity says
+        // which.  With one barrier for both halves a late reader would take two completions for none.)
+        if (own > 0) guard.wait(&o_ready[tile][(own - 1) & 1], ((own - 1) >> 1) & 1);
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
