@@ -129,7 +129,7 @@ __device__ __forceinline__ void tmem_store_16(uint32_t taddr, const uint32_t (&r
 }
 
 template <int HD, bool E4M3>
-__global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8AttentionArgs a) {
+__global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8AttentionArgs a, const int block_columns) {
     using Smem = PromptSmem<HD>;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* const smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
     const int tid = threadIdx.x, lane = tid % kWarp, warp = __shfl_sync(0xffffffffu, tid / kWarp, 0);
     const int heads = a.cache.heads, group = a.query_heads / heads;
 
-    // ---- this CTA's columns: the rows of many columns have ceil(columns / 256) items a KV head; those of a row's last tokens, which see
+    // ---- this CTA's columns: the rows of many columns have ceil(columns / block_columns) items a KV head; those of a row's last tokens, which see
     // the most, first, all KV heads of a block together
     if (tid == 0) found.row = -1;
     __syncthreads();
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         if (row < a.rows) {
             span = row_span(a.starts, a.lengths, row, a.tokens, a.most, a.max_sequence);
             const long long columns = (long long)span.count * group;
-            own = columns > kKv8RowColumns ? (int)((columns + 2 * kTileRows - 1) / (2 * kTileRows)) * heads : 0;
+            own = columns > kKv8RowColumns ? (int)((columns + block_columns - 1) / block_columns) * heads : 0;
             mine = own;
         }
 #pragma unroll
@@ -182,8 +182,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         pdl_wait();                                                    // what follows relies on this launch to be behind the one before
         return;
     }
-    const int column0 = item.block * 2 * kTileRows;
-    const int columns = min(2 * kTileRows, item.span.count * group - column0);
+    const int column0 = item.block * block_columns;
+    const int columns = min(block_columns, item.span.count * group - column0);
     // tokens that the last column of each tile sees
     auto seen_by = [&](int column) { return min(max(item.span.base + column / group + 1, 0), a.max_sequence); };
     // (both tiles go as far as the second one's last column sees; one that is empty not at all)
@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         unsigned char* const buffers = is_value ? values : keys;
         uint64_t* const empty = is_value ? empty_v : empty_k;
         const int last = min(max(item.span.base + item.span.count, 0), a.max_sequence);        // what lies behind may read as NaN
-        const bool last_block = column0 + 2 * kTileRows >= item.span.count * group;
+        const bool last_block = column0 + block_columns >= item.span.count * group;
         const int* const ids_at = a.table + (size_t)item.row * a.table_stride;
         int ids = -1;                                                  // of 32 pages, a lane each
         int4 code[kStepPages];
@@ -599,12 +599,13 @@ cudaError_t launch_prompts(const Kv8AttentionArgs& a, cudaStream_t stream) {
     }
     const cudaError_t e = kv8_allow_smem(allowed, kv8_prompt_kernel<HD, E4M3>, (int)PromptSmem<HD>::kBytes);
     if (e != cudaSuccess) return e;
-    // as many items as any split of the tokens over the rows can make
+    // as many items as any split of the tokens over the rows can make; of one tile where two would leave SMs idle
     const long long columns = (long long)a.tokens * (a.query_heads / a.cache.heads);
     const long long rows = columns / (kKv8RowColumns + 1) < a.rows ? columns / (kKv8RowColumns + 1) : a.rows;
-    const long long items = (columns / (2 * kTileRows) + rows) * a.cache.heads;
+    const int block_columns = (columns / (2 * kTileRows) + 1) * a.cache.heads <= 148 ? kTileRows : 2 * kTileRows;
+    const long long items = (columns / block_columns + rows) * a.cache.heads;
     if (items > 0x7fffffffll) return cudaErrorInvalidValue;
-    return launch_pdl(kv8_prompt_kernel<HD, E4M3>, dim3((unsigned)(items > 0 ? items : 1)), dim3(kPromptThreads), PromptSmem<HD>::kBytes, stream, a);
+    return launch_pdl(kv8_prompt_kernel<HD, E4M3>, dim3((unsigned)(items > 0 ? items : 1)), dim3(kPromptThreads), PromptSmem<HD>::kBytes, stream, a, block_columns);
 }
 
 }  // namespace
