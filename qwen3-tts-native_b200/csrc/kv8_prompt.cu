@@ -426,12 +426,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
             if (!__all_sync(0xffffffffu, guard.wait(&s_ready[tile][n & 1], (n >> 1) & 1))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t s_at = lanes + tile * kStep + (n & 1) * kHalf;
-            const float4* const page_scales = scales[(n >> 1) % kScaleRing] + (n & 1) * kHalfPages;
+            // (read together and ahead: beside the copies' stores and the products' operands a load from shared memory takes 300 cycles)
+            float4 page_scales[kHalfPages];
+#pragma unroll
+            for (int p = 0; p < kHalfPages; ++p) page_scales[p] = scales[(n >> 1) % kScaleRing][(n & 1) * kHalfPages + p];
             const int visible = seen - n * kHalf;                      // of the half's tokens
             if (open) {
                 // the reference becomes the largest score so far
                 float most = -INFINITY;
-#pragma unroll 1
+#pragma unroll
                 for (int p = 0; p < kHalfPages; ++p) {
                     uint32_t s[16];
                     tmem_load_16(s_at + 16 * p, s);
