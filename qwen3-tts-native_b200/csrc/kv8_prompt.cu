@@ -15,8 +15,6 @@
 #include "q3t_kernels.cuh"
 #include "q3t_tcgen05.cuh"
 
-#include <type_traits>
-
 namespace q3t {
 namespace {
 
@@ -27,7 +25,7 @@ constexpr int kHalf = kStep / 2, kHalfPages = kStepPages / 2;
 constexpr int kPromptThreads = 640;                     // warps 0..7 softmax (a tile each four), 8..11 K, 12..15 V, 16 and 17 products (a tile each)
 constexpr int kSoftmaxWarps = 8, kKeyWarp = 8, kValueWarp = 12, kProductWarp = 16;
 // What setmaxnreg hands out is what the block was launched with
-constexpr int kLaunchRegisters = 96, kSoftmaxRegisters = 136, kCopyRegisters = 72, kProductRegisters = 64;
+constexpr int kLaunchRegisters = 96, kSoftmaxRegisters = 144, kCopyRegisters = 72, kProductRegisters = 48;
 static_assert(2 * kSoftmaxRegisters + 2 * kCopyRegisters + kProductRegisters <= 5 * kLaunchRegisters, "registers of the five warpgroups");
 constexpr int kScaleRing = 4;                           // steps whose scales are kept: K runs two steps ahead of the softmax
 constexpr uint32_t kTmemCols = 512, kOut = 256;         // scores of the tiles at 0 and 128, outputs at 256 and 384
@@ -107,12 +105,6 @@ __device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[N]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
     for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));        // not to be used ahead of the wait
-}
-__device__ __forceinline__ void tmem_load_8(uint32_t taddr, uint32_t (&r)[8]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                 : "r"(taddr)
-                 : "memory");
 }
 __device__ __forceinline__ void tmem_store_8(uint32_t taddr, const uint32_t (&r)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
@@ -408,7 +400,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         const uint32_t o_at = lanes + kOut + tile * 128;
         const int own = tile < tiles ? halves : 0;
         float top = real ? -INFINITY : 0.0f, total = 0.0f;
-        bool open = true;                                              // some row of the warp has no reference yet
+        int settled = 0;                                               // halves that every row of the warp sees all of and has a reference for
         auto rescale_output = [&](float keep, int n) {                 // when the products of the halves before are done
             if (!__all_sync(0xffffffffu, guard.wait(&o_ready[tile][(n - 1) & 1], ((n - 1) >> 1) & 1))) return;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -430,109 +422,88 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
             float4 page_scales[kHalfPages];
 #pragma unroll
             for (int p = 0; p < kHalfPages; ++p) page_scales[p] = scales[(n >> 1) % kScaleRing][(n & 1) * kHalfPages + p];
-            const int visible = seen - n * kHalf;                      // of the half's tokens
-            if (open) {
-                // the reference becomes the largest score so far
+            uint32_t s[2][32];
+            tmem_load_32(s_at, s[0]);
+            tmem_load_32(s_at + 32, s[1]);
+            tmem_wait_load(s[0]);
+            tmem_wait_load(s[1]);
+            // No maximum is looked for: a weight is at most its page's sum, which says whether one may have outgrown fp16
+            bool written = false;
+            if (n < settled) {
+                const float reference = top - kKv8Lift;
+                uint32_t w[2][16];
+                float largest = 0.0f, added = 0.0f;
+#pragma unroll
+                for (int p = 0; p < kHalfPages; ++p) {
+                    const float4 f = page_scales[p];
+                    const float slope = f.x * up, shift = f.y - reference;
+                    const unsigned long long slope2 = pack2(slope, slope), shift2 = pack2(shift, shift);
+                    unsigned long long sums[2];
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) {
+                        const uint32_t* const at = &s[p >> 1][(p & 1) * 16 + j];
+                        float x, y;
+                        unpack2(fma2(pack2(__uint_as_float(at[0]), __uint_as_float(at[1])), slope2, shift2), x, y);
+                        x = exp2_ftz(x);
+                        y = exp2_ftz(y);
+                        sums[(j >> 1) & 1] = j < 4 ? pack2(x, y) : add2(sums[(j >> 1) & 1], pack2(x, y));
+                        w[p >> 1][(p & 1) * 8 + j / 2] = pack_half2(x, y);
+                    }
+                    float x, y;
+                    unpack2(add2(sums[0], sums[1]), x, y);
+                    x += y;
+                    largest = fmaxf(largest, x);
+                    added = fmaf(x, f.z, added);
+                }
+                if (!__any_sync(0xffffffffu, largest > kMostWeight)) {
+                    total += added;
+                    tmem_store_16(s_at, w[0]);
+                    tmem_store_16(s_at + 16, w[1]);
+                    written = true;
+                } else {
+                    tmem_load_32(s_at, s[0]);
+                    tmem_load_32(s_at + 32, s[1]);
+                    tmem_wait_load(s[0]);
+                    tmem_wait_load(s[1]);
+                }
+            }
+            if (!written) {
+                // ---- halves that some row does not see all of, and scores that have outgrown their reference
+                const int visible = seen - n * kHalf;                  // of the half's tokens
                 float most = -INFINITY;
 #pragma unroll
                 for (int p = 0; p < kHalfPages; ++p) {
-                    uint32_t s[16];
-                    tmem_load_16(s_at + 16 * p, s);
-                    tmem_wait_load(s);
                     float m = -INFINITY;
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) m = fmaxf(m, 16 * p + j >= visible ? -INFINITY : __uint_as_float(s[j]));
-                    const float4 f = page_scales[p];
-                    most = fmaxf(most, m == -INFINITY ? m : fmaf(m, f.x * up, f.y));
+                    for (int j = 0; j < 16; ++j) {
+                        m = fmaxf(m, 16 * p + j >= visible ? -INFINITY : __uint_as_float(s[p >> 1][(p & 1) * 16 + j]));
+                    }
+                    most = fmaxf(most, m == -INFINITY ? m : fmaf(m, page_scales[p].x * up, page_scales[p].y));
                 }
-                const float moved = fmaxf(top, most), keep = moved == top ? 1.0f : exp2_ftz(top - moved);
+                const float moved = most > top + kKv8Slack ? most : top, keep = moved == top ? 1.0f : exp2_ftz(top - moved);
                 top = moved;
                 total *= keep;
-                if (n > 0) rescale_output(keep, n);
-                open = __any_sync(0xffffffffu, top == -INFINITY);
-            }
-            auto weigh = [&](auto mask) {
+                if (n > 0 && __any_sync(0xffffffffu, keep != 1.0f)) rescale_output(keep, n);
+                settled = __any_sync(0xffffffffu, top == -INFINITY) ? 0 : unmasked;
                 // (nothing but -inf so far: weights of zero)
-                float reference = top == -INFINITY ? 0.0f : top - kKv8Lift;
-                uint32_t s[2][32];
-                tmem_load_32(s_at, s[0]);
-                tmem_load_32(s_at + 32, s[1]);
+                const float reference = top == -INFINITY ? 0.0f : top - kKv8Lift;
 #pragma unroll
-                for (int c = 0; c < kHalf / 32; ++c) {
-                    if (c == 0) {
-                        tmem_wait_load(s[0]);
-                        tmem_wait_load(s[1]);
+                for (int p = 0; p < kHalfPages; ++p) {
+                    uint32_t w[8];
+                    const float slope = page_scales[p].x * up, shift = page_scales[p].y - reference;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) {
+                        const uint32_t* const at = &s[p >> 1][(p & 1) * 16 + j];
+                        const float x = exp2_ftz(16 * p + j >= visible ? -INFINITY : fmaf(__uint_as_float(at[0]), slope, shift));
+                        const float y = exp2_ftz(16 * p + j + 1 >= visible ? -INFINITY : fmaf(__uint_as_float(at[1]), slope, shift));
+                        sum += x + y;
+                        w[j / 2] = pack_half2(x, y);
                     }
-                    uint32_t w[16];
-                    float largest, added;
-                    auto pages = [&]() {
-                        largest = added = 0.0f;
-#pragma unroll
-                        for (int p = 0; p < 2; ++p) {
-                            const float4 f = page_scales[2 * c + p];
-                            const float slope = f.x * up, shift = f.y - reference;
-                            const unsigned long long slope2 = pack2(slope, slope), shift2 = pack2(shift, shift);
-                            unsigned long long sums[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
-#pragma unroll
-                            for (int j = 0; j < 16; j += 2) {
-                                const uint32_t* const at = &s[c][16 * p + j];
-                                float x, y;
-                                unpack2(fma2(pack2(__uint_as_float(at[0]), __uint_as_float(at[1])), slope2, shift2), x, y);
-                                if (mask.value) {
-                                    if (32 * c + 16 * p + j >= visible) x = -INFINITY;
-                                    if (32 * c + 16 * p + j + 1 >= visible) y = -INFINITY;
-                                }
-                                x = exp2_ftz(x);
-                                y = exp2_ftz(y);
-                                sums[(j >> 1) & 1] = add2(sums[(j >> 1) & 1], pack2(x, y));
-                                w[8 * p + j / 2] = pack_half2(x, y);
-                            }
-                            float x, y;
-                            unpack2(add2(sums[0], sums[1]), x, y);
-                            x += y;
-                            largest = fmaxf(largest, x);
-                            added = fmaf(x, f.z, added);
-                        }
-                    };
-                    // No maximum is looked for: a weight is at most its page's sum, which says whether one may have outgrown fp16.  The
-                    // reference then rises by a whole number, so that the weights that are stored already shrink exactly.
-                    pages();
-                    if (__any_sync(0xffffffffu, largest > kMostWeight)) {
-                        float rise = 0.0f;
-#pragma unroll
-                        for (int p = 0; p < 2; ++p) {
-                            const float4 f = page_scales[2 * c + p];
-                            float most = -INFINITY;
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) most = fmaxf(most, mask.value && 32 * c + 16 * p + j >= visible ? -INFINITY : __uint_as_float(s[c][16 * p + j]));
-                            if (most > -INFINITY) rise = fmaxf(rise, ceilf(fmaf(most, f.x * up, f.y - reference) - kKv8Lift));
-                        }
-                        if (!(largest > kMostWeight)) rise = 0.0f;
-                        const float keep = exp2_ftz(-rise);
-                        top += rise;
-                        reference += rise;
-                        total *= keep;
-                        if (n > 0) rescale_output(keep, n);
-                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-#pragma unroll 1
-                        for (int before = 0; before < 2 * c; ++before) {
-                            uint32_t h[8];
-                            tmem_load_8(s_at + 8 * before, h);
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
-                                h[j] = pack_half2(x.x * keep, x.y * keep);
-                            }
-                            tmem_store_8(s_at + 8 * before, h);
-                        }
-                        pages();
-                    }
-                    total += added;
-                    tmem_store_16(s_at + 16 * c, w);
+                    total = fmaf(sum, page_scales[p].z, total);
+                    tmem_store_8(s_at + 8 * p, w);
                 }
-            };
-            if (n < unmasked) weigh(std::false_type{});
-            else weigh(std::true_type{});
+            }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
