@@ -143,6 +143,15 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+// 2^n, -126 <= n <= 127
+__device__ __forceinline__ float power_of_two(int n) { return __uint_as_float((uint32_t)(n + 127) << 23); }
+// A query's way to fp16: times 2^shift its largest value, of which `most` is the bf16 without its sign, lies in 2^7..2^8 (or as near
+// as fp32 can scale it; what is not finite stays so).  The score's scale takes it back.
+__device__ __forceinline__ int query_shift(uint32_t most) { return min(134 - (int)min(most >> 7, 254u), 127); }
+__device__ __forceinline__ float query_back(float scale, int shift) {
+    const int half = shift / 2;
+    return scale * power_of_two(-half) * power_of_two(half - shift);
+}
 // four codes as two pairs of fp16
 template <bool E4M3>
 __device__ __forceinline__ void codes_to_half(uint32_t word, uint32_t& lo, uint32_t& hi) {

@@ -222,9 +222,9 @@ struct Walk {
             most = max(most & 0xffffu, most >> 16);
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-            const int shift = min(134 - (int)min(most >> 7, 254u), 127);
-            const float up = ldexpf(1.0f, shift);
-            column_scale[n] = ldexpf(a.scale * 1.4426950408889634f, -shift);
+            const int shift = query_shift(most);
+            const float up = power_of_two(shift);
+            column_scale[n] = query_back(a.scale * 1.4426950408889634f, shift);
 #pragma unroll
             for (int j = 0; j < kParts; ++j) {
 #pragma unroll

@@ -359,31 +359,38 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
         // ---- queries to fp16, by a power of two that brings the largest of each to 2^7..2^8
         constexpr int kLanes = HD / 8, kAtOnce = kWarp / kLanes;       // of a row, rows of a warp
-#pragma unroll 4
-        for (int i = 0; i < 2 * kTileRows / (kSoftmaxWarps * kAtOnce); ++i) {
-            const int r = warp * (2 * kTileRows / kSoftmaxWarps) + i * kAtOnce + lane / kLanes, piece = lane % kLanes;
-            const int column = column0 + r, token = column / group;
-            int4 raw = make_int4(0, 0, 0, 0);
-            if (r < columns) {
-                raw = *reinterpret_cast<const int4*>(a.query + (size_t)(item.span.first + token) * a.query_stride
-                                                     + (size_t)(item.kv_head * group + column - token * group) * HD + piece * 8);
+        constexpr int kRounds = kTileRows / (kSoftmaxWarps * kAtOnce);
+        for (int t = 0; t < tiles; ++t) {
+            int4 raw[kRounds];                                         // one latency
+            const int piece = lane % kLanes, r0 = t * kTileRows + warp * (kTileRows / kSoftmaxWarps) + lane / kLanes;
+#pragma unroll
+            for (int i = 0; i < kRounds; ++i) {
+                const int r = r0 + i * kAtOnce, column = column0 + r, token = column / group;
+                raw[i] = make_int4(0, 0, 0, 0);
+                if (r < columns) {
+                    raw[i] = *reinterpret_cast<const int4*>(a.query + (size_t)(item.span.first + token) * a.query_stride
+                                                            + (size_t)(item.kv_head * group + column - token * group) * HD + piece * 8);
+                }
             }
-            const uint32_t x[4] = {(uint32_t)raw.x, (uint32_t)raw.y, (uint32_t)raw.z, (uint32_t)raw.w};
-            uint32_t most = 0u;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) most = __vmaxu2(most, x[e] & 0x7fff7fffu);
-            most = max(most & 0xffffu, most >> 16);
+            for (int i = 0; i < kRounds; ++i) {
+                const uint32_t x[4] = {(uint32_t)raw[i].x, (uint32_t)raw[i].y, (uint32_t)raw[i].z, (uint32_t)raw[i].w};
+                uint32_t most = 0u;
 #pragma unroll
-            for (int o = 1; o < kLanes; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-            const int shift = min(134 - (int)min(most >> 7, 254u), 127);
-            const float up = ldexpf(1.0f, shift);
-            int4 h;
-            h.x = (int)pack_half2(bf_lo(x[0]) * up, bf_hi(x[0]) * up);
-            h.y = (int)pack_half2(bf_lo(x[1]) * up, bf_hi(x[1]) * up);
-            h.z = (int)pack_half2(bf_lo(x[2]) * up, bf_hi(x[2]) * up);
-            h.w = (int)pack_half2(bf_lo(x[3]) * up, bf_hi(x[3]) * up);
-            *reinterpret_cast<int4*>(queries + (r / kTileRows) * kTileRows * HD * 2 + tile_offset(r % kTileRows, piece)) = h;
-            if (piece == 0) row_scale[r] = ldexpf(a.scale * 1.4426950408889634f, -shift);
+                for (int e = 0; e < 4; ++e) most = __vmaxu2(most, x[e] & 0x7fff7fffu);
+                most = max(most & 0xffffu, most >> 16);
+#pragma unroll
+                for (int o = 1; o < kLanes; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+                const int shift = query_shift(most), r = r0 + i * kAtOnce;
+                const float up = power_of_two(shift);
+                int4 h;
+                h.x = (int)pack_half2(bf_lo(x[0]) * up, bf_hi(x[0]) * up);
+                h.y = (int)pack_half2(bf_lo(x[1]) * up, bf_hi(x[1]) * up);
+                h.z = (int)pack_half2(bf_lo(x[2]) * up, bf_hi(x[2]) * up);
+                h.w = (int)pack_half2(bf_lo(x[3]) * up, bf_hi(x[3]) * up);
+                *reinterpret_cast<int4*>(queries + t * kTileRows * HD * 2 + tile_offset(r % kTileRows, piece)) = h;
+                if (piece == 0) row_scale[r] = query_back(a.scale * 1.4426950408889634f, shift);
+            }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
