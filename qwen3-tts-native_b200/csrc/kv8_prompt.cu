@@ -176,11 +176,22 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
     }
     const int column0 = item.block * block_columns;
     const int columns = min(block_columns, item.span.count * group - column0);
-    // tokens that the last column of each tile sees
-    auto seen_by = [&](int column) { return min(max(item.span.base + column / group + 1, 0), a.max_sequence); };
+    // of column r of the item the token, among the row's new ones, and the head among the KV head's: one division, and a product that is
+    // exact for what is below 320
+    const int token0 = column0 / group, rest0 = column0 - token0 * group;
+    const float per_group = 1.0f / static_cast<float>(group);
+    auto place_of = [&](int r, int& head) {
+        const int more = (int)((static_cast<float>(rest0 + r) + 0.5f) * per_group);
+        head = rest0 + r - more * group;
+        return token0 + more;
+    };
+    auto seen_by = [&](int r) {
+        int head;
+        return min(max(item.span.base + place_of(r, head) + 1, 0), a.max_sequence);
+    };
     // (both tiles go as far as the second one's last column sees; one that is empty not at all)
     const int tiles = columns > kTileRows ? 2 : 1;
-    const int halves = (seen_by(column0 + columns - 1) + kHalf - 1) / kHalf, steps = (halves + 1) / 2;
+    const int halves = (seen_by(columns - 1) + kHalf - 1) / kHalf, steps = (halves + 1) / 2;
 
     Guard guard;
     guard.deadline = clock64() + kBudgetCycles;
@@ -360,28 +371,34 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         // ---- queries to fp16, by a power of two that brings the largest of each to 2^7..2^8
         constexpr int kLanes = HD / 8, kAtOnce = kWarp / kLanes;       // of a row, rows of a warp
         constexpr int kRounds = kTileRows / (kSoftmaxWarps * kAtOnce);
-        for (int t = 0; t < tiles; ++t) {
-            int4 raw[kRounds];                                         // one latency
-            const int piece = lane % kLanes, r0 = t * kTileRows + warp * (kTileRows / kSoftmaxWarps) + lane / kLanes;
+        int4 raw[2][kRounds];                                          // one latency
+        const int piece = lane % kLanes;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
 #pragma unroll
             for (int i = 0; i < kRounds; ++i) {
-                const int r = r0 + i * kAtOnce, column = column0 + r, token = column / group;
-                raw[i] = make_int4(0, 0, 0, 0);
+                const int r = t * kTileRows + warp * (kTileRows / kSoftmaxWarps) + i * kAtOnce + lane / kLanes;
+                raw[t][i] = make_int4(0, 0, 0, 0);
                 if (r < columns) {
-                    raw[i] = *reinterpret_cast<const int4*>(a.query + (size_t)(item.span.first + token) * a.query_stride
-                                                            + (size_t)(item.kv_head * group + column - token * group) * HD + piece * 8);
+                    int head;
+                    const size_t token = item.span.first + place_of(r, head);
+                    raw[t][i] = *reinterpret_cast<const int4*>(a.query + token * a.query_stride + (size_t)(item.kv_head * group + head) * HD + piece * 8);
                 }
             }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            if (t >= tiles) break;
 #pragma unroll
             for (int i = 0; i < kRounds; ++i) {
-                const uint32_t x[4] = {(uint32_t)raw[i].x, (uint32_t)raw[i].y, (uint32_t)raw[i].z, (uint32_t)raw[i].w};
+                const uint32_t x[4] = {(uint32_t)raw[t][i].x, (uint32_t)raw[t][i].y, (uint32_t)raw[t][i].z, (uint32_t)raw[t][i].w};
                 uint32_t most = 0u;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) most = __vmaxu2(most, x[e] & 0x7fff7fffu);
                 most = max(most & 0xffffu, most >> 16);
 #pragma unroll
                 for (int o = 1; o < kLanes; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-                const int shift = query_shift(most), r = r0 + i * kAtOnce;
+                const int shift = query_shift(most), r = t * kTileRows + warp * (kTileRows / kSoftmaxWarps) + i * kAtOnce + lane / kLanes;
                 const float up = power_of_two(shift);
                 int4 h;
                 h.x = (int)pack_half2(bf_lo(x[0]) * up, bf_hi(x[0]) * up);
@@ -400,7 +417,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         const int tile = warp >> 2, quarter = warp & 3;
         const int r = tile * kTileRows + quarter * kWarp + lane;
         const bool real = r < columns;
-        const int seen = real ? seen_by(column0 + r) : 0;
+        const int seen = real ? seen_by(r) : 0;
         const int unmasked = (int)__reduce_min_sync(0xffffffffu, (unsigned int)seen) / kHalf;      // halves all of which every row of the warp sees
         const float up = row_scale[r];
         const uint32_t lanes = tmem + ((uint32_t)(quarter * kWarp) << 16);
@@ -522,28 +539,32 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-        const int column = column0 + min(r, columns - 1), i = column / group;
-        const size_t token = item.span.first + i, at = (size_t)(item.kv_head * group + column - i * group) * HD;
+        int head;
+        const size_t token = item.span.first + place_of(min(r, columns - 1), head), at = (size_t)(item.kv_head * group + head) * HD;
 #pragma unroll 1
-        for (int c = 0; c < HD; c += 16) {
-            float o[16];
+        for (int c = 0; c < HD; c += 64) {
+            uint32_t o[2][32];
             if (own > 0) {
-                tc::tmem_load_row<16>(o_at + c, o);
+                tmem_load_32(o_at + c, o[0]);
+                tmem_load_32(o_at + c + 32, o[1]);
+                tmem_wait_load(o[0]);
+                tmem_wait_load(o[1]);
             }
             if (!real || *abort_flag != 0) continue;
+            // (8 dims)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) o[j] = own > 0 ? o[j] * inverse : 0.0f;
+            for (int j = 0; j < 64; j += 8) {
+                float v[8];
 #pragma unroll
-            for (int j = 0; j < 16; j += 8) {
+                for (int e = 0; e < 8; ++e) v[e] = own > 0 ? __uint_as_float(o[j >> 5][(j & 31) + e]) * inverse : 0.0f;
                 __nv_bfloat162 x[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = __floats2bfloat162_rn(o[j + 2 * e], o[j + 2 * e + 1]);
+                for (int e = 0; e < 4; ++e) x[e] = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
                 *reinterpret_cast<int4*>(a.out + token * a.out_stride + at + c + j) = *reinterpret_cast<const int4*>(x);
-            }
-            if (a.out32 != nullptr) {
-#pragma unroll
-                for (int j = 0; j < 16; j += 4) {
-                    *reinterpret_cast<float4*>(a.out32 + token * a.query_heads * HD + at + c + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                if (a.out32 != nullptr) {
+                    float* const to = a.out32 + token * a.query_heads * HD + at + c + j;
+                    *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+                    *reinterpret_cast<float4*>(to + 4) = make_float4(v[4], v[5], v[6], v[7]);
                 }
             }
         }
