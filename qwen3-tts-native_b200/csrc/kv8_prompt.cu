@@ -129,7 +129,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
     unsigned char* const keys = smem + Smem::kQueryBytes;              // [step % 2]
     unsigned char* const values = keys + 2 * Smem::kTileBytes;         // [step % 2]
     __shared__ float4 scales[kScaleRing][kStepPages];                  // of each page: key scale, log2 and reciprocal of the value scale
-    __shared__ float row_scale[2 * kTileRows];
     // full: V of a step and K of the next one
     __shared__ uint64_t first_k, full[2], empty_k[2], empty_v[2], s_ready[2][2], p_ready[2][2], o_ready[2][2], q_ready;     // [tile][half]
     __shared__ uint32_t tmem_slot;
@@ -370,56 +369,52 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
         // ---- queries to fp16, by a power of two that brings the largest of each to 2^7..2^8
         constexpr int kLanes = HD / 8, kAtOnce = kWarp / kLanes;       // of a row, rows of a warp
-        constexpr int kRounds = kTileRows / (kSoftmaxWarps * kAtOnce);
-        int4 raw[2][kRounds];                                          // one latency
+        // copied as they are to where they belong, then turned over in place, a thread a row: a row's largest takes no shuffles, which
+        // beside the copies' stores are slow (with a row on 16 lanes 11,000 cycles an item, so 7,000)
         const int piece = lane % kLanes;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-#pragma unroll
-            for (int i = 0; i < kRounds; ++i) {
-                const int r = t * kTileRows + warp * (kTileRows / kSoftmaxWarps) + i * kAtOnce + lane / kLanes;
-                raw[t][i] = make_int4(0, 0, 0, 0);
-                if (r < columns) {
-                    int head;
-                    const size_t token = item.span.first + place_of(r, head);
-                    raw[t][i] = *reinterpret_cast<const int4*>(a.query + token * a.query_stride + (size_t)(item.kv_head * group + head) * HD + piece * 8);
-                }
-            }
+#pragma unroll 4
+        for (int q_row = warp * kAtOnce + lane / kLanes; q_row < tiles * kTileRows; q_row += kSoftmaxWarps * kAtOnce) {
+            int head;
+            const size_t token = item.span.first + place_of(min(q_row, columns - 1), head);
+            const bf16* const from = a.query + token * a.query_stride + (size_t)(item.kv_head * group + head) * HD + piece * 8;
+            const uint32_t to = tc::smem_u32(queries) + (q_row / kTileRows) * kTileRows * HD * 2 + tile_offset(q_row % kTileRows, piece);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(q_row < columns ? 16 : 0) : "memory");
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const int tile = warp >> 2, quarter = warp & 3;
+        const int r = tile * kTileRows + quarter * kWarp + lane;
+        float up = 0.0f;                                               // of the row's scores
+        if (tile < tiles) {
+            unsigned char* const row_at = queries + tile * kTileRows * HD * 2;
+            int4 raw[kLanes];
+            uint32_t most = 0u;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            if (t >= tiles) break;
+            for (int i = 0; i < kLanes; ++i) raw[i] = *reinterpret_cast<const int4*>(row_at + tile_offset(r % kTileRows, i));
 #pragma unroll
-            for (int i = 0; i < kRounds; ++i) {
-                const uint32_t x[4] = {(uint32_t)raw[t][i].x, (uint32_t)raw[t][i].y, (uint32_t)raw[t][i].z, (uint32_t)raw[t][i].w};
-                uint32_t most = 0u;
+            for (int i = 0; i < kLanes; ++i) {
+                most = __vmaxu2(most, __vmaxu2(__vmaxu2((uint32_t)raw[i].x & 0x7fff7fffu, (uint32_t)raw[i].y & 0x7fff7fffu),
+                                               __vmaxu2((uint32_t)raw[i].z & 0x7fff7fffu, (uint32_t)raw[i].w & 0x7fff7fffu)));
+            }
+            const int shift = query_shift(max(most & 0xffffu, most >> 16));
+            const float to_half = power_of_two(shift);
+            up = query_back(a.scale * 1.4426950408889634f, shift);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) most = __vmaxu2(most, x[e] & 0x7fff7fffu);
-                most = max(most & 0xffffu, most >> 16);
+            for (int i = 0; i < kLanes; ++i) {
+                const uint32_t x[4] = {(uint32_t)raw[i].x, (uint32_t)raw[i].y, (uint32_t)raw[i].z, (uint32_t)raw[i].w};
+                uint32_t h[4];
 #pragma unroll
-                for (int o = 1; o < kLanes; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-                const int shift = query_shift(most), r = t * kTileRows + warp * (kTileRows / kSoftmaxWarps) + i * kAtOnce + lane / kLanes;
-                const float up = power_of_two(shift);
-                int4 h;
-                h.x = (int)pack_half2(bf_lo(x[0]) * up, bf_hi(x[0]) * up);
-                h.y = (int)pack_half2(bf_lo(x[1]) * up, bf_hi(x[1]) * up);
-                h.z = (int)pack_half2(bf_lo(x[2]) * up, bf_hi(x[2]) * up);
-                h.w = (int)pack_half2(bf_lo(x[3]) * up, bf_hi(x[3]) * up);
-                *reinterpret_cast<int4*>(queries + t * kTileRows * HD * 2 + tile_offset(r % kTileRows, piece)) = h;
-                if (piece == 0) row_scale[r] = query_back(a.scale * 1.4426950408889634f, shift);
+                for (int e = 0; e < 4; ++e) h[e] = pack_half2(bf_lo(x[e]) * to_half, bf_hi(x[e]) * to_half);
+                *reinterpret_cast<int4*>(row_at + tile_offset(r % kTileRows, i)) = make_int4((int)h[0], (int)h[1], (int)h[2], (int)h[3]);
             }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&q_ready);
-        asm volatile("bar.sync 1, 256;" ::: "memory");                 // row_scale
         // ---- softmax: a thread a row
-        const int tile = warp >> 2, quarter = warp & 3;
-        const int r = tile * kTileRows + quarter * kWarp + lane;
         const bool real = r < columns;
         const int seen = real ? seen_by(r) : 0;
         const int unmasked = (int)__reduce_min_sync(0xffffffffu, (unsigned int)seen) / kHalf;      // halves all of which every row of the warp sees
-        const float up = row_scale[r];
         const uint32_t lanes = tmem + ((uint32_t)(quarter * kWarp) << 16);
         const uint32_t o_at = lanes + kOut + tile * 128;
         const int own = tile < tiles ? halves : 0;
