@@ -7,8 +7,16 @@
 // The reciprocal is taken once a page and head: a division a value would cost more issue slots than the memory takes time.  2^-126
 // keeps it finite and makes a page of zeros no special case.
 // The page's first new token (its slot's page is not the token's before) owns the page; a warp looks for owners in a window of
-// consecutive tokens: one token where there are few (a decode step: every token owns a page, and the pages' chains of loads
-// have to run side by side), 16 where there are many (a prompt: one or two owners a window).
+// consecutive tokens and takes them one after the other.  Where every token owns a page (a decode step) small windows let the pages'
+// chains of loads run side by side; where one or two of 16 do (a prompt) large ones spare warps that find nothing.  The host does not
+// know which it is, only how many warps windows of one token would take (tokens x 2 x heads), so the window grows where that many no
+// longer run at once: 4 from 2^14 on and 16 from 2^16 on.  Measured with 8 heads of 128, int8, in us, windows of 1 / 4 / 16:
+//   a prompt of 512 tokens 4.5 / 4.1 / 4.5, of 1,024 6.2 / 4.6 / 4.5, of 2,048 9.2 / 5.7 / 4.8, of 4,096 15.4 / 8.4 / 5.8, of 8,192 27.8 / 13.7 / 8.8;
+//   512 rows of one token 8.0 / 8.7 / 21, 1,024 14.1 / 14.0 / 21, 2,048 26.0 / 23.0 / 28, 4,096 51.8 / 43.9 / 50.3.
+//
+// What bounds it: a decode step the latency of five loads and sums one behind the other (64 rows: 3.0 us); a large batch memory (65,536
+// tokens in rows of 1 to 8,192, 302 MB: 54.5 us, 5.5 TB/s;
+// three CTAs an SM instead of four, with more registers: 60.9 us).  A prompt of 1,500 tokens takes 4.8 us (4 an SM: 5.1).
 
 #include "kv8.cuh"
 #include "q3t_kernels.cuh"
@@ -18,7 +26,7 @@ namespace {
 
 constexpr int kAppendThreads = 256;
 constexpr int kAppendWarps = kAppendThreads / kWarp;
-constexpr int kManyTokens = 2048;              // from here on windows of 16
+constexpr long long kManyWarps = 1 << 14, kMostWarps = 1 << 16;      // windows of 4 and of 16 tokens from here on
 
 __device__ unsigned int g_kv8_nonfinite = 0;
 __device__ unsigned int g_kv8_append_page_errors = 0;
@@ -70,7 +78,7 @@ __device__ __forceinline__ void unpack_codes(uint32_t word, float (&v)[4]) {
 }
 
 template <int HD, bool E4M3, int WINDOW>
-__global__ void __launch_bounds__(kAppendThreads, 4) kv8_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, WINDOW == 4 ? 3 : 4) kv8_append_kernel(const AppendArgs a) {
     constexpr int kLanes = HD / 8;                        // of a token: 8 values each
     constexpr int kAtOnce = kWarp / kLanes;               // tokens
     constexpr int kRounds = kPageTokens / kAtOnce;
@@ -196,11 +204,13 @@ __global__ void __launch_bounds__(kAppendThreads, 4) kv8_append_kernel(const App
 
 template <int HD, bool E4M3>
 cudaError_t launch_append(const AppendArgs& a, cudaStream_t stream) {
-    const int window = a.tokens < kManyTokens ? 1 : kPageTokens;
-    const long long warps = (long long)((a.tokens + window - 1) / window) * 2 * a.cache.heads;
-    const dim3 grid((unsigned)((warps + kAppendWarps - 1) / kAppendWarps));
-    return window == 1 ? launch_pdl(kv8_append_kernel<HD, E4M3, 1>, grid, dim3(kAppendThreads), 0, stream, a)
-                       : launch_pdl(kv8_append_kernel<HD, E4M3, kPageTokens>, grid, dim3(kAppendThreads), 0, stream, a);
+    const long long heads = 2 * a.cache.heads, most = heads * a.tokens;
+    const int window = most < kManyWarps ? 1 : most < kMostWarps ? 4 : kPageTokens;
+    const long long warps = (a.tokens + window - 1) / window * heads;
+    const dim3 grid((unsigned)((warps + kAppendWarps - 1) / kAppendWarps)), block(kAppendThreads);
+    return window == 1 ? launch_pdl(kv8_append_kernel<HD, E4M3, 1>, grid, block, 0, stream, a)
+           : window == 4 ? launch_pdl(kv8_append_kernel<HD, E4M3, 4>, grid, block, 0, stream, a)
+                         : launch_pdl(kv8_append_kernel<HD, E4M3, kPageTokens>, grid, block, 0, stream, a);
 }
 
 }  // namespace

@@ -47,10 +47,11 @@ def test_rows_of_tokens(ops, e4m3, heads, dim, held, new):
 
 
 @pytest.mark.parametrize("e4m3", [False, True])
-def test_windows_of_many_tokens(ops, e4m3):
-    """Enough tokens for the kernel's larger windows: whole and broken pages, single tokens, padding between them."""
+@pytest.mark.parametrize("heads", [2, 8, 16])
+def test_windows_of_many_tokens(ops, heads, e4m3):
+    """The kernel's three windows, which grow with tokens and heads: whole and broken pages, single tokens, padding between them."""
     rng = np.random.default_rng(11)
-    heads, dim, pages = 2, 64, 400
+    dim, pages = 64, 400
     held = [int(x) for x in rng.integers(0, 40, 60)]
     new = [1 if rng.integers(0, 2) else int(rng.integers(1, 90)) for _ in held]
     new[-1] += max(0, 2111 - sum(new))
