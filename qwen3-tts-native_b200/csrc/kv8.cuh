@@ -103,7 +103,6 @@ __device__ __forceinline__ RowSpan row_span(const int* starts, const int* length
 
 constexpr float kKv8Slack = 8.0f;         // log2 of how far a score may exceed its row's reference
 constexpr float kKv8Lift = 6.0f;          // log2 of the weight at the reference
-constexpr int kKv8RowColumns = 64;        // (new tokens x query heads of a KV head) of a row up to which kv8_attention.cu takes it
 
 struct Kv8AttentionArgs {
     Kv8View cache;
@@ -121,6 +120,7 @@ struct Kv8AttentionArgs {
     float scale;
     void* scratch;
     int prompts;              // a launch of kv8_prompt.cu follows
+    int row_columns;          // (new tokens x query heads of a KV head) of a row up to which it is not that one's
 };
 
 __device__ __forceinline__ float exp2_ftz(float x) {

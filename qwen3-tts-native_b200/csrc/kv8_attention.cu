@@ -33,8 +33,9 @@ constexpr int kRowWarps = kRowThreads / kWarp;
 constexpr int kRowCtas = 2 * 148;
 constexpr int kTileColumns = 8;                        // of a product
 constexpr int kStartUnits = 2;                         // what the start of a segment counts for in the cut, in pages
-constexpr int kClusterCtas = 8;
-constexpr int kFewTokens = 8192;                       // of a row, up to which a cluster a segment is the shortest way
+constexpr int kClusterCtas = 8;                        // the most of a segment
+constexpr int kFewCtas = 256, kFewTokens = 1024, kFewest = 64;
+constexpr int kRowColumns = 32, kPromptColumns = 4096, kShort = 1024;
 constexpr int kCounterBytes = (kRowCtas * 4 + 255) / 256 * 256;
 
 __device__ unsigned int g_kv8_range_errors = 0;
@@ -97,7 +98,7 @@ __device__ __forceinline__ RowWork row_work(const Kv8AttentionArgs& a, int row, 
     RowWork w;
     w.span = row_span(a.starts, a.lengths, row, a.tokens, a.most, a.max_sequence);
     w.last = min(max(w.span.base + w.span.count, 0), a.max_sequence);
-    w.blocks = w.span.count * group > kKv8RowColumns ? 0 : (w.span.count * group + block_columns - 1) / block_columns;
+    w.blocks = w.span.count * group > a.row_columns ? 0 : (w.span.count * group + block_columns - 1) / block_columns;
     w.pages = max(1, (w.last + kPageTokens - 1) / kPageTokens);
     return w;
 }
@@ -509,7 +510,7 @@ __global__ void __launch_bounds__(kRowThreads, rows_residency<HD, TILES>()) kv8_
     }
     __syncthreads();
 
-    // ---- pieces of a segment that lie in this CTA stand in order; a warp a segment merges them
+    // ---- pieces of a segment that lie in this CTA stand in order; warps merge them, 32 times 8 dims of its columns each
     float* const left = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + kCounterBytes);
     auto left_by = [&](int cta, int which) { return left + (size_t)(2 * cta + which) * kPiece; };
     // the CTA whose range has a unit
@@ -520,6 +521,13 @@ __global__ void __launch_bounds__(kRowThreads, rows_residency<HD, TILES>()) kv8_
         for (int e = 0; e < 8; ++e) v.sum[e] *= inverse;
         write8<HD>(a, p.first, p.kv_head, p.column + column, d, v.sum);
     };
+    auto put = [&](float* piece, int column, int d, const Merged& v) {
+        float* const to = piece + column * kPitch;
+        *reinterpret_cast<float4*>(to + d) = make_float4(v.sum[0], v.sum[1], v.sum[2], v.sum[3]);
+        *reinterpret_cast<float4*>(to + d + 4) = make_float4(v.sum[4], v.sum[5], v.sum[6], v.sum[7]);
+        if (d == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(v.top, v.total);
+    };
+    auto chunks_of = [](const Piece& p) { return (p.columns * (HD / 8) + kWarp - 1) / kWarp; };
     {
         const long long mine = lane < 2 * kRowWarps ? held[lane].start : -1;
         const unsigned int real = __ballot_sync(0xffffffffu, mine >= 0);
@@ -567,13 +575,16 @@ __global__ void __launch_bounds__(kRowThreads, rows_residency<HD, TILES>()) kv8_
         return;
     }
     __threadfence();
-    // all warps for one segment, half of them each for two; a warp takes pieces share, share + shares, ...
-    const int shares = kRowWarps / folding, share = warp % shares, which = folding == 2 ? warp / shares : (folds[0] >= 0 ? 0 : 1);
+    // all warps for one segment, half of them each for two: of each 32 times 8 dims several warps share the pieces where there are more
+    const int warps_here = kRowWarps / folding, own_warp = warp % warps_here, which = folding == 2 ? warp / warps_here : (folds[0] >= 0 ? 0 : 1);
     const Piece p = held[folds[which]];
-    {
+    const int chunks = chunks_of(p), shares = max(1, warps_here / chunks), share = own_warp / chunks;
+    float* const shared_by = parts + (size_t)(folding == 2 ? which * warps_here : 0) * kPiece;
+    if (share < shares) {
         const int first_cta = owner(p.start), count = owner(p.start + p.pages - 1) - first_cta + 1;
-        for (int x = lane; x < p.columns * (HD / 8); x += kWarp) {
-            const int column = x / (HD / 8), d = x % (HD / 8) * 8;
+        for (int chunk = own_warp % chunks; chunk < chunks; chunk += warps_here) {
+            const int x = chunk * kWarp + lane, column = x / (HD / 8), d = x % (HD / 8) * 8;
+            if (column >= p.columns) continue;
             Merged v;
             constexpr int kAtOnce = 4;
             for (int n0 = share; n0 < count; n0 += kAtOnce * shares) {
@@ -593,36 +604,37 @@ __global__ void __launch_bounds__(kRowThreads, rows_residency<HD, TILES>()) kv8_
                     if (n0 + i * shares < count) v.add(stats[i], lo[i], hi[i]);
                 }
             }
-            float* const to = parts + (size_t)warp * kPiece + column * kPitch;
-            *reinterpret_cast<float4*>(to + d) = make_float4(v.sum[0], v.sum[1], v.sum[2], v.sum[3]);
-            *reinterpret_cast<float4*>(to + d + 4) = make_float4(v.sum[4], v.sum[5], v.sum[6], v.sum[7]);
-            if (d == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(v.top, v.total);
+            if (shares == 1) finish(p, column, d, v);
+            else put(shared_by + (size_t)share * kPiece, column, d, v);
         }
     }
     __syncthreads();
-    for (int x = share * kWarp + lane; x < p.columns * (HD / 8); x += shares * kWarp) {
-        const int column = x / (HD / 8), d = x % (HD / 8) * 8;
-        Merged v;
-        for (int n = 0; n < shares; ++n) {
-            const float* const from = parts + (size_t)((folding == 2 ? which * shares : 0) + n) * kPiece + column * kPitch;
-            v.add(*reinterpret_cast<const float2*>(from + HD), *reinterpret_cast<const float4*>(from + d), *reinterpret_cast<const float4*>(from + d + 4));
+    if (shares > 1) {
+        for (int x = own_warp * kWarp + lane; x < p.columns * (HD / 8); x += warps_here * kWarp) {
+            const int column = x / (HD / 8), d = x % (HD / 8) * 8;
+            Merged v;
+            for (int n = 0; n < shares; ++n) {
+                const float* const from = shared_by + (size_t)n * kPiece + column * kPitch;
+                v.add(*reinterpret_cast<const float2*>(from + HD), *reinterpret_cast<const float4*>(from + d), *reinterpret_cast<const float4*>(from + d + 4));
+            }
+            finish(p, column, d, v);
         }
-        finish(p, column, d, v);
     }
     pdl_trigger();
 }
 
-// Few segments (one listener, or a few): a cluster each, whose 64 warps share its pages.  What they leave is merged through distributed
-// shared memory: no sums over the batch, no tickets, no way through the L2 and back.
-template <int HD, bool E4M3, int TILES>
-__global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kRowThreads, rows_residency<HD, TILES>()) kv8_few_rows_kernel(const Kv8AttentionArgs a, int blocks) {
-    using W = Walk<HD, E4M3, TILES>;
-    constexpr int kWarpsOf = kClusterCtas * kRowWarps, kItems = HD / 8;                    // of a segment; of a column
+// Segments that a CTA each, or a cluster of 2, 4 or 8, gets through sooner than the ranges above get started: its warps share the
+// segment's pages.  What the CTAs of a cluster leave is merged through distributed shared memory: no sums over the batch, no tickets, no
+// way through the L2 and back.
+template <int HD, bool E4M3>
+__global__ void __launch_bounds__(kRowThreads, 2) kv8_few_rows_kernel(const Kv8AttentionArgs a, int blocks, int cluster) {
+    using W = Walk<HD, E4M3, 1>;
+    constexpr int kItems = HD / 8;                                                          // of a column
     extern __shared__ __align__(16) unsigned char smem[];
     float* const parts = reinterpret_cast<float*>(smem);                                    // a piece a warp, then the CTA's
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid / kWarp, 0);
     const int heads = a.cache.heads, group = a.query_heads / heads;
-    const int rank = (int)(blockIdx.x % kClusterCtas), number = (int)(blockIdx.x / kClusterCtas), block = number % blocks;
+    const int number = (int)blockIdx.x / cluster, rank = (int)blockIdx.x - number * cluster, block = number % blocks;
     const int kv_head = number / blocks % heads, row = number / blocks / heads;
     pdl_wait();
     pdl_trigger();
@@ -630,14 +642,20 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kRowThrea
     if (w.span.cut && tid == 0 && rank == 0 && block == 0 && kv_head == 0) atomicAdd(&g_kv8_range_errors, 1u);
     if (block >= w.blocks) return;                                                          // the whole cluster
     const Segment of{row, kv_head, block * W::kColumns, min(W::kColumns, w.span.count * group - block * W::kColumns), kv_head == 0 && block == 0};
-    const int which = rank * kRowWarps + warp;
-    const int page_first = (int)((long long)w.pages * which / kWarpsOf), page_end = (int)((long long)w.pages * (which + 1) / kWarpsOf);
+    const int which = rank * kRowWarps + warp, warps = cluster * kRowWarps;
+    const int page_first = (int)((long long)w.pages * which / warps), page_end = (int)((long long)w.pages * (which + 1) / warps);
     {
         W walk;
         if (page_first < page_end) walk.run(a, w, of, page_first, page_end);
         walk.keep(parts + (size_t)warp * W::kPiece, of.columns);
     }
     __syncthreads();
+    auto finish = [&](Merged& v, int column, int d) {
+        const float inverse = v.total == 0.0f ? 0.0f : 1.0f / v.total;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v.sum[e] *= inverse;
+        write8<HD>(a, w.span.first, kv_head, of.column + column, d, v.sum);
+    };
     float* const own = parts + (size_t)kRowWarps * W::kPiece;
     for (int x = tid; x < of.columns * kItems; x += kRowThreads) {
         const int column = x / kItems, d = x % kItems * 8;
@@ -647,41 +665,54 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kRowThrea
             const float* const from = parts + (size_t)n * W::kPiece + column * W::kPitch;
             v.add(*reinterpret_cast<const float2*>(from + HD), *reinterpret_cast<const float4*>(from + d), *reinterpret_cast<const float4*>(from + d + 4));
         }
+        if (cluster == 1) {
+            finish(v, column, d);
+            continue;
+        }
         float* const to = own + column * W::kPitch;
         *reinterpret_cast<float4*>(to + d) = make_float4(v.sum[0], v.sum[1], v.sum[2], v.sum[3]);
         *reinterpret_cast<float4*>(to + d + 4) = make_float4(v.sum[4], v.sum[5], v.sum[6], v.sum[7]);
         if (d == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(v.top, v.total);
     }
+    if (cluster == 1) return;
     tc::cluster_sync();
-    for (int x = tid * kClusterCtas + rank; x < of.columns * kItems; x += kRowThreads * kClusterCtas) {
+    for (int x = tid * cluster + rank; x < of.columns * kItems; x += kRowThreads * cluster) {
         const int column = x / kItems, d = x % kItems * 8;
         Merged v;
-#pragma unroll
-        for (int n = 0; n < kClusterCtas; ++n) {
+#pragma unroll 8
+        for (int n = 0; n < cluster; ++n) {
             const uint32_t from = tc::peer_smem(tc::smem_u32(own + column * W::kPitch), (uint32_t)n);
             v.add(peer_float2(from + HD * 4), peer_float4(from + d * 4), peer_float4(from + d * 4 + 16));
         }
-        const float inverse = v.total == 0.0f ? 0.0f : 1.0f / v.total;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v.sum[e] *= inverse;
-        write8<HD>(a, w.span.first, kv_head, of.column + column, d, v.sum);
+        finish(v, column, d);
     }
     tc::cluster_sync();                                                                     // no CTA leaves while another reads its memory
 }
 
+template <int HD, bool E4M3>
+cudaError_t launch_few_rows(const Kv8AttentionArgs& a, int blocks, int cluster, cudaStream_t stream) {
+    static std::atomic<unsigned long long> allowed{0};
+    constexpr int kBytes = (kRowWarps + 1) * Walk<HD, E4M3, 1>::kPiece * (int)sizeof(float);
+    const cudaError_t e = kv8_allow_smem(allowed, kv8_few_rows_kernel<HD, E4M3>, kBytes);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(blocks * a.cache.heads * a.rows * cluster));
+    cfg.blockDim = dim3(kRowThreads);
+    cfg.dynamicSmemBytes = kBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kv8_few_rows_kernel<HD, E4M3>, a, blocks, cluster);
+}
+
 template <int HD, bool E4M3, int TILES>
 cudaError_t launch_rows(const Kv8AttentionArgs& a, cudaStream_t stream) {
-    constexpr int kPiece = Walk<HD, E4M3, TILES>::kPiece;
-    // segments: as many clusters as are resident at once, and pages of 8 to a warp at most
-    const long long blocks = ((long long)a.most * (a.query_heads / a.cache.heads) + TILES * kTileColumns - 1) / (TILES * kTileColumns);
-    const long long clusters = blocks * a.cache.heads * a.rows;
-    if (!a.prompts && clusters * kClusterCtas <= 148 * rows_residency<HD, TILES>() && a.max_sequence <= kFewTokens) {
-        static std::atomic<unsigned long long> allowed{0};
-        constexpr int kBytes = (kRowWarps + 1) * kPiece * (int)sizeof(float);
-        const cudaError_t e = kv8_allow_smem(allowed, kv8_few_rows_kernel<HD, E4M3, TILES>, kBytes);
-        return e != cudaSuccess ? e : launch_pdl(kv8_few_rows_kernel<HD, E4M3, TILES>, dim3((unsigned)(clusters * kClusterCtas)), dim3(kRowThreads), kBytes, stream,
-                                                 a, (int)blocks);
-    }
     static std::atomic<unsigned long long> allowed{0};
     cudaError_t e = kv8_allow_smem(allowed, kv8_rows_kernel<HD, E4M3, TILES>, (int)rows_smem<HD, TILES>(Q3T_MAX_TABLE_ROWS));
     if (e == cudaSuccess) e = launch_pdl(kv8_zero_tickets_kernel, dim3(1), dim3(kRowCtas), 0, stream, static_cast<unsigned int*>(a.scratch));
@@ -691,9 +722,20 @@ cudaError_t launch_rows(const Kv8AttentionArgs& a, cudaStream_t stream) {
 }
 
 template <int HD, bool E4M3>
-cudaError_t launch_attention(const Kv8AttentionArgs& a, cudaStream_t stream) {
+cudaError_t launch_attention(Kv8AttentionArgs& a, cudaStream_t stream) {
+    const long long columns = (long long)a.most * (a.query_heads / a.cache.heads), blocks = (columns + kTileColumns - 1) / kTileColumns;
+    const long long segments = blocks * a.cache.heads * a.rows;
+    int cluster = kClusterCtas;
+    while (cluster > 1 && (segments * cluster > kFewCtas || a.max_sequence <= kFewest * cluster)) cluster /= 2;
+    a.prompts = 0;
+    a.row_columns = INT_MAX;
+    if (segments * cluster <= kFewCtas && a.max_sequence <= kFewTokens * cluster) return launch_few_rows<HD, E4M3>(a, (int)blocks, cluster, stream);
+    if (columns > kRowColumns && ((long long)a.tokens * a.query_heads >= kPromptColumns || a.max_sequence <= kShort)) {
+        a.prompts = 1;
+        a.row_columns = kRowColumns;
+    }
     // two tiles of columns a warp where rows may have more than one: what a page costs to read and to convert is paid once
-    return (long long)a.most * (a.query_heads / a.cache.heads) > kTileColumns ? launch_rows<HD, E4M3, 2>(a, stream) : launch_rows<HD, E4M3, 1>(a, stream);
+    return columns > kTileColumns ? launch_rows<HD, E4M3, 2>(a, stream) : launch_rows<HD, E4M3, 1>(a, stream);
 }
 
 // false: refused
@@ -762,7 +804,6 @@ extern "C" int32_t q3t_launch_kv8_attention(const Q3tKv8AttentionDesc* desc, voi
     }
     if (a.most == 0) return cudaSuccess;
     a.scratch = desc->scratch;
-    a.prompts = (long long)a.most * (a.query_heads / a.cache.heads) > kKv8RowColumns ? 1 : 0;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool e4m3 = desc->cache->format == Q3T_KV8_E4M3;
     if (desc->cache->head_dimension == 128) return static_cast<int32_t>(e4m3 ? launch_attention<128, true>(a, s) : launch_attention<128, false>(a, s));

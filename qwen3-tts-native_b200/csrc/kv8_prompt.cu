@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         if (row < a.rows) {
             span = row_span(a.starts, a.lengths, row, a.tokens, a.most, a.max_sequence);
             const long long columns = (long long)span.count * group;
-            own = columns > kKv8RowColumns ? (int)((columns + block_columns - 1) / block_columns) * heads : 0;
+            own = columns > a.row_columns ? (int)((columns + block_columns - 1) / block_columns) * heads : 0;
             mine = own;
         }
 #pragma unroll
@@ -413,12 +413,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         if (lane == 0) tc::mbar_arrive(&q_ready);
         // ---- softmax: a thread a row
         const bool real = r < columns;
-        const int seen = real ? seen_by(r) : 0;
+        const int seen = seen_by(min(r, columns - 1));                 // (rows behind the last column: queries of zeros that see what it sees)
         const int unmasked = (int)__reduce_min_sync(0xffffffffu, (unsigned int)seen) / kHalf;      // halves all of which every row of the warp sees
         const uint32_t lanes = tmem + ((uint32_t)(quarter * kWarp) << 16);
         const uint32_t o_at = lanes + kOut + tile * 128;
         const int own = tile < tiles ? halves : 0;
-        float top = real ? -INFINITY : 0.0f, total = 0.0f;
+        float top = -INFINITY, total = 0.0f;
         int settled = 0;                                               // halves that every row of the warp sees all of and has a reference for
         auto rescale_output = [&](float keep, int n) {                 // when the products of the halves before are done
             if (!__all_sync(0xffffffffu, guard.wait(&o_ready[tile][(n - 1) & 1], ((n - 1) >> 1) & 1))) return;
@@ -433,8 +433,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
                 tmem_store_16(o_at + c, bits);
             }
         };
+        const bool idle = r - lane >= columns;                         // no row of the warp is real: what stands for its weights is as good as any
         for (int n = 0; n < own; ++n) {
             if (!__all_sync(0xffffffffu, guard.wait(&s_ready[tile][n & 1], (n >> 1) & 1))) break;
+            if (idle) {
+                if (lane == 0) tc::mbar_arrive(&p_ready[tile][n & 1]);
+                continue;
+            }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t s_at = lanes + tile * kStep + (n & 1) * kHalf;
             // (read together and ahead: beside the copies' stores and the products' operands a load from shared memory takes 300 cycles)
@@ -598,7 +603,7 @@ cudaError_t launch_prompts(const Kv8AttentionArgs& a, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     // as many items as any split of the tokens over the rows can make; of one tile where two would leave SMs idle
     const long long columns = (long long)a.tokens * (a.query_heads / a.cache.heads);
-    const long long rows = columns / (kKv8RowColumns + 1) < a.rows ? columns / (kKv8RowColumns + 1) : a.rows;
+    const long long rows = columns / (a.row_columns + 1) < a.rows ? columns / (a.row_columns + 1) : a.rows;
     const int block_columns = (columns / (2 * kTileRows) + 1) * a.cache.heads <= 148 ? kTileRows : 2 * kTileRows;
     const long long items = (columns / block_columns + rows) * a.cache.heads;
     if (items > 0x7fffffffll) return cudaErrorInvalidValue;
