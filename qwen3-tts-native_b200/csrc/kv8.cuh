@@ -119,6 +119,7 @@ struct Kv8AttentionArgs {
     int tokens, most, max_sequence;
     float scale;
     void* scratch;
+    int scratch_taken;        // bytes of it that are kv8_attention.cu's
     int prompts;              // a launch of kv8_prompt.cu follows
     int row_columns;          // (new tokens x query heads of a KV head) of a row up to which it is not that one's
 };
@@ -143,6 +144,21 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+// 8 dims of the pieces of a column: their sum in terms of the largest reference
+struct Merged {
+    float top = -INFINITY, total = 0.0f, sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    // stats: reference and total of a piece
+    __device__ __forceinline__ void add(const float2& stats, const float4& lo, const float4& hi) {
+        const float most = fmaxf(top, stats.x);
+        const float keep = top == -INFINITY ? 0.0f : exp2_ftz(top - most), f = stats.x == -INFINITY ? 0.0f : exp2_ftz(stats.x - most);
+        const float more[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        top = most;
+        total = fmaf(f, stats.y, total * keep);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] = fmaf(f, more[e], sum[e] * keep);
+    }
+};
+
 // 2^n, -126 <= n <= 127
 __device__ __forceinline__ float power_of_two(int n) { return __uint_as_float((uint32_t)(n + 127) << 23); }
 // A query's way to fp16: times 2^shift its largest value, of which `most` is the bf16 without its sign, lies in 2^7..2^8 (or as near

@@ -24,7 +24,9 @@
 
 namespace q3t {
 
-cudaError_t launch_kv8_prompts(const Kv8AttentionArgs& a, int head_dim, bool e4m3, cudaStream_t stream);      // kv8_prompt.cu
+// kv8_prompt.cu
+size_t kv8_prompt_scratch_bytes(const Kv8AttentionArgs& a, int head_dim);
+cudaError_t launch_kv8_prompts(const Kv8AttentionArgs& a, int head_dim, bool e4m3, cudaStream_t stream);
 
 namespace {
 
@@ -35,7 +37,8 @@ constexpr int kTileColumns = 8;                        // of a product
 constexpr int kStartUnits = 2;                         // what the start of a segment counts for in the cut, in pages
 constexpr int kClusterCtas = 8;                        // the most of a segment
 constexpr int kFewCtas = 256, kFewTokens = 1024, kFewest = 64;
-constexpr int kRowColumns = 32, kPromptColumns = 4096, kShort = 1024;
+constexpr int kRowColumns = 32, kShort = 1024;
+constexpr long long kPromptWork = 1 << 23;
 constexpr int kCounterBytes = (kRowCtas * 4 + 255) / 256 * 256;
 
 __device__ unsigned int g_kv8_range_errors = 0;
@@ -71,21 +74,6 @@ __device__ __forceinline__ float4 peer_float4(uint32_t at) {
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
     return v;
 }
-
-// 8 dims of the pieces of a column: their sum in terms of the largest reference
-struct Merged {
-    float top = -INFINITY, total = 0.0f, sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    // stats: reference and total of a piece
-    __device__ __forceinline__ void add(const float2& stats, const float4& lo, const float4& hi) {
-        const float most = fmaxf(top, stats.x);
-        const float keep = top == -INFINITY ? 0.0f : exp2_ftz(top - most), f = stats.x == -INFINITY ? 0.0f : exp2_ftz(stats.x - most);
-        const float more[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-        top = most;
-        total = fmaf(f, stats.y, total * keep);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum[e] = fmaf(f, more[e], sum[e] * keep);
-    }
-};
 
 // What a row asks of the kernel
 struct RowWork {
@@ -721,21 +709,33 @@ cudaError_t launch_rows(const Kv8AttentionArgs& a, cudaStream_t stream) {
     return e != cudaSuccess || !a.prompts ? e : launch_kv8_prompts(a, HD, E4M3, stream);
 }
 
-template <int HD, bool E4M3>
-cudaError_t launch_attention(Kv8AttentionArgs& a, cudaStream_t stream) {
+// Which kernels a launch takes
+struct Plan {
+    int cluster;       // of kv8_few_rows_kernel; 0: not that one
+    int blocks;        // its blocks of columns
+    int tiles;         // of kv8_rows_kernel
+};
+Plan plan_of(Kv8AttentionArgs& a, int head_dim) {
     const long long columns = (long long)a.most * (a.query_heads / a.cache.heads), blocks = (columns + kTileColumns - 1) / kTileColumns;
     const long long segments = blocks * a.cache.heads * a.rows;
     int cluster = kClusterCtas;
     while (cluster > 1 && (segments * cluster > kFewCtas || a.max_sequence <= kFewest * cluster)) cluster /= 2;
     a.prompts = 0;
     a.row_columns = INT_MAX;
-    if (segments * cluster <= kFewCtas && a.max_sequence <= kFewTokens * cluster) return launch_few_rows<HD, E4M3>(a, (int)blocks, cluster, stream);
-    if (columns > kRowColumns && ((long long)a.tokens * a.query_heads >= kPromptColumns || a.max_sequence <= kShort)) {
+    a.scratch_taken = kCounterBytes + kRowCtas * 2 * 2 * kTileColumns * (head_dim + 4) * (int)sizeof(float);
+    if (segments * cluster <= kFewCtas && a.max_sequence <= kFewTokens * cluster) return Plan{cluster, (int)blocks, 0};
+    if (columns > kRowColumns && ((long long)a.tokens * a.query_heads * a.max_sequence >= kPromptWork || a.max_sequence <= kShort)) {
         a.prompts = 1;
         a.row_columns = kRowColumns;
     }
     // two tiles of columns a warp where rows may have more than one: what a page costs to read and to convert is paid once
-    return columns > kTileColumns ? launch_rows<HD, E4M3, 2>(a, stream) : launch_rows<HD, E4M3, 1>(a, stream);
+    return Plan{0, 0, columns > kTileColumns ? 2 : 1};
+}
+
+template <int HD, bool E4M3>
+cudaError_t launch_attention(const Kv8AttentionArgs& a, const Plan& plan, cudaStream_t stream) {
+    if (plan.cluster > 0) return launch_few_rows<HD, E4M3>(a, plan.blocks, plan.cluster, stream);
+    return plan.tiles == 2 ? launch_rows<HD, E4M3, 2>(a, stream) : launch_rows<HD, E4M3, 1>(a, stream);
 }
 
 // false: refused
@@ -792,7 +792,8 @@ extern "C" uint32_t q3t_kv8_page_error_count(void) {
 extern "C" size_t q3t_kv8_attention_scratch_bytes(const Q3tKv8AttentionDesc* desc) {
     q3t::Kv8AttentionArgs a;
     if (!q3t::attention_args(desc, &a)) return 0;
-    return q3t::kCounterBytes + (size_t)q3t::kRowCtas * 2 * 2 * q3t::kTileColumns * (desc->cache->head_dimension + 4) * sizeof(float);
+    q3t::plan_of(a, desc->cache->head_dimension);
+    return a.scratch_taken + (a.prompts ? q3t::kv8_prompt_scratch_bytes(a, desc->cache->head_dimension) : 0);
 }
 
 extern "C" int32_t q3t_launch_kv8_attention(const Q3tKv8AttentionDesc* desc, void* stream) {
@@ -804,8 +805,11 @@ extern "C" int32_t q3t_launch_kv8_attention(const Q3tKv8AttentionDesc* desc, voi
     }
     if (a.most == 0) return cudaSuccess;
     a.scratch = desc->scratch;
+    const Plan plan = plan_of(a, desc->cache->head_dimension);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool e4m3 = desc->cache->format == Q3T_KV8_E4M3;
-    if (desc->cache->head_dimension == 128) return static_cast<int32_t>(e4m3 ? launch_attention<128, true>(a, s) : launch_attention<128, false>(a, s));
-    return static_cast<int32_t>(e4m3 ? launch_attention<64, true>(a, s) : launch_attention<64, false>(a, s));
+    if (desc->cache->head_dimension == 128) {
+        return static_cast<int32_t>(e4m3 ? launch_attention<128, true>(a, plan, s) : launch_attention<128, false>(a, plan, s));
+    }
+    return static_cast<int32_t>(e4m3 ? launch_attention<64, true>(a, plan, s) : launch_attention<64, false>(a, plan, s));
 }

@@ -29,6 +29,7 @@ constexpr int kLaunchRegisters = 96, kSoftmaxRegisters = 144, kCopyRegisters = 7
 static_assert(2 * kSoftmaxRegisters + 2 * kCopyRegisters + kProductRegisters <= 5 * kLaunchRegisters, "registers of the five warpgroups");
 constexpr int kScaleRing = 4;                           // steps whose scales are kept: K runs two steps ahead of the softmax
 constexpr uint32_t kTmemCols = 512, kOut = 256;         // scores of the tiles at 0 and 128, outputs at 256 and 384
+constexpr int kPartTokens = 1024;                       // what a row sees is cut into parts of so many and more
 constexpr float kMostWeight = 32768.0f;                 // of a page's weights together
 constexpr long long kBudgetCycles = 4000000000ll;        // about two seconds
 
@@ -60,8 +61,29 @@ struct Guard {
 };
 
 struct Item {
-    int row, kv_head, block;
+    int row, kv_head, block, part;
     RowSpan span;
+};
+
+// How a launch is cut: blocks of 128 or 256 columns, and what they see into so many parts at most
+struct PromptCut {
+    int block_columns, parts;
+    long long items;
+};
+
+// What an item's parts leave is 16 bytes of each row for 4 dims at a time, then the rows' references and sums; kv8_join_kernel learns from
+// the first part what there is to join
+struct Joint {
+    int parts;         // fewer than two: nothing
+    int columns, column0;
+    int kv_head, first;
+    int unused[3];
+};
+constexpr int kMostParts = 8;
+constexpr int kJointBytes = 148 * (int)sizeof(Joint);
+template <int HD>
+struct Part {
+    static constexpr size_t kFloats = (size_t)2 * kTileRows * (HD + 2);
 };
 
 // 16-byte piece `piece` of row `t` of a tile of 128: 64 dims in 128 bytes, swizzled, the next 64 a tile of rows further on
@@ -120,8 +142,10 @@ __device__ __forceinline__ void tmem_store_16(uint32_t taddr, const uint32_t (&r
         : "memory");
 }
 
-template <int HD, bool E4M3>
-__global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8AttentionArgs a, const int block_columns) {
+// PARTS: items may come in parts (without: two divisions and a branch an item fewer, 1.3 us of a prompt of 1,500 tokens)
+template <int HD, bool E4M3, bool PARTS>
+__global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8AttentionArgs a, const int block_columns, const int parts_asked, unsigned char* const left) {
+    const int most_parts = PARTS ? parts_asked : 1;
     using Smem = PromptSmem<HD>;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* const smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -152,7 +176,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         if (row < a.rows) {
             span = row_span(a.starts, a.lengths, row, a.tokens, a.most, a.max_sequence);
             const long long columns = (long long)span.count * group;
-            own = columns > a.row_columns ? (int)((columns + block_columns - 1) / block_columns) * heads : 0;
+            own = columns > a.row_columns ? (int)((columns + block_columns - 1) / block_columns) * heads * most_parts : 0;
             mine = own;
         }
 #pragma unroll
@@ -164,12 +188,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         __syncthreads();
         for (int w = 0; w < warp; ++w) mine += warp_items[w];
         const int to = sum + mine, from = to - own, at = (int)blockIdx.x;
-        if (at >= from && at < to) found = Item{row, (at - from) % heads, own / heads - 1 - (at - from) / heads, span};
+        if (at >= from && at < to) {
+            const int number = (at - from) / most_parts;
+            found = Item{row, number % heads, own / most_parts / heads - 1 - number / heads, (at - from) % most_parts, span};
+        }
         for (int w = 0; w < kPromptThreads / kWarp; ++w) sum += warp_items[w];
         __syncthreads();
     }
     const Item item = found;
+    Joint* const joint = reinterpret_cast<Joint*>(left) + (int)blockIdx.x / most_parts;
     if (item.row < 0) {                                                // (a grid is as large as tokens and rows may need)
+        if (most_parts > 1 && tid == 0 && (int)blockIdx.x % most_parts == 0) joint->parts = 0;
         pdl_wait();                                                    // what follows relies on this launch to be behind the one before
         return;
     }
@@ -190,7 +219,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
     };
     // (both tiles go as far as the second one's last column sees; one that is empty not at all)
     const int tiles = columns > kTileRows ? 2 : 1;
-    const int halves = (seen_by(columns - 1) + kHalf - 1) / kHalf, steps = (halves + 1) / 2;
+    const int all_halves = (seen_by(columns - 1) + kHalf - 1) / kHalf, all_steps = (all_halves + 1) / 2, parts = PARTS ? max(1, min(most_parts, all_steps)) : 1;
+    if (most_parts > 1 && tid == 0 && item.part == 0) *joint = Joint{parts, columns, column0, item.kv_head, item.span.first, {0, 0, 0}};
+    if (item.part >= parts) {
+        pdl_wait();
+        return;
+    }
+    // this part's steps; what follows counts them from 0
+    const int step0 = all_steps * item.part / parts, steps = all_steps * (item.part + 1) / parts - step0;
+    const int halves = min(2 * steps, all_halves - 2 * step0);
 
     Guard guard;
     guard.deadline = clock64() + kBudgetCycles;
@@ -234,6 +271,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         unsigned char* const buffers = is_value ? values : keys;
         uint64_t* const empty = is_value ? empty_v : empty_k;
         const int last = min(max(item.span.base + item.span.count, 0), a.max_sequence);        // what lies behind may read as NaN
+        const int page0 = step0 * kStepPages;
         const bool last_block = column0 + block_columns >= item.span.count * group;
         const int* const ids_at = a.table + (size_t)item.row * a.table_stride;
         int ids = -1;                                                  // of 32 pages, a lane each
@@ -241,10 +279,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         uint32_t good = 0u;                                            // pages of the step that are there
         auto request = [&](int step) {
             if (step % (kWarp / kStepPages) == 0) {
-                const int page = step * kStepPages + lane;
+                const int page = page0 + step * kStepPages + lane;
                 ids = page * kPageTokens < last ? ids_at[page] : -1;
                 if (ids < 0 || ids >= a.cache.pages) {
-                    if (page * kPageTokens < last && page < steps * kStepPages && t < kWarp && !is_value && item.kv_head == 0 && last_block) {
+                    if (page * kPageTokens < last && page < page0 + steps * kStepPages && t < kWarp && !is_value && item.kv_head == 0 && last_block) {
                         atomicAdd(&g_kv8_prompt_page_errors, 1u);
                     }
                     ids = -1;
@@ -255,7 +293,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
             for (int p = 0; p < kStepPages; ++p) {
                 const int id = __shfl_sync(0xffffffffu, ids, step % (kWarp / kStepPages) * kStepPages + p);
                 code[p] = make_int4(0, 0, 0, 0);
-                if (id >= 0 && (step * kStepPages + p) * kPageTokens + token < last) {
+                if (id >= 0 && (page0 + step * kStepPages + p) * kPageTokens + token < last) {
                     const uint8_t* const from = plane + (long long)id * a.cache.page_stride;
                     if (kCodes == 16) {
                         asm volatile("ld.global.L1::no_allocate.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(code[p].x), "=r"(code[p].y), "=r"(code[p].z), "=r"(code[p].w) : "l"(from));
@@ -413,7 +451,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         if (lane == 0) tc::mbar_arrive(&q_ready);
         // ---- softmax: a thread a row
         const bool real = r < columns;
-        const int seen = seen_by(min(r, columns - 1));                 // (rows behind the last column: queries of zeros that see what it sees)
+        const int seen = max(seen_by(min(r, columns - 1)) - step0 * kStep, 0);                 // (rows behind the last column: queries of zeros that see what it sees)
         const int unmasked = (int)__reduce_min_sync(0xffffffffu, (unsigned int)seen) / kHalf;      // halves all of which every row of the warp sees
         const uint32_t lanes = tmem + ((uint32_t)(quarter * kWarp) << 16);
         const uint32_t o_at = lanes + kOut + tile * 128;
@@ -434,12 +472,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
             }
         };
         const bool idle = r - lane >= columns;                         // no row of the warp is real: what stands for its weights is as good as any
-        for (int n = 0; n < own; ++n) {
+        for (int n = 0; idle && n < own; ++n) {
             if (!__all_sync(0xffffffffu, guard.wait(&s_ready[tile][n & 1], (n >> 1) & 1))) break;
-            if (idle) {
-                if (lane == 0) tc::mbar_arrive(&p_ready[tile][n & 1]);
-                continue;
-            }
+            if (lane == 0) tc::mbar_arrive(&p_ready[tile][n & 1]);
+        }
+        for (int n = idle ? own : 0; n < own; ++n) {
+            if (!__all_sync(0xffffffffu, guard.wait(&s_ready[tile][n & 1], (n >> 1) & 1))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t s_at = lanes + tile * kStep + (n & 1) * kHalf;
             // (read together and ahead: beside the copies' stores and the products' operands a load from shared memory takes 300 cycles)
@@ -538,7 +576,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         if (own > 0) guard.wait(&o_ready[tile][(own - 1) & 1], ((own - 1) >> 1) & 1);
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+        const float inverse = parts > 1 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
+        float* const part_at = reinterpret_cast<float*>(left + kJointBytes) + (size_t)blockIdx.x * Part<HD>::kFloats;
+        if (parts > 1 && real) *reinterpret_cast<float2*>(part_at + 2 * kTileRows * HD + 2 * r) = make_float2(top, total);
         int head;
         const size_t token = item.span.first + place_of(min(r, columns - 1), head), at = (size_t)(item.kv_head * group + head) * HD;
 #pragma unroll 1
@@ -557,6 +597,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
                 float v[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = own > 0 ? __uint_as_float(o[j >> 5][(j & 31) + e]) * inverse : 0.0f;
+                if (parts > 1) {
+                    float4* const to = reinterpret_cast<float4*>(part_at) + (c + j) / 4 * (2 * kTileRows) + r;
+                    to[0] = make_float4(v[0], v[1], v[2], v[3]);
+                    to[2 * kTileRows] = make_float4(v[4], v[5], v[6], v[7]);
+                    continue;
+                }
                 __nv_bfloat162 x[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[e] = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
@@ -588,29 +634,94 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
     pdl_trigger();
 }
 
-template <int HD, bool E4M3>
-cudaError_t launch_prompts(const Kv8AttentionArgs& a, cudaStream_t stream) {
+// An item's parts, one after the other: a CTA 32 of its rows, a warp 8 dims of them at a time
+template <int HD>
+__global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8AttentionArgs a, const int most_parts, const unsigned char* const left) {
+    pdl_wait();
+    pdl_trigger();
+    const int item = (int)blockIdx.x / (2 * kTileRows / kWarp), r = (int)blockIdx.x % (2 * kTileRows / kWarp) * kWarp + (int)threadIdx.x % kWarp;
+    const Joint joint = reinterpret_cast<const Joint*>(left)[item];
+    if (joint.parts < 2 || r >= joint.columns) return;
+    const float* const from = reinterpret_cast<const float*>(left + kJointBytes) + (size_t)item * most_parts * Part<HD>::kFloats;
+    const int group = a.query_heads / a.cache.heads, i = (joint.column0 + r) / group;
+    const size_t token = joint.first + i, at = (size_t)(joint.kv_head * group + joint.column0 + r - i * group) * HD;
+    for (int d = (int)threadIdx.x / kWarp * 8; d < HD; d += 64) {
+        Merged v;
+#pragma unroll 4
+        for (int n = 0; n < joint.parts; ++n) {
+            const float* const part = from + n * Part<HD>::kFloats;
+            const float4* const o = reinterpret_cast<const float4*>(part) + d / 4 * (2 * kTileRows) + r;
+            v.add(*reinterpret_cast<const float2*>(part + 2 * kTileRows * HD + 2 * r), o[0], o[2 * kTileRows]);
+        }
+        const float inverse = v.total == 0.0f ? 0.0f : 1.0f / v.total;
+        __nv_bfloat162 x[4];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v.sum[e] *= inverse;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = __floats2bfloat162_rn(v.sum[2 * e], v.sum[2 * e + 1]);
+        *reinterpret_cast<int4*>(a.out + token * a.out_stride + at + d) = *reinterpret_cast<const int4*>(x);
+        if (a.out32 != nullptr) {
+            float* const to = a.out32 + token * a.query_heads * HD + at + d;
+            *reinterpret_cast<float4*>(to) = make_float4(v.sum[0], v.sum[1], v.sum[2], v.sum[3]);
+            *reinterpret_cast<float4*>(to + 4) = make_float4(v.sum[4], v.sum[5], v.sum[6], v.sum[7]);
+        }
+    }
+}
+
+// Blocks of 128 columns where 256 would leave SMs idle, and where those are so few that each could have several SMs, parts
+PromptCut prompt_cut(const Kv8AttentionArgs& a) {
+    // as many items as any split of the tokens over the rows can make
+    const long long columns = (long long)a.tokens * (a.query_heads / a.cache.heads);
+    const long long rows = columns / (a.row_columns + 1) < a.rows ? columns / (a.row_columns + 1) : a.rows;
+    auto items = [&](int block) {
+        return (a.rows == 1 ? (columns + block - 1) / block : columns / block + rows) * a.cache.heads;
+    };
+    PromptCut cut{2 * kTileRows, 1, items(2 * kTileRows)};
+    if (cut.items >= 1 && cut.items <= 148 / 2) {
+        const long long parts = 148 / cut.items, most = a.max_sequence / kPartTokens;
+        cut.parts = (int)(parts < kMostParts ? parts : kMostParts);
+        if (cut.parts > most) cut.parts = (int)most;
+    }
+    if (cut.parts < 2) {
+        cut.parts = 1;
+        if ((columns / (2 * kTileRows) + 1) * a.cache.heads <= 148) cut = PromptCut{kTileRows, 1, items(kTileRows)};
+    }
+    return cut;
+}
+
+template <int HD, bool E4M3, bool PARTS>
+cudaError_t launch_cut(const Kv8AttentionArgs& a, const PromptCut& cut, unsigned char* left, cudaStream_t stream) {
     static std::atomic<unsigned long long> allowed{0};
     static std::atomic<bool> looked{false};
     if (!looked.load(std::memory_order_acquire)) {
         cudaFuncAttributes built;
-        const cudaError_t e = cudaFuncGetAttributes(&built, kv8_prompt_kernel<HD, E4M3>);
+        const cudaError_t e = cudaFuncGetAttributes(&built, kv8_prompt_kernel<HD, E4M3, PARTS>);
         if (e != cudaSuccess) return e;
         if (built.numRegs < kLaunchRegisters) return cudaErrorInvalidConfiguration;     // what setmaxnreg hands out has to be there
         looked.store(true, std::memory_order_release);
     }
-    const cudaError_t e = kv8_allow_smem(allowed, kv8_prompt_kernel<HD, E4M3>, (int)PromptSmem<HD>::kBytes);
+    const cudaError_t e = kv8_allow_smem(allowed, kv8_prompt_kernel<HD, E4M3, PARTS>, (int)PromptSmem<HD>::kBytes);
     if (e != cudaSuccess) return e;
-    // as many items as any split of the tokens over the rows can make; of one tile where two would leave SMs idle
-    const long long columns = (long long)a.tokens * (a.query_heads / a.cache.heads);
-    const long long rows = columns / (a.row_columns + 1) < a.rows ? columns / (a.row_columns + 1) : a.rows;
-    const int block_columns = (columns / (2 * kTileRows) + 1) * a.cache.heads <= 148 ? kTileRows : 2 * kTileRows;
-    const long long items = (columns / block_columns + rows) * a.cache.heads;
-    if (items > 0x7fffffffll) return cudaErrorInvalidValue;
-    return launch_pdl(kv8_prompt_kernel<HD, E4M3>, dim3((unsigned)(items > 0 ? items : 1)), dim3(kPromptThreads), PromptSmem<HD>::kBytes, stream, a, block_columns);
+    const unsigned grid = (unsigned)(cut.items > 0 ? cut.items * cut.parts : 1);
+    return launch_pdl(kv8_prompt_kernel<HD, E4M3, PARTS>, dim3(grid), dim3(kPromptThreads), PromptSmem<HD>::kBytes, stream, a, cut.block_columns, cut.parts, left);
+}
+
+template <int HD, bool E4M3>
+cudaError_t launch_prompts(const Kv8AttentionArgs& a, cudaStream_t stream) {
+    const PromptCut cut = prompt_cut(a);
+    if (cut.items > 0x7fffffffll) return cudaErrorInvalidValue;
+    unsigned char* const left = static_cast<unsigned char*>(a.scratch) + a.scratch_taken;
+    if (cut.parts < 2) return launch_cut<HD, E4M3, false>(a, cut, left, stream);
+    const cudaError_t e = launch_cut<HD, E4M3, true>(a, cut, left, stream);
+    return e != cudaSuccess ? e : launch_pdl(kv8_join_kernel<HD>, dim3((unsigned)cut.items * (2 * kTileRows / kWarp)), dim3(256), 0, stream, a, cut.parts, left);
 }
 
 }  // namespace
+
+size_t kv8_prompt_scratch_bytes(const Kv8AttentionArgs& a, int head_dim) {
+    const PromptCut cut = prompt_cut(a);
+    return cut.parts < 2 ? 0 : kJointBytes + (size_t)cut.items * cut.parts * (head_dim == 128 ? Part<128>::kFloats : Part<64>::kFloats) * sizeof(float);
+}
 
 cudaError_t launch_kv8_prompts(const Kv8AttentionArgs& a, int head_dim, bool e4m3, cudaStream_t stream) {
     if (head_dim == 128) return e4m3 ? launch_prompts<128, true>(a, stream) : launch_prompts<128, false>(a, stream);
