@@ -7,9 +7,11 @@
 // through memory to be taken in the same launch, and nothing is serial in the rows.
 //
 // What bounds it: latency (lengths, sums, table entries: three loads one behind the other) and, with long prompts, the 12 bytes
-// a new token that are written.  Few tokens are one CTA's.  More are filled in by as many CTAs as they need, each of which repeats the
-// sums, and a second launch writes lengths, states and the free count, which may lie over what the first one reads; it has its sums
-// by the time the first is done.
+// a new token that are written.  A step of a token a row is one CTA's.  Others are filled in by a CTA for each 32 rows or 2,048 tokens, each of
+// which repeats the sums, and a second launch writes lengths, states and the free count, which may lie over what the first one
+// reads; it has its sums by the time the first is done.  One launch / two, in us: a token a row 3.2 / 3.8 (64 rows), 4.3 / 4.7 (512), 6.3 / 5.5
+// (1,000); every eighth row with a prompt of up to 8 tokens and every sixteenth giving all pages back 7.0 / 6.5 (64), 13.2 / 8.7 (1,000); prompts of
+// up to 1,500 for 113,000 tokens 69.6 / 8.7 (1.4 MB written, 0.3 us of memory).
 
 #include "kv8.cuh"
 #include "q3t_kernels.cuh"
@@ -23,7 +25,8 @@ constexpr int kMostThreads = 1024;
 constexpr int kFillThreads = 512;              // of the CTAs that only fill in
 constexpr int kChunk = 128;                    // tokens, or pages given back, that a warp takes at a time
 constexpr int kFew = 8;                        // tokens of a row that a thread fills in
-constexpr int kOneCtaTokens = kMostThreads / kWarp * kChunk;
+constexpr int kOneCtaRows = 512;
+constexpr int kCtaTokens = kFillThreads / kWarp * kChunk, kCtaRows = 32;      // of a CTA that fills in
 constexpr int kFill = 1, kSettle = 2;          // what a launch writes: tables, stack and tokens; lengths, states, starts and the free count
 
 struct TableArgs {
@@ -283,13 +286,9 @@ extern "C" int32_t q3t_launch_page_tables(const Q3tPageTablesDesc* d, void* stre
     a.rows = d->rows; a.stride = d->page_table_stride; a.pages = d->pages; a.capacity = d->token_capacity;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int rows_up = (d->rows + kWarp - 1) / kWarp * kWarp;
-    if (d->token_capacity <= kOneCtaTokens) {
-        const int tokens_up = (d->token_capacity + kChunk - 1) / kChunk * kWarp;
-        const int threads = rows_up > tokens_up ? rows_up : tokens_up;
-        return static_cast<int32_t>(launch_tables<kFill | kSettle>(a, 1, threads < kMostThreads ? threads : kMostThreads, s));
-    }
-    constexpr int kCtaTokens = kFillThreads / kWarp * kChunk;
-    const int ctas = (d->token_capacity - 1) / kCtaTokens + 1;
+    if (d->token_capacity <= d->rows && d->rows <= kOneCtaRows) return static_cast<int32_t>(launch_tables<kFill | kSettle>(a, 1, rows_up, s));
+    const int for_tokens = d->token_capacity / kCtaTokens + 1, for_rows = (d->rows + kCtaRows - 1) / kCtaRows;
+    const int ctas = for_tokens > for_rows ? for_tokens : for_rows;
     const cudaError_t e = launch_tables<kFill>(a, ctas < 148 ? ctas : 148, kFillThreads, s);
     return static_cast<int32_t>(e != cudaSuccess ? e : launch_tables<kSettle>(a, 1, rows_up < kMostThreads ? rows_up : kMostThreads, s));
 }
