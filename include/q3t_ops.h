@@ -457,7 +457,8 @@ typedef struct Q3tKv8AttentionDesc {
     void* scratch;               /* 16-byte aligned; launches that share it must be ordered */
     size_t scratch_bytes;
 } Q3tKv8AttentionDesc;
-QWEN3_TTS_API size_t q3t_kv8_attention_scratch_bytes(const Q3tKv8AttentionDesc* desc);      /* 0: arguments that are refused */
+/* Enough also for launches of fewer rows, tokens, tokens a row or shorter sequences.  0: arguments that are refused */
+QWEN3_TTS_API size_t q3t_kv8_attention_scratch_bytes(const Q3tKv8AttentionDesc* desc);
 QWEN3_TTS_API int32_t q3t_launch_kv8_attention(const Q3tKv8AttentionDesc* desc, void* stream);
 QWEN3_TTS_API uint32_t q3t_kv8_nonfinite_count(void);
 QWEN3_TTS_API uint32_t q3t_kv8_page_error_count(void);

@@ -24,8 +24,8 @@
 
 namespace q3t {
 
-// kv8_prompt.cu
-size_t kv8_prompt_scratch_bytes(const Kv8AttentionArgs& a, int head_dim);
+// kv8_prompt.cu.  As much as any launch of rows no longer may need
+size_t kv8_prompt_scratch_bytes(int max_sequence, int head_dim);
 cudaError_t launch_kv8_prompts(const Kv8AttentionArgs& a, int head_dim, bool e4m3, cudaStream_t stream);
 
 namespace {
@@ -793,7 +793,7 @@ extern "C" size_t q3t_kv8_attention_scratch_bytes(const Q3tKv8AttentionDesc* des
     q3t::Kv8AttentionArgs a;
     if (!q3t::attention_args(desc, &a)) return 0;
     q3t::plan_of(a, desc->cache->head_dimension);
-    return a.scratch_taken + (a.prompts ? q3t::kv8_prompt_scratch_bytes(a, desc->cache->head_dimension) : 0);
+    return a.scratch_taken + (a.prompts ? q3t::kv8_prompt_scratch_bytes(a.max_sequence, desc->cache->head_dimension) : 0);
 }
 
 extern "C" int32_t q3t_launch_kv8_attention(const Q3tKv8AttentionDesc* desc, void* stream) {

@@ -718,9 +718,8 @@ cudaError_t launch_prompts(const Kv8AttentionArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
-size_t kv8_prompt_scratch_bytes(const Kv8AttentionArgs& a, int head_dim) {
-    const PromptCut cut = prompt_cut(a);
-    return cut.parts < 2 ? 0 : kJointBytes + (size_t)cut.items * cut.parts * (head_dim == 128 ? Part<128>::kFloats : Part<64>::kFloats) * sizeof(float);
+size_t kv8_prompt_scratch_bytes(int max_sequence, int head_dim) {
+    return max_sequence < 2 * kPartTokens ? 0 : kJointBytes + 148 * (head_dim == 128 ? Part<128>::kFloats : Part<64>::kFloats) * sizeof(float);
 }
 
 cudaError_t launch_kv8_prompts(const Kv8AttentionArgs& a, int head_dim, bool e4m3, cudaStream_t stream) {

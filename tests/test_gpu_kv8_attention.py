@@ -1,5 +1,9 @@
 """Attention over an 8-bit paged cache (q3t_launch_kv8_attention) against the formula in 64 bits (tests/kv8_oracle.py, which derives the
-tolerance).  The bf16 output may be half a bf16 step further off: 2^-9 of the next power of two, 2^-8 of the value at most."""
+tolerance).  The bf16 output may be half a bf16 step further off: 2^-9 of the next power of two, 2^-8 of the value at most.
+
+Which kernel takes a row depends on the bounds that the host gives, so most tests run with page tables of several widths: as wide as
+the rows need (a CTA or a cluster a segment, prompts in one part), FEW_TOKENS pages (ranges of pages for every warp) and LONG pages
+(prompts of many tokens in parts)."""
 import ctypes as C
 
 import numpy as np
@@ -8,6 +12,8 @@ import pytest
 import kv8_oracle as plain
 
 pytestmark = pytest.mark.gpu
+FEW_TOKENS, LONG = 520, 70000
+ROOMS = pytest.mark.parametrize("room", [None, FEW_TOKENS, LONG])
 
 
 def _query(rng, count, heads, dim, size=1.0):
@@ -28,7 +34,7 @@ def _run(ops, rng, heads, dim, group, lengths, new, e4m3, **more):
     spread = more.pop("spread", 0.5)
     size = more.pop("size", 1.0)
     planes = plain.cache(rng, pages, heads, dim, e4m3, spread)
-    table = plain.tables_of(rng, lengths, pages)
+    table = plain.tables_of(rng, lengths, pages, more.pop("room", None))
     starts = None if new is None else np.concatenate([[0], np.cumsum(new)])
     count = len(lengths) if new is None else int(starts[-1])
     q = _query(rng, count, heads * group, dim, size)
@@ -40,45 +46,123 @@ def _run(ops, rng, heads, dim, group, lengths, new, e4m3, **more):
 @pytest.mark.parametrize("e4m3", [False, True])
 @pytest.mark.parametrize("dim", [128, 64])
 @pytest.mark.parametrize("heads,group", [(8, 2), (1, 1), (2, 4), (1, 8), (2, 7), (1, 16), (1, 33)])
-def test_single_tokens(ops, e4m3, dim, heads, group):
+@pytest.mark.parametrize("room", [None, FEW_TOKENS])
+def test_single_tokens(ops, e4m3, dim, heads, group, room):
     rng = np.random.default_rng(heads * 100 + group)
-    _run(ops, rng, heads, dim, group, [1, 15, 16, 17, 300, 128, 129, 1025, 0], None, e4m3)
+    _run(ops, rng, heads, dim, group, [1, 15, 16, 17, 300, 128, 129, 1025, 0], None, e4m3, room=room)
 
 
 @pytest.mark.parametrize("e4m3", [False, True])
 @pytest.mark.parametrize("length", [1, 127, 2048, 2049, 5000, 40000])
-def test_one_row_of_any_length(ops, e4m3, length):
-    _run(ops, np.random.default_rng(length), 2, 128, 2, [length], None, e4m3)
+@pytest.mark.parametrize("room", [None, 2600])
+def test_one_row_of_any_length(ops, e4m3, length, room):
+    _run(ops, np.random.default_rng(length), 2, 128, 2, [length], None, e4m3, room=room)
 
 
 @pytest.mark.parametrize("rows", [2, 64, 300, 1500])
-def test_many_rows(ops, rows):
+@pytest.mark.parametrize("room", [None, FEW_TOKENS])
+def test_many_rows(ops, rows, room):
     rng = np.random.default_rng(rows)
-    _run(ops, rng, 1, 64, 2, [int(n) for n in rng.integers(0, 200, rows)], None, rows % 4 == 0)
+    _run(ops, rng, 1, 64, 2, [int(n) for n in rng.integers(0, 200, rows)], None, rows % 4 == 0, room=room)
 
 
 @pytest.mark.parametrize("e4m3", [False, True])
-@pytest.mark.parametrize("heads,dim,group", [(2, 128, 2), (1, 64, 4), (2, 64, 1), (1, 128, 5)])
-@pytest.mark.parametrize("lengths,new", [([5, 100, 33], [5, 5, 5]), ([700, 20, 0, 9], [1, 17, 0, 9]), ([64, 300], [64, 3]), ([2, 40], [4, 40])])
-def test_ragged_new_tokens(ops, e4m3, heads, dim, group, lengths, new):
-    """Drafts, prompts, rows without new tokens, and one that is shorter than its new tokens (its first ones get zeros)."""
-    _run(ops, np.random.default_rng(sum(lengths) + group), heads, dim, group, lengths, new, e4m3)
+@pytest.mark.parametrize("heads,dim,group,rows,longest,new", [
+    (1, 128, 2, 4, 5000, None), (2, 64, 1, 16, 7000, None), (8, 128, 1, 8, 4096, None), (8, 128, 2, 16, 2000, None), (4, 64, 8, 60, 900, None),
+    (2, 128, 4, 4, 3000, [3, 1, 9, 0]), (8, 64, 2, 3, 1500, [30, 4, 11])])
+def test_clusters_of_every_size(ops, e4m3, heads, dim, group, rows, longest, new):
+    """8, 8, 4, 2 and 1 CTAs a segment, with blocks that some rows do not have; among the rows one of nothing and one of one page."""
+    rng = np.random.default_rng(rows + longest)
+    lengths = [int(n) for n in rng.integers(20, longest + 1, rows)]
+    lengths[0] = longest
+    if new is None:
+        lengths[1:3] = [0, 9]
+    _run(ops, rng, heads, dim, group, lengths, new, e4m3)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("heads,dim,group,lengths,new", [(8, 128, 2, [2100], [64]), (8, 64, 1, [1200, 90, 1500], [40, 60, 9]), (1, 128, 16, [9000, 40], [20, 7])])
+def test_rows_of_many_columns_over_a_long_context(ops, e4m3, heads, dim, group, lengths, new):
+    """Too few tokens to fill the SMs with prompts' blocks: the ranges of the short rows' kernel, several blocks of columns a row."""
+    _run(ops, np.random.default_rng(sum(lengths)), heads, dim, group, lengths, new, e4m3)
 
 
 @pytest.mark.parametrize("e4m3", [False, True])
 @pytest.mark.parametrize("heads,dim,group,lengths,new", [
-    (2, 128, 2, [200], [200]), (1, 128, 2, [129, 400], [129, 130]), (1, 64, 4, [257], [257]), (1, 128, 8, [700], [90]), (1, 64, 1, [600, 1, 350], [300, 1, 129]),
-    (1, 128, 3, [301], [170]), (1, 128, 16, [130], [67])])
-def test_prompts_and_chunks(ops, e4m3, heads, dim, group, lengths, new):
-    _run(ops, np.random.default_rng(sum(lengths) + group), heads, dim, group, lengths, new, e4m3)
+    (1, 128, 16, [3000], [200]), (2, 64, 2, [8200], [260]), (1, 64, 4, [8200, 130, 40, 20], [230, 120, 40, 60]), (1, 128, 8, [5000, 0, 4097], [33, 0, 190])])
+def test_prompts_in_parts(ops, e4m3, heads, dim, group, lengths, new):
+    """Two to eight parts of a long context; rows of fewer steps than parts and one that is shorter than its new tokens."""
+    _run(ops, np.random.default_rng(sum(lengths) + 1), heads, dim, group, lengths, new, e4m3)
+
+
+@pytest.mark.parametrize("heads,group,lengths,new", [(64, 1, [300], [300]), (64, 1, [310, 300], [300, 300])])
+def test_more_prompt_blocks_than_sms(ops, heads, group, lengths, new):
+    """Blocks of 128 columns and of 256."""
+    _run(ops, np.random.default_rng(len(new)), heads, 64, group, lengths, new, len(new) == 1)
+
+
+@pytest.mark.parametrize("heads,lengths,new,room", [(2, [700, 500], None, None), (2, [700, 500], None, FEW_TOKENS), (2, [900], [200], LONG), (8, [900], [200], None)])
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_scores_that_grow_along_the_context(ops, heads, lengths, new, room, e4m3):
+    """Keys a fifth larger from page to page: references are outgrown again and again, late ones by far."""
+    rng = np.random.default_rng(79)
+    planes = plain.cache(rng, 120, heads, 128, e4m3)
+    table = plain.tables_of(rng, lengths, 120, room)
+    for r, n in enumerate(lengths):
+        ids = table[r, :-(-n // 16)]
+        planes[2][ids] *= (1.2 ** np.arange(len(ids)) * 0.02).astype(np.float32)[:, None]
+    starts = None if new is None else np.concatenate([[0], np.cumsum(new)])
+    q = _query(rng, len(lengths) if new is None else sum(new), heads * 2, 128)
+    out, f32 = ops.kv8_attention(q, *planes, table, lengths, starts, e4m3=e4m3, want_f32=True)
+    want, tol = plain.attention(q, planes, table, lengths, starts, e4m3)
+    _compare(out, f32, want, tol)
+
+
+@pytest.mark.parametrize("heads,lengths,new,room", [(2, [300, 200], None, None), (2, [300, 200], None, FEW_TOKENS), (2, [300], [150], LONG), (8, [300], [150], None)])
+@pytest.mark.parametrize("value", [0x7f80, 0xffc0])
+def test_queries_that_are_not_finite_stay_in_their_rows(ops, heads, lengths, new, room, value):
+    rng = np.random.default_rng(83)
+    planes = plain.cache(rng, 40, heads, 128, False)
+    table = plain.tables_of(rng, lengths, 40, room)
+    starts = None if new is None else np.concatenate([[0], np.cumsum(new)])
+    count = len(lengths) if new is None else sum(new)
+    q = _query(rng, count, heads * 2, 128)
+    want, tol = plain.attention(q, planes, table, lengths, starts, False)
+    bad = np.zeros(want.shape[:2], dtype=bool)
+    for token, head in ((0, 1), (count - 1, heads * 2 - 1)):
+        q[token, head * 128 + 5] = value
+        bad[token, head] = True
+    out, f32 = ops.kv8_attention(q, *planes, table, lengths, starts, want_f32=True)
+    f32 = f32.reshape(want.shape)
+    assert np.isnan(f32[bad]).all()
+    assert (np.abs(f32 - want)[~bad] <= tol[~bad]).all()
 
 
 @pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("heads,dim,group", [(2, 128, 2), (1, 64, 4), (2, 64, 1), (1, 128, 5)])
+@ROOMS
+@pytest.mark.parametrize("lengths,new", [([5, 100, 33], [5, 5, 5]), ([700, 20, 0, 9], [1, 17, 0, 9]), ([64, 300], [64, 3]), ([2, 40], [4, 40])])
+def test_ragged_new_tokens(ops, e4m3, heads, dim, group, lengths, new, room):
+    """Drafts, prompts, rows without new tokens, and one that is shorter than its new tokens (its first ones get zeros)."""
+    _run(ops, np.random.default_rng(sum(lengths) + group), heads, dim, group, lengths, new, e4m3, room=room)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@ROOMS
+@pytest.mark.parametrize("heads,dim,group,lengths,new", [
+    (8, 128, 2, [140, 33, 32, 350], [140, 16, 17, 129]), (8, 64, 1, [65, 500, 257], [65, 300, 257]), (2, 128, 2, [200], [200]), (1, 128, 2, [129, 400], [129, 130]), (1, 64, 4, [257], [257]), (1, 128, 8, [700], [90]), (1, 64, 1, [600, 1, 350], [300, 1, 129]),
+    (1, 128, 3, [301], [170]), (1, 128, 16, [130], [67])])
+def test_prompts_and_chunks(ops, e4m3, heads, dim, group, lengths, new, room):
+    _run(ops, np.random.default_rng(sum(lengths) + group), heads, dim, group, lengths, new, e4m3, room=room)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@ROOMS
 @pytest.mark.parametrize("new", [None, [40, 140]])
 @pytest.mark.parametrize("spread,size", [(6.0, 1.0), (0.1, 30.0), (0.5, 1e-30)])
-def test_scales_and_queries_of_any_size(ops, e4m3, new, spread, size):
+def test_scales_and_queries_of_any_size(ops, e4m3, new, spread, size, room):
     """Page scales a factor of e^12 apart, scores that leave one token standing, queries that leave none."""
-    _run(ops, np.random.default_rng(41), 2, 128, 2, [500, 333], new, e4m3, spread=spread, size=size)
+    _run(ops, np.random.default_rng(41), 2, 128, 2, [500, 333], new, e4m3, spread=spread, size=size, room=room)
 
 
 @pytest.mark.parametrize("new", [None, [1, 150]])
@@ -92,13 +176,14 @@ def test_scale_of_the_scores_and_a_cut_context(ops, q3t, new):
 
 
 @pytest.mark.parametrize("e4m3", [False, True])
+@ROOMS
 @pytest.mark.parametrize("new", [None, [1, 1, 150]])
-def test_what_lies_behind_the_last_token_does_not_matter(ops, e4m3, new):
+def test_what_lies_behind_the_last_token_does_not_matter(ops, e4m3, new, room):
     """Slots past the end hold NaN codes (e4m3) or -128, pages past the end lie anywhere."""
     rng = np.random.default_rng(47)
     lengths = [21, 250, 199]
     planes = plain.cache(rng, 40, 2, 128, e4m3)
-    table = plain.tables_of(rng, lengths, 40, 20)
+    table = plain.tables_of(rng, lengths, 40, room or 20)
     starts = None if new is None else np.concatenate([[0], np.cumsum(new)])
     q = _query(rng, 3 if new is None else sum(new), 4, 128)
     clean = ops.kv8_attention(q, *planes, table, lengths, starts, e4m3=e4m3)[0]
@@ -109,18 +194,19 @@ def test_what_lies_behind_the_last_token_does_not_matter(ops, e4m3, new):
     assert np.array_equal(clean, dirty)
 
 
+@ROOMS
 @pytest.mark.parametrize("new", [None, [1, 140, 2]])
-def test_bad_pages_are_left_out_and_counted(ops, q3t, new):
+def test_bad_pages_are_left_out_and_counted(ops, q3t, new, room):
     rng = np.random.default_rng(53)
     lengths = [100, 250, 31]
     planes = plain.cache(rng, 40, 2, 128, False)
-    table = plain.tables_of(rng, lengths, 40)
+    table = plain.tables_of(rng, lengths, 40, room)
     table[0, 2], table[1, 0], table[1, 9], table[2, 0], table[2, 1] = 40, -1, 2 ** 31 - 1, -2 ** 31, 41
     starts = None if new is None else np.concatenate([[0], np.cumsum(new)])
     q = _query(rng, 3 if new is None else sum(new), 4, 128)
     before = q3t.library().q3t_kv8_page_error_count()
     out, f32 = ops.kv8_attention(q, *planes, table, lengths, starts, want_f32=True)
-    assert q3t.library().q3t_kv8_page_error_count() > before
+    assert q3t.library().q3t_kv8_page_error_count() >= before + 5
     want, tol = plain.attention(q, planes, table, lengths, starts, False)
     _compare(out, f32, want, tol)
     assert not plain.from_bf16(out[-1]).any()                                 # nothing left of row 2
@@ -197,13 +283,102 @@ def test_the_same_call_gives_the_same_bits(ops):
     lengths = [3000, 700, 1, 5000]
     planes = plain.cache(rng, 560, 2, 128, False)
     table = plain.tables_of(rng, lengths, 560)
-    for new in (None, [1, 100, 1, 300]):
+    for new in (None, [1, 100, 1, 300], [1, 100, 1, 500]):                  # (ranges; the same; prompts in parts)
         starts = None if new is None else np.concatenate([[0], np.cumsum(new)])
         q = _query(rng, 4 if new is None else sum(new), 4, 128)
         first = ops.kv8_attention(q, *planes, table, lengths, starts, want_f32=True)
         for _ in range(4):
             again = ops.kv8_attention(q, *planes, table, lengths, starts, want_f32=True)
             assert np.array_equal(first[0], again[0]) and np.array_equal(first[1], again[1])
+
+
+class _Call:
+    """A launch of its own: descriptor, buffers and, unless one is lent, scratch."""
+    def __init__(self, ops, lib, planes, table, lengths, starts, q, group, scratch=None):
+        import torch
+        i32 = lambda a: torch.tensor(np.asarray(a, dtype=np.int32), device="cuda")  # noqa: E731
+        heads, dim = planes[0].shape[1], planes[0].shape[3]
+        self.lib, self.planes = lib, ops._planes(*planes, False)
+        self.cache = ops.kv8_cache(*self.planes)
+        self.held = [i32(table), i32(lengths), i32(starts), torch.from_numpy(q.view(np.int16)).cuda()]
+        self.out = torch.zeros(q.shape, dtype=torch.int16, device="cuda")
+        self.desc = d = ops.Kv8AttentionDescC(rows=len(lengths), query_heads=heads * group, page_table_stride=table.shape[1], tokens=len(q),
+                                              max_row_tokens=int(np.diff(starts).max()), max_sequence_length=16 * table.shape[1])
+        d.struct_size = C.sizeof(d)
+        d.cache, d.output = C.addressof(self.cache), self.out.data_ptr()
+        d.page_table, d.lengths, d.token_starts, d.query = (t.data_ptr() for t in self.held)
+        size = lib.q3t_kv8_attention_scratch_bytes(C.byref(d))
+        self.scratch = torch.empty(size, dtype=torch.uint8, device="cuda") if scratch is None else scratch
+        assert self.scratch.numel() >= size
+        d.scratch, d.scratch_bytes = self.scratch.data_ptr(), self.scratch.numel()
+
+    def launch(self, stream):
+        assert self.lib.q3t_launch_kv8_attention(C.byref(self.desc), C.c_void_p(stream.cuda_stream)) == 0
+
+    def result(self):
+        return self.out.cpu().numpy().copy()
+
+
+def _calls(ops, lib, scratch=None):
+    """Single tokens, a few tokens over long rows, and prompts in parts beside single tokens."""
+    rng = np.random.default_rng(89)
+    calls = []
+    for lengths, new in (([900, 3000, 40], [1, 1, 1]), ([9000, 700], [12, 30]), ([5000, 4100, 60], [700, 1, 60])):
+        planes = plain.cache(rng, 700, 2, 128, False)
+        q = _query(rng, sum(new), 4, 128)
+        calls.append(_Call(ops, lib, planes, plain.tables_of(rng, lengths, 700, 600), lengths, np.concatenate([[0], np.cumsum(new)]), q, 2, scratch))
+    return calls
+
+
+def test_two_streams_at_once(ops, q3t):
+    import torch
+    first, second = _calls(ops, q3t.library()), _calls(ops, q3t.library())[::-1]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for call in first:
+        call.launch(streams[0])
+    torch.cuda.synchronize()
+    want = [call.result() for call in first]
+    for call in first:
+        call.out.zero_()
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for a, b in zip(first, second):
+            a.launch(streams[0])
+            b.launch(streams[1])
+    torch.cuda.synchronize()
+    for call, other, right in zip(first, second[::-1], want):
+        assert np.array_equal(call.result(), right) and np.array_equal(other.result(), right)
+
+
+def test_captured_graphs_that_share_a_scratch(ops, q3t):
+    """One scratch for launches of every kind, in two graphs that are replayed in turn."""
+    import torch
+    lib = q3t.library()
+    alone = _calls(ops, lib)
+    scratch = max((call.scratch for call in alone), key=lambda t: t.numel())
+    scratch.fill_(0xa5)
+    calls = _calls(ops, lib, scratch)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for call in alone:
+        call.launch(stream)
+        torch.cuda.synchronize()
+    graphs = []
+    for order in ((0, 1, 2), (2, 0, 1)):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=stream):
+            for i in order:
+                calls[i].launch(stream)
+    for n in range(6):
+        for call in calls:
+            call.out.zero_()
+        torch.cuda.synchronize()
+        for _ in range(3):
+            graphs[n % 2].replay()
+        torch.cuda.synchronize()
+        for call, right in zip(calls, alone):
+            assert np.array_equal(call.result(), right.result())
 
 
 @pytest.mark.parametrize("e4m3", [False, True])

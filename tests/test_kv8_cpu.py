@@ -101,6 +101,26 @@ def test_attention_refuses_a_scratch(bind, lib, over):
     assert lib.q3t_launch_kv8_attention(None, None) == INVALID and lib.q3t_kv8_attention_scratch_bytes(None) == 0
 
 
+def test_scratch_is_enough_for_smaller_launches(bind, lib):
+    import random
+    rng = random.Random(5)
+    size = lambda high: int(round(2 ** rng.uniform(0, high)))  # noqa: E731
+    for _ in range(400):
+        heads, group, dim = rng.choice([1, 2, 8, 16]), rng.choice([1, 2, 8]), rng.choice([64, 128])
+        c = _cache(bind, key_value_heads=heads, head_dimension=dim)
+        rows, tokens, length = size(9), size(14), size(18)
+        most = min(size(14), tokens)
+
+        def need(rows, tokens, most, length):
+            d = _attention(bind, c, rows=rows, query_heads=heads * group, page_table_stride=-(-length // 16), tokens=tokens, max_row_tokens=most,
+                           max_sequence_length=length, query_stride=0, output_stride=0)
+            return lib.q3t_kv8_attention_scratch_bytes(C.byref(d))
+        whole = need(rows, tokens, most, length)
+        for _ in range(6):
+            less = [rng.randint(1, n) for n in (rows, tokens, most, length)]
+            assert 0 < need(*less) <= whole
+
+
 @pytest.mark.parametrize("over", BAD_CACHES)
 def test_attention_refuses_a_cache(bind, lib, over):
     c = _cache(bind, **over)
