@@ -11,10 +11,15 @@
 // maximum until a score exceeds it by 2^8, so that outputs are rescaled almost never; weights are kept 2^6 times larger than that
 // needs, which leaves fp16 its 11 bits down to 2^-20 of the largest.
 //
-// The batch's work, the pages of every (row, KV head, block of columns), is cut into as many equal ranges as there are warps, wherever
-// that falls.  A warp writes what it has whole; what is cut is merged by the CTA in shared memory, and of what its range cuts
+// Where segments, (row, KV head, block of 8 columns), are few or short, each is a CTA's or a cluster's (kv8_few_rows_kernel).  Else the
+// batch's work, the pages of every segment, is cut into as many equal ranges as there are warps, wherever that falls
+// (kv8_rows_kernel).  A warp writes what it has whole; what is cut is merged by the CTA in shared memory, and of what its range cuts
 // the CTA leaves (reference, sum, output) and the one with the last ticket folds them in order, so a result depends on
 // the batch's lengths, not on timing.
+//
+// What bounds it: one row, latencies one behind the other (3,000 tokens, 8 heads of 128: 7.0 us); a full batch memory (64 rows of 64 to 2,048 tokens,
+// 140 MB: 31 us, of which 21 are memory's; 7 rows of 90,000 to 131,072, 4 heads, 804 MB: 130 us, 6.2 TB/s); rows of several tokens the conversions
+// and products of 4 warps a scheduler that each wait for their next page (23 drafts of five, heads of 64, 48 MB: 22.5 us).
 
 #include "kv8.cuh"
 #include "q3t_kernels.cuh"
@@ -34,11 +39,21 @@ constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / kWarp;
 constexpr int kRowCtas = 2 * 148;
 constexpr int kTileColumns = 8;                        // of a product
-constexpr int kStartUnits = 2;                         // what the start of a segment counts for in the cut, in pages
+constexpr int kStartUnits = 2;                         // what the start of a segment counts for in the cut, in pages (1 to 3: the same; 4: 2 % more)
 constexpr int kClusterCtas = 8;                        // the most of a segment
+// Clusters as large as lets all segments' CTAs run at once (256 of 296 places: clusters leave some), and not so large that warps have
+// less than half a page; up to 1,024 tokens a CTA.  One token a row, 8 KV heads of 128, clusters / ranges in us: 1 row of 64 tokens 4.1 / 8.6, of
+// 8,192 11.4 / 12.7, of 16,384 18.6 / 14.9; 8 rows of 4,096 15.6 / 18.5; 16 of 2,048 15.3 / 18.7, of 4,096 27.4 / 29.7; 32 of 1,024 15.2 / 20.2, of 2,048
+// 28.7 / 30.7.  (Rows of one length, which suits the clusters: others leave some idle where ranges are even.  Hence the bound on the near side.)
 constexpr int kFewCtas = 256, kFewTokens = 1024, kFewest = 64;
-constexpr int kRowColumns = 32, kShort = 1024;
+// Rows of more columns than this are kv8_prompt.cu's, which takes 64 tokens for 128 columns in the time it takes them for one.  64 rows over 2,048
+// tokens, here / there in us: 32 columns 127 / 132, 48 167 / 132; 16 rows: 32 37 / 37, 48 45 / 37.
+constexpr int kRowColumns = 32;
+// But too few of them leave SMs idle there: they stay here while (query heads x new tokens x tokens seen) is below 2^23, unless even the longest
+// context takes no time there.  One row, 8 KV heads, here / there: over 16,384 48 columns 32 / 45, 64 (2^23) 37 / 45, 256 102 / 55; over
+// 2,048 256 columns 26 / 33, 512 (2^23) 37 / 33; over 1,024 512 columns 25 / 23; over 256 512 columns 16 / 13.
 constexpr long long kPromptWork = 1 << 23;
+constexpr int kShort = 1024;
 constexpr int kCounterBytes = (kRowCtas * 4 + 255) / 256 * 256;
 
 __device__ unsigned int g_kv8_range_errors = 0;
@@ -728,8 +743,10 @@ Plan plan_of(Kv8AttentionArgs& a, int head_dim) {
         a.prompts = 1;
         a.row_columns = kRowColumns;
     }
-    // two tiles of columns a warp where rows may have more than one: what a page costs to read and to convert is paid once
-    return Plan{0, 0, columns > kTileColumns ? 2 : 1};
+    // Two tiles of columns a warp where rows may have more than one: what a page costs to read and to convert is paid once (one tile / two,
+    // 64 rows of 2,048 tokens: 10 columns 94 / 73 us, 32 145 / 127; 16 rows of 512: 16 columns 20 / 21).  Beside prompts the others are mostly
+    // single tokens, which fill one (63 of them and a prompt of 512: 44 / 52; 32 drafts of five and a prompt of 300: 38 / 35).
+    return Plan{0, 0, !a.prompts && columns > kTileColumns ? 2 : 1};
 }
 
 template <int HD, bool E4M3>

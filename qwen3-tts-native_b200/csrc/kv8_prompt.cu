@@ -10,6 +10,14 @@
 //   output    O += W V, the weights from tensor memory
 // While a tile's half is in the softmax the products of its other half and of the other tile run.  A row's reference follows its scores
 // only when its weights outgrow fp16, so that the output in tensor memory is rescaled almost never.
+//
+// Where the blocks of 256 columns are fewer than the SMs they become blocks of 128, and where each could have several SMs to itself and sees 2,048 tokens
+// and more, its steps are cut into parts, which kv8_join_kernel merges.
+//
+// What bounds it: of a half's 2,000 cycles (1,550 with one tile) the products take 1,024 and the exponentials as much, on units that
+// run side by side; the rest is the way of a tile's half through barriers, tensor memory and registers, of which two tiles hide one in the other
+// what two can.  A block costs 7 us more before and after its steps.  A chunk of 4,096 tokens over 16,384 (16 query heads, 8 KV heads of 128): 475 us,
+// 1,010 TFLOP/s; 11 prompts of 667 to 1,333 over 1,400 to 3,333 (32, 8): 410 us; a prompt of 1,500: 29 us; 256 tokens over 16,384: 55 us.
 
 #include "kv8.cuh"
 #include "q3t_kernels.cuh"
@@ -362,7 +370,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         const int tile = warp - kProductWarp;
         if (tile < tiles && steps > 0 && tc::elect_one()) {
             // ---- products of a tile: both operands fp16, sums fp32.  What a step takes here is the looks at barriers, 350 cycles each beside the
-            // copies' stores: hence a thread a tile (one for both: a chunk of 4096 at 16k 645 us), and one barrier for V and the next K.
+            // copies' stores: hence a thread a tile (one for both took 30 % longer), and one barrier for V and the next K.
             const uint32_t scores_idesc = (1u << 4) | ((uint32_t)(kHalf >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
             // B with its rows (dims) contiguous: bit 16
             const uint32_t out_idesc = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
@@ -668,7 +676,9 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8AttentionArgs a,
     }
 }
 
-// Blocks of 128 columns where 256 would leave SMs idle, and where those are so few that each could have several SMs, parts
+// Blocks of 128 columns where 256 would leave SMs idle (one row, 8 KV heads, 128 / 256 in us: 1,024 tokens 23 / 29, 2,048 42 / 46, 2,200 47 / 48; 3,000, past
+// the rule, 79 / 61), and where those of 256 are so few that each could have several SMs, parts (256 tokens over 16,384: 55 us, without 216; over 2,048
+// 32.7 / 36)
 PromptCut prompt_cut(const Kv8AttentionArgs& a) {
     // as many items as any split of the tokens over the rows can make
     const long long columns = (long long)a.tokens * (a.query_heads / a.cache.heads);

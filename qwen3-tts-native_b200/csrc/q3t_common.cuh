@@ -55,7 +55,8 @@ __device__ __forceinline__ float warp_sum_xor(float v) {
 // Library-wide rule: a kernel calls pdl_trigger() only after its own pdl_wait() has returned (in the calling thread).
 // The one exception is rms_norm_rows_kernel, which calls it first of all.  When a grid starts, every grid launched before
 // the last one upstream of it that is not such a norm has therefore completed, and what those wrote may be read
-// ahead of the wait; everything since has to wait.
+// ahead of the wait; everything since has to wait.  (kv8_zero_tickets_kernel triggers first of all too, but the grid behind
+// it waits before anything else, its own trigger included, so that the rule holds from that grid on.)
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

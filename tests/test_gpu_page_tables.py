@@ -58,7 +58,8 @@ def _check(got, want, table, stack, fill=-7):
 
 @pytest.mark.parametrize("rows,longest,stride,spare,prompts,refuse", [
     (1, 0, 4, 4, 40, False), (1, 64, 4, 0, 0, False), (64, 2048, 160, 200, 0, False), (3, 15, 7, 1, 60, False),
-    (37, 300, 64, 60, 500, True), (1000, 400, 96, 900, 700, True), (1025, 90, 12, 40, 60, True), (4096, 100, 40, 2000, 300, True)])
+    (37, 300, 64, 60, 500, True), (1000, 400, 96, 900, 700, True), (1025, 90, 12, 40, 60, True), (4096, 100, 40, 2000, 300, True),
+    (512, 500, 40, 300, 0, True), (513, 500, 40, 300, 0, False)])
 def test_against_a_loop_over_the_rows(ops, rows, longest, stride, spare, prompts, refuse):
     rng = np.random.default_rng(rows + longest)
     for _ in range(3):
@@ -95,11 +96,12 @@ def test_free_count_outside_the_pool_is_clamped(ops):
     assert got["status"].tolist() == [plain.NO_PAGES] and got["free_count"] == 0
 
 
-def test_in_place_captured_and_replayed_on_another_stream(ops, q3t):
-    """A step's tables captured once, lengths and stack advanced in place by every replay."""
+@pytest.mark.parametrize("capacity", [5, 64, 5000])
+def test_in_place_captured_and_replayed_on_another_stream(ops, q3t, capacity):
+    """A step's tables captured once, lengths and stack advanced in place by every replay (one launch, or two)."""
     import torch
     lib = q3t.library()
-    rows, stride, pages, capacity, steps = 5, 8, 40, 5, 37
+    rows, stride, pages, steps = 5, 8, 40, 37
     rng = np.random.default_rng(3)
     lengths = np.array([0, 1, 15, 16, 40])
     table = plain.tables_of(rng, lengths, pages, stride)
