@@ -151,7 +151,9 @@ struct Walk {
         }
     }
 
-    // pages page_first .. page_end - 1, at least one
+    // pages page_first .. page_end - 1, at least one.  AHEAD: the page after the next one is called into the L2, a line a lane, where a warp
+    // walks many of 4 KB (64 rows of 8,192 tokens: 169 us, without 176.5; heads of 64, which wait for instructions: 6 % longer with it)
+    template <bool AHEAD>
     __device__ __forceinline__ void run(const Kv8AttentionArgs& a, const RowWork& w, const Segment& of, int page_first, int page_end) {
         const int row = of.row, kv_head = of.kv_head, columns = of.columns;
         const bool counts = of.counts;
@@ -259,6 +261,14 @@ struct Walk {
             const int next_raw = __shfl_sync(0xffffffffu, ids, next & 31);
             const int next_id = usable(next_raw) ? next_raw : 0;
             const bool more = page + 1 < page_end;
+            if (AHEAD && page + 2 < page_end && (next & 31) != 31) {
+                const int ahead = __shfl_sync(0xffffffffu, ids, (next + 1) & 31);
+                constexpr int kLines = kPageTokens * HD / 128;
+                const uint8_t* const plane = lane < kLines ? a.cache.k : a.cache.v;
+                if (lane < 2 * kLines && usable(ahead)) {
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(plane + (long long)ahead * a.cache.page_stride + (size_t)kv_head * (kPageTokens * HD) + lane % kLines * 128));
+                }
+            }
 
             // ---- scores
             float s[TILES][4];
@@ -501,7 +511,7 @@ __global__ void __launch_bounds__(kRowThreads, rows_residency<HD, TILES>()) kv8_
 
         const Segment of{row, kv_head, block * kColumns, columns, segment == 0};
         Walk<HD, E4M3, TILES> walk;
-        walk.run(a, w, of, page_first, page_end);
+        walk.template run<HD == 128>(a, w, of, page_first, page_end);
         // ---- whole: written; cut: into shared memory
         if (page_first == 0 && page_end == w.pages) {
             walk.write(a, w.span.first, of);
@@ -649,7 +659,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) kv8_few_rows_kernel(const Kv8A
     const int page_first = (int)((long long)w.pages * which / warps), page_end = (int)((long long)w.pages * (which + 1) / warps);
     {
         W walk;
-        if (page_first < page_end) walk.run(a, w, of, page_first, page_end);
+        if (page_first < page_end) walk.template run<false>(a, w, of, page_first, page_end);
         walk.keep(parts + (size_t)warp * W::kPiece, of.columns);
     }
     __syncthreads();
