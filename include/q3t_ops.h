@@ -433,7 +433,7 @@ QWEN3_TTS_API int32_t q3t_launch_kv8_append(const Q3tKv8Cache* cache, const uint
  * the positions up to its own.  Query head h reads key/value head h / (query_heads / key_value_heads).  A token without a
  * position (a row shorter than its new tokens) gets zeros; output behind the last token is left as it was.
  * Scores, statistics and sums are fp32; query and weights enter the products as fp16 with 11 bits kept, scaled by powers of two so
- * that neither size matters.  Bounds that the host gives (tokens, max_row_tokens, max_sequence_length) cut what the device finds
+ * that neither size matters; the scales of a row's value pages may lie 2^80 apart, and values below 2^-71 lose bits.  Bounds that the host gives (tokens, max_row_tokens, max_sequence_length) cut what the device finds
  * larger: a row is then computed over its first max_sequence_length tokens and counted by q3t_attention_range_error_count. A page id
  * outside 0..pages - 1 is left out of the attention, as if masked, and counted by q3t_kv8_page_error_count. */
 typedef struct Q3tKv8AttentionDesc {

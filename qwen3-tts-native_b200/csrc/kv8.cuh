@@ -103,6 +103,10 @@ __device__ __forceinline__ RowSpan row_span(const int* starts, const int* length
 
 constexpr float kKv8Slack = 8.0f;         // log2 of how far a score may exceed its row's reference
 constexpr float kKv8Lift = 6.0f;          // log2 of the weight at the reference
+// A smaller value scale (a page of zeros has 2^-126) counts as this one where references and sums are concerned, or w / value scale would pass fp32,
+// and its weights are made smaller by as much.  Values below 2^-71 so lose bits of their weights; and 2^80 is as far as others' scales
+// may lie above without weights of 2^-40 of the largest leaving fp32's range.
+constexpr float kKv8LeastValueScale = 8.27180613e-25f;        // 2^-80
 
 struct Kv8AttentionArgs {
     Kv8View cache;

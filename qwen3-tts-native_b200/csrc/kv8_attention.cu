@@ -287,7 +287,8 @@ struct Walk {
                     for (int n = 0; n < TILES; ++n) mma_f16(s[n], a0, a1, a2, a3, qf[n][j][e][0], qf[n][j][e][1]);
                 }
             }
-            const float ks = key_scale, vs = fmaxf(value_scale, kKv8SmallestScale);
+            const float ks = key_scale, vs = fmaxf(value_scale, kKv8LeastValueScale);
+            const float back = fminf(value_scale * (1.0f / kKv8LeastValueScale), 1.0f);
             if (more) load_keys(next_id);
             // ---- weights of the codes
             const float lv = log2_fast(vs), inverse = reciprocal_fast(vs);
@@ -329,6 +330,13 @@ struct Walk {
                     low[c] = exp2_ftz(s[n][c] - reference);
                     high[c] = exp2_ftz(s[n][2 + c] - reference);
                     sum_of[n][c] = fmaf(low[c] + high[c], inverse, sum_of[n][c]);
+                }
+                if (back != 1.0f) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        low[c] *= back;
+                        high[c] *= back;
+                    }
                 }
                 b0[n] = transpose8(pack_half2(low[0], low[1]));
                 b1[n] = transpose8(pack_half2(high[0], high[1]));

@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
     unsigned char* const queries = smem;                               // [tile]
     unsigned char* const keys = smem + Smem::kQueryBytes;              // [step % 2]
     unsigned char* const values = keys + 2 * Smem::kTileBytes;         // [step % 2]
-    __shared__ float4 scales[kScaleRing][kStepPages];                  // of each page: key scale, log2 and reciprocal of the value scale
+    __shared__ float4 scales[kScaleRing][kStepPages];                  // of each page: key scale, log2 and reciprocal of the value scale, what its weights miss
     // full: V of a step and K of the next one
     __shared__ uint64_t first_k, full[2], empty_k[2], empty_v[2], s_ready[2][2], p_ready[2][2], o_ready[2][2], q_ready;     // [tile][half]
     __shared__ uint32_t tmem_slot;
@@ -333,9 +333,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
             if (step >= 2 && !__all_sync(0xffffffffu, guard.wait(&empty[buffer], ((step >> 1) - 1) & 1))) break;
             if (t < kStepPages && !is_value) {
                 // a page that is not there weighs nothing: its codes are zeros, its value scale is as well
-                const float vs = fmaxf(value_scale, kKv8SmallestScale);
-                scales[step % kScaleRing][t] = (good >> t) & 1u ? make_float4(key_scale, log2_fast(vs), reciprocal_fast(vs), 0.0f)
-                                                               : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+                const float vs = fmaxf(value_scale, kKv8LeastValueScale), back = fminf(value_scale * (1.0f / kKv8LeastValueScale), 1.0f);
+                scales[step % kScaleRing][t] = (good >> t) & 1u ? make_float4(key_scale, log2_fast(vs), reciprocal_fast(vs), back)
+                                                               : make_float4(0.0f, -INFINITY, 0.0f, 1.0f);
             }
             unsigned char* const tile = buffers + buffer * Smem::kTileBytes + store_at;
 #pragma unroll
@@ -525,6 +525,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
                     largest = fmaxf(largest, x);
                     added = fmaf(x, f.z, added);
                 }
+                // (nor does this path take value scales below the least)
+                static_assert(kHalfPages == 4, "pages of a half");
+                if (fminf(fminf(page_scales[0].w, page_scales[1].w), fminf(page_scales[2].w, page_scales[3].w)) != 1.0f) largest = INFINITY;
                 if (!__any_sync(0xffffffffu, largest > kMostWeight)) {
                     total += added;
                     tmem_store_16(s_at, w[0]);
@@ -568,7 +571,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
                         const float x = exp2_ftz(16 * p + j >= visible ? -INFINITY : fmaf(__uint_as_float(at[0]), slope, shift));
                         const float y = exp2_ftz(16 * p + j + 1 >= visible ? -INFINITY : fmaf(__uint_as_float(at[1]), slope, shift));
                         sum += x + y;
-                        w[j / 2] = pack_half2(x, y);
+                        w[j / 2] = pack_half2(x * page_scales[p].w, y * page_scales[p].w);
                     }
                     total = fmaf(sum, page_scales[p].z, total);
                     tmem_store_8(s_at + 8 * p, w);

@@ -145,7 +145,8 @@ def attention(q, planes, table, lengths, starts, e4m3, max_seq=None, scale=None)
     fp32: a sum of dim products (and one scale) is off by (dim + 8) * 2^-24 of the sum of magnitudes, and an error of the exponent is
     a relative error of the weight; 2^-21 for the exponential itself.  Sums over n tokens: n * 2^-24.  What multiplies the codes, p_j times
     the page's scale, is subnormal as fp16 (or, far below, zero) where it is less than 2^-20 of the largest such product: an absolute error of
-    2^-31 of that one each, times a code of at most M in any dimension, whatever the dimension's own sum is."""
+    2^-31 of that one each, times a code of at most M in any dimension, whatever the dimension's own sum is.  Scales below 2^-80 count as
+    that there."""
     kc, vc, ks, vs = planes
     heads, dim = kc.shape[1], kc.shape[3]
     qf = from_bf16(q).astype(np.float64).reshape(len(q), -1, dim)
@@ -175,7 +176,7 @@ def attention(q, planes, table, lengths, starts, e4m3, max_seq=None, scale=None)
                 out[t, g] = p @ v
                 size = p @ np.abs(v)
                 each = 2.0 ** -11 + off[:, None] + 2.0 ** -21 + len(k) * 2.0 ** -24
-                most = (448 if e4m3 else 127) * np.repeat(vs[ids, h].astype(np.float64), PAGE)[:seen][good]
+                most = (448 if e4m3 else 127) * np.repeat(np.maximum(vs[ids, h].astype(np.float64), 2.0 ** -80), PAGE)[:seen][good]
                 tol[t, g] = 2 * each * size + len(k) * 2.0 ** -31 * (p * most).max(axis=1)[:, None]
     return out, tol
 

@@ -118,6 +118,26 @@ def test_scores_that_grow_along_the_context(ops, heads, lengths, new, room, e4m3
     _compare(out, f32, want, tol)
 
 
+@pytest.mark.parametrize("heads,lengths,new,room", [(2, [700, 500], None, None), (2, [700, 500], None, FEW_TOKENS), (2, [900, 64], [90, 30], LONG), (8, [400], [140], None)])
+@pytest.mark.parametrize("zeros,size", [(z, n) for z in ("first", "most", "all") for n in (1.0, 1e8, 1e-18, 1e-27)] + [("none", 1e36), ("none", 1e-30)])
+def test_pages_of_zeros_weigh_what_their_scores_say(ops, heads, lengths, new, room, zeros, size):
+    """Values of nothing have the scale 2^-126, and their tokens a share of the sum all the same; values from the smallest to the largest."""
+    e4m3 = zeros in ("first", "none")
+    rng = np.random.default_rng(97)
+    planes = plain.cache(rng, 120, heads, 128, e4m3)
+    table = plain.tables_of(rng, lengths, 120, room)
+    planes[3] *= np.float32(size)
+    for r, n in enumerate(lengths):
+        ids = table[r, :-(-n // 16)]
+        none = {"none": ids[:0], "first": ids[:len(ids) // 2], "most": ids[np.arange(len(ids)) % 9 != 4], "all": ids}[zeros]
+        planes[1][none], planes[3][none] = 0, plain.SMALLEST
+    starts = None if new is None else np.concatenate([[0], np.cumsum(new)])
+    q = _query(rng, len(lengths) if new is None else sum(new), heads * 2, 128, 2.0)
+    out, f32 = ops.kv8_attention(q, *planes, table, lengths, starts, e4m3=e4m3, want_f32=True)
+    want, tol = plain.attention(q, planes, table, lengths, starts, e4m3)
+    _compare(out, f32, want, tol)
+
+
 @pytest.mark.parametrize("heads,lengths,new,room", [(2, [300, 200], None, None), (2, [300, 200], None, FEW_TOKENS), (2, [300], [150], LONG), (8, [300], [150], None)])
 @pytest.mark.parametrize("value", [0x7f80, 0xffc0])
 def test_queries_that_are_not_finite_stay_in_their_rows(ops, heads, lengths, new, room, value):
