@@ -45,6 +45,7 @@ constexpr int kClusterCtas = 8;                        // the most of a segment
 // less than half a page; up to 1,024 tokens a CTA.  One token a row, 8 KV heads of 128, clusters / ranges in us: 1 row of 64 tokens 4.1 / 8.6, of
 // 8,192 11.4 / 12.7, of 16,384 18.6 / 14.9; 8 rows of 4,096 15.6 / 18.5; 16 of 2,048 15.3 / 18.7, of 4,096 27.4 / 29.7; 32 of 1,024 15.2 / 20.2, of 2,048
 // 28.7 / 30.7.  (Rows of one length, which suits the clusters: others leave some idle where ranges are even.  Hence the bound on the near side.)
+// Short rows also in two rounds: 64 rows of 64 8.1 / 11.1, of 256 12.3 / 14.7, of 512 17.7 / 19.8, of 1 to 512 13.7 / 15.2, of 1,024 31.5 / 30.7.
 constexpr int kFewCtas = 256, kFewTokens = 1024, kFewest = 64;
 // Rows of more columns than this are kv8_prompt.cu's, which takes 64 tokens for 128 columns in the time it takes them for one.  64 rows over 2,048
 // tokens, here / there in us: 32 columns 127 / 132, 48 167 / 132; 16 rows: 32 37 / 37, 48 45 / 37.
@@ -756,7 +757,9 @@ Plan plan_of(Kv8AttentionArgs& a, int head_dim) {
     a.prompts = 0;
     a.row_columns = INT_MAX;
     a.scratch_taken = kCounterBytes + kRowCtas * 2 * 2 * kTileColumns * (head_dim + 4) * (int)sizeof(float);
-    if (segments * cluster <= kFewCtas && a.max_sequence <= kFewTokens * cluster) return Plan{cluster, (int)blocks, 0};
+    if ((segments * cluster <= kFewCtas && a.max_sequence <= kFewTokens * cluster) || (segments <= 2 * kFewCtas && a.max_sequence <= kFewTokens / 2)) {
+        return Plan{cluster, (int)blocks, 0};
+    }
     if (columns > kRowColumns && ((long long)a.tokens * a.query_heads * a.max_sequence >= kPromptWork || a.max_sequence <= kShort)) {
         a.prompts = 1;
         a.row_columns = kRowColumns;

@@ -69,9 +69,9 @@ def test_many_rows(ops, rows, room):
 @pytest.mark.parametrize("e4m3", [False, True])
 @pytest.mark.parametrize("heads,dim,group,rows,longest,new", [
     (1, 128, 2, 4, 5000, None), (2, 64, 1, 16, 7000, None), (8, 128, 1, 8, 4096, None), (8, 128, 2, 16, 2000, None), (4, 64, 8, 60, 900, None),
-    (2, 128, 4, 4, 3000, [3, 1, 9, 0]), (8, 64, 2, 3, 1500, [30, 4, 11])])
+    (8, 128, 2, 50, 500, None), (2, 128, 4, 4, 3000, [3, 1, 9, 0]), (8, 64, 2, 3, 1500, [30, 4, 11])])
 def test_clusters_of_every_size(ops, e4m3, heads, dim, group, rows, longest, new):
-    """8, 8, 4, 2 and 1 CTAs a segment, with blocks that some rows do not have; among the rows one of nothing and one of one page."""
+    """8, 8, 4, 2 and 1 CTAs a segment, these in two rounds as well, with blocks that some rows do not have; among the rows one of nothing and one of one page."""
     rng = np.random.default_rng(rows + longest)
     lengths = [int(n) for n in rng.integers(20, longest + 1, rows)]
     lengths[0] = longest
