@@ -19,7 +19,7 @@
 //
 // What bounds it: one row, latencies one behind the other (3,000 tokens, 8 heads of 128: 7.0 us); a full batch memory (64 rows of 64 to 2,048 tokens,
 // 140 MB: 31 us, of which 21 are memory's; 7 rows of 90,000 to 131,072, 4 heads, 804 MB: 130 us, 6.2 TB/s); rows of several tokens the conversions
-// and products of 4 warps a scheduler that each wait for their next page (23 drafts of five, heads of 64, 48 MB: 22.5 us).
+// and products of 4 warps a scheduler that each wait for their next page (23 drafts of five, heads of 64, 48 MB: 23 us).
 
 #include "kv8.cuh"
 #include "q3t_kernels.cuh"
