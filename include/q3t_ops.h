@@ -361,6 +361,7 @@ QWEN3_TTS_API int32_t q3t_test_prompt_attention(const Q3tAttentionDesc* desc, in
  * the stack (a row's own in the order of its table), then rows that grow take theirs from its top.  Same inputs, same tables.
  * A row is served whole or not at all: status[r] says which, and one that is not served keeps its length and table and gets
  * no tokens.  What it asked for still counts against the rows behind it; rows that need no page are served either way.
+ * Rows do not share pages: one that two of them gave back would be on the stack twice.
  * New tokens get numbers in the order of the rows: those of row r are token_starts[r] .. token_starts[r + 1] - 1, at the
  * positions lengths[r], lengths[r] + 1, ... and in the slots page id * 16 + position % 16.  positions and slots behind the last
  * token, table entries behind a row's last page and stack entries from *new_free_count on are left as they were.
@@ -395,7 +396,7 @@ QWEN3_TTS_API int32_t q3t_launch_page_tables(const Q3tPageTablesDesc* desc, void
 
 /* A cache of 8-bit codes.  A page holds 16 tokens of one plane (K or V) as [key_value_heads][16][head_dimension] codes, the
  * layout of the bf16 pages, and has one fp32 scale for each head: value = code * scale.  Codes are int8 (-127..127) or
- * e4m3.  The planes' pages may lie apart (page_stride, scale_stride), so that one pool can hold many layers. */
+ * e4m3; scales are positive.  The planes' pages may lie apart (page_stride, scale_stride), so that one pool can hold many layers. */
 enum { Q3T_KV8_INT8 = 0, Q3T_KV8_E4M3 = 1 };
 typedef struct Q3tKv8Cache {
     uint32_t struct_size;        /* sizeof(Q3tKv8Cache) */
