@@ -125,7 +125,7 @@ struct Kv8AttentionArgs {
     void* scratch;
     int scratch_taken;        // bytes of it that are kv8_attention.cu's
     int prompts;              // a launch of kv8_prompt.cu follows
-    int row_columns;          // (new tokens x query heads of a KV head) of a row up to which it is not that one's
+    int row_columns;          // (new tokens x query heads of a KV head) of a row up to which it is not that one's; 0: every row is, and no other launch precedes it
 };
 
 __device__ __forceinline__ float exp2_ftz(float x) {

@@ -48,11 +48,12 @@ constexpr int kClusterCtas = 8;                        // the most of a segment
 // Short rows also in two rounds: 64 rows of 64 8.1 / 11.1, of 256 12.3 / 14.7, of 512 17.7 / 19.8, of 1 to 512 13.7 / 15.2, of 1,024 31.5 / 30.7.
 constexpr int kFewCtas = 256, kFewTokens = 1024, kFewest = 64;
 // Rows of more columns than this are kv8_prompt.cu's, which takes 64 tokens for 128 columns in the time it takes them for one.  64 rows over 2,048
-// tokens, here / there in us: 32 columns 127 / 132, 48 167 / 132; 16 rows: 32 37 / 37, 48 45 / 37.
+// tokens, here / there in us: 32 columns 127 / 132, 48 167 / 132; 16 rows: 32 36 / 37, 48 45 / 37.
 constexpr int kRowColumns = 32;
 // But too few of them leave SMs idle there: they stay here while (query heads x new tokens x tokens seen) is below 2^23, unless even the longest
-// context takes no time there.  One row, 8 KV heads, here / there: over 16,384 48 columns 32 / 45, 64 (2^23) 37 / 45, 256 102 / 55; over
-// 2,048 256 columns 26 / 33, 512 (2^23) 37 / 33; over 1,024 512 columns 25 / 23; over 256 512 columns 16 / 13.
+// context takes no time there.  One row, 8 KV heads, here / there: over 16,384 48 columns 34 / 40, 64 (2^23) 40 / 40, 256 111 / 51; over
+// 2,048 256 columns 27 / 31, 512 (2^23) 39 / 31; over 1,024 512 columns 27 / 21; over 256 512 columns 17 / 11.  A row alone that goes there is the only
+// one, so that nothing is launched here (a prompt of 1,500 tokens 27.5 us, with two launches for rows that are not there 29.2).
 constexpr long long kPromptWork = 1 << 23;
 constexpr int kShort = 1024;
 constexpr int kCounterBytes = (kRowCtas * 4 + 255) / 256 * 256;
@@ -747,7 +748,7 @@ cudaError_t launch_rows(const Kv8AttentionArgs& a, cudaStream_t stream) {
 struct Plan {
     int cluster;       // of kv8_few_rows_kernel; 0: not that one
     int blocks;        // its blocks of columns
-    int tiles;         // of kv8_rows_kernel
+    int tiles;         // of kv8_rows_kernel; 0: not that one either, the one row is a prompt
 };
 Plan plan_of(Kv8AttentionArgs& a, int head_dim) {
     const long long columns = (long long)a.most * (a.query_heads / a.cache.heads), blocks = (columns + kTileColumns - 1) / kTileColumns;
@@ -762,7 +763,8 @@ Plan plan_of(Kv8AttentionArgs& a, int head_dim) {
     }
     if (columns > kRowColumns && ((long long)a.tokens * a.query_heads * a.max_sequence >= kPromptWork || a.max_sequence <= kShort)) {
         a.prompts = 1;
-        a.row_columns = kRowColumns;
+        a.row_columns = a.rows > 1 ? kRowColumns : 0;
+        if (a.rows == 1) return Plan{0, 0, 0};
     }
     // Two tiles of columns a warp where rows may have more than one: what a page costs to read and to convert is paid once (one tile / two,
     // 64 rows of 2,048 tokens: 10 columns 94 / 73 us, 32 145 / 127; 16 rows of 512: 16 columns 20 / 21).  Beside prompts the others are mostly
@@ -773,6 +775,7 @@ Plan plan_of(Kv8AttentionArgs& a, int head_dim) {
 template <int HD, bool E4M3>
 cudaError_t launch_attention(const Kv8AttentionArgs& a, const Plan& plan, cudaStream_t stream) {
     if (plan.cluster > 0) return launch_few_rows<HD, E4M3>(a, plan.blocks, plan.cluster, stream);
+    if (plan.tiles == 0) return launch_kv8_prompts(a, HD, E4M3, stream);
     return plan.tiles == 2 ? launch_rows<HD, E4M3, 2>(a, stream) : launch_rows<HD, E4M3, 1>(a, stream);
 }
 
@@ -815,9 +818,10 @@ bool attention_args(const Q3tKv8AttentionDesc* d, Kv8AttentionArgs* a) {
 
 unsigned int kv8_append_page_error_count();
 unsigned int kv8_prompt_page_error_count();
+unsigned int kv8_prompt_range_error_count();
 unsigned int kv8_range_error_count() {
     unsigned int v = 0;
-    return cudaMemcpyFromSymbol(&v, g_kv8_range_errors, sizeof(v)) == cudaSuccess ? v : ~0u;
+    return cudaMemcpyFromSymbol(&v, g_kv8_range_errors, sizeof(v)) == cudaSuccess ? v + kv8_prompt_range_error_count() : ~0u;
 }
 
 }  // namespace q3t

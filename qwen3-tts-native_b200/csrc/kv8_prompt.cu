@@ -16,8 +16,8 @@
 //
 // What bounds it: of a half's 2,000 cycles (1,550 with one tile) the products take 1,024 and the exponentials as much, on units that
 // run side by side; the rest is the way of a tile's half through barriers, tensor memory and registers, of which two tiles hide one in the other
-// what two can.  A block costs 7 us more before and after its steps.  A chunk of 4,096 tokens over 16,384 (16 query heads, 8 KV heads of 128): 475 us,
-// 1,010 TFLOP/s; 11 prompts of 667 to 1,333 over 1,400 to 3,333 (32, 8): 410 us; a prompt of 1,500: 29 us; 256 tokens over 16,384: 55 us.
+// what two can.  A block costs 7 us more before and after its steps.  A chunk of 4,096 tokens over 16,384 (16 query heads, 8 KV heads of 128): 472 us,
+// 1,018 TFLOP/s; 11 prompts of 667 to 1,333 over 1,400 to 3,333 (32, 8): 408 us; a prompt of 1,500: 27.5 us; 256 tokens over 16,384: 53 us.
 
 #include "kv8.cuh"
 #include "q3t_kernels.cuh"
@@ -43,6 +43,7 @@ constexpr long long kBudgetCycles = 4000000000ll;        // about two seconds
 
 __device__ unsigned int g_kv8_prompt_errors = 0;
 __device__ unsigned int g_kv8_prompt_page_errors = 0;
+__device__ unsigned int g_kv8_prompt_range_errors = 0;
 
 template <int HD>
 struct PromptSmem {
@@ -174,6 +175,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
 
     // ---- this CTA's columns: the rows of many columns have ceil(columns / block_columns) items a KV head; those of a row's last tokens, which see
     // the most, first, all KV heads of a block together
+    if (a.row_columns == 0) pdl_wait();                                // (else the launch ahead has waited and counts what lies outside the host's bounds)
     if (tid == 0) found.row = -1;
     __syncthreads();
     int sum = 0;
@@ -184,6 +186,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         if (row < a.rows) {
             span = row_span(a.starts, a.lengths, row, a.tokens, a.most, a.max_sequence);
             const long long columns = (long long)span.count * group;
+            if (a.row_columns == 0 && span.cut && blockIdx.x == 0) atomicAdd(&g_kv8_prompt_range_errors, 1u);
             own = columns > a.row_columns ? (int)((columns + block_columns - 1) / block_columns) * heads * most_parts : 0;
             mine = own;
         }
@@ -679,9 +682,9 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8AttentionArgs a,
     }
 }
 
-// Blocks of 128 columns where 256 would leave SMs idle (one row, 8 KV heads, 128 / 256 in us: 1,024 tokens 23 / 29, 2,048 42 / 46, 2,200 47 / 48; 3,000, past
-// the rule, 79 / 61), and where those of 256 are so few that each could have several SMs, parts (256 tokens over 16,384: 55 us, without 216; over 2,048
-// 32.7 / 36)
+// Blocks of 128 columns where 256 would leave SMs idle (one row, 8 KV heads, 128 / 256 in us, behind the short rows' launches: 1,024 tokens 23 / 29, 2,048
+// 42 / 46, 2,200 47 / 48; 3,000, past the rule, 79 / 61), and where those of 256 are so few that each could have several SMs, parts (256 tokens over
+// 16,384: 55 us, without 216; over 2,048 32.7 / 36)
 PromptCut prompt_cut(const Kv8AttentionArgs& a) {
     // as many items as any split of the tokens over the rows can make
     const long long columns = (long long)a.tokens * (a.query_heads / a.cache.heads);
@@ -743,6 +746,10 @@ cudaError_t launch_kv8_prompts(const Kv8AttentionArgs& a, int head_dim, bool e4m
 unsigned int kv8_prompt_error_count() {
     unsigned int v = 0;
     return cudaMemcpyFromSymbol(&v, g_kv8_prompt_errors, sizeof(v)) == cudaSuccess ? v : ~0u;
+}
+unsigned int kv8_prompt_range_error_count() {
+    unsigned int v = 0;
+    return cudaMemcpyFromSymbol(&v, g_kv8_prompt_range_errors, sizeof(v)) == cudaSuccess ? v : ~0u;
 }
 unsigned int kv8_prompt_page_error_count() {
     unsigned int v = 0;

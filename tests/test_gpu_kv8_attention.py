@@ -195,6 +195,19 @@ def test_scale_of_the_scores_and_a_cut_context(ops, q3t, new):
     assert q3t.library().q3t_attention_range_error_count() == before + 1
 
 
+@pytest.mark.parametrize("heads,group,length,new,most", [(16, 2, 300, 140, 272), (1, 16, 9000, 64, 8992), (2, 2, 300, 20, 272)])
+def test_a_cut_context_of_one_row(ops, q3t, heads, group, length, new, most):
+    """A prompt alone is one launch (or, in parts, two), which counts for itself; a row of no new tokens has nothing to write."""
+    before = q3t.library().q3t_attention_range_error_count()
+    _run(ops, np.random.default_rng(most), heads, 64, group, [length], [new], False, max_seq=most)
+    assert q3t.library().q3t_attention_range_error_count() == before + 1
+    rng = np.random.default_rng(most + 1)
+    planes = plain.cache(rng, 570, heads, 64, False)
+    q = _query(rng, new, heads * group, 64)
+    out, _ = ops.kv8_attention(q, *planes, plain.tables_of(rng, [length], 570), [length], [0, 0], max_row_tokens=new, fill=0x1234)
+    assert (out == 0x1234).all()
+
+
 @pytest.mark.parametrize("e4m3", [False, True])
 @ROOMS
 @pytest.mark.parametrize("new", [None, [1, 1, 150]])
