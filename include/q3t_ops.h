@@ -282,7 +282,8 @@ QWEN3_TTS_API int32_t q3t_launch_batch_causal_gqa_attention_fast(
  * scratch, the grid and the per-row ticket counts are sized from max_sequence_length).  A row whose
  * position lies outside is computed over the clamped length instead of running past them, and is
  * counted (process-wide) in q3t_attention_range_error_count(): a caller that cannot vouch for its
- * positions compares that counter before and after. */
+ * positions compares that counter before and after.  UINT32_MAX, here and from the other counters:
+ * it could not be read. */
 QWEN3_TTS_API uint32_t q3t_attention_range_error_count(void);
 
 /* No counterpart in the reference.  The same operator for hosts that may not allocate device

@@ -1161,10 +1161,11 @@ int32_t q3t_test_sort_chain_places(const uint32_t* of_sm, const uint32_t* of_pag
 int32_t q3t_test_hold_sms(int32_t ctas, uint64_t ns, void* stream) { return static_cast<int32_t>(launch_hold_sms(ctas, ns, S(stream))); }
 
 uint32_t q3t_kernel_error_count(void) {
-    return gemm_tc_error_count() + gemm_wide_error_count() + gemm_pair_error_count() + gemv_mma_error_count() + chain_error_count() + lockstep_error_count() + prompt_attention_error_count() + kv8_prompt_error_count();
+    return sum_of_counts({gemm_tc_error_count(), gemm_wide_error_count(), gemm_pair_error_count(), gemv_mma_error_count(), chain_error_count(),
+                          lockstep_error_count(), prompt_attention_error_count(), kv8_prompt_error_count()});
 }
 
-uint32_t q3t_attention_range_error_count(void) { return attention_range_error_count() + kv8_range_error_count(); }
+uint32_t q3t_attention_range_error_count(void) { return sum_of_counts({attention_range_error_count(), kv8_range_error_count()}); }
 
 int32_t q3t_session_current_token(Qwen3TtsSessionHandle session, uint16_t* token, char* error,
                                   size_t error_capacity) {

@@ -821,14 +821,16 @@ unsigned int kv8_prompt_page_error_count();
 unsigned int kv8_prompt_range_error_count();
 unsigned int kv8_range_error_count() {
     unsigned int v = 0;
-    return cudaMemcpyFromSymbol(&v, g_kv8_range_errors, sizeof(v)) == cudaSuccess ? v + kv8_prompt_range_error_count() : ~0u;
+    return cudaMemcpyFromSymbol(&v, g_kv8_range_errors, sizeof(v)) == cudaSuccess ? sum_of_counts({v, kv8_prompt_range_error_count()}) : ~0u;
 }
 
 }  // namespace q3t
 
 extern "C" uint32_t q3t_kv8_page_error_count(void) {
+    using namespace q3t;
     unsigned int v = 0;
-    return cudaMemcpyFromSymbol(&v, q3t::g_kv8_page_errors, sizeof(v)) == cudaSuccess ? v + q3t::kv8_append_page_error_count() + q3t::kv8_prompt_page_error_count() : ~0u;
+    return cudaMemcpyFromSymbol(&v, g_kv8_page_errors, sizeof(v)) == cudaSuccess
+               ? sum_of_counts({v, kv8_append_page_error_count(), kv8_prompt_page_error_count()}) : ~0u;
 }
 
 extern "C" size_t q3t_kv8_attention_scratch_bytes(const Q3tKv8AttentionDesc* desc) {

@@ -5,6 +5,8 @@
 
 #include "q3t_common.cuh"
 
+#include <initializer_list>
+
 namespace q3t {
 
 // Per-device one-time set-up (dynamic shared-memory ceilings).  Call with the device current
@@ -213,9 +215,18 @@ cudaError_t launch_attention_reference_order(const AttentionArgs& args, cudaStre
 // launcher that honours it: in mode 0 a fused call appends with the split-KV kernel's prologue,
 // then attends in the reference's order.
 // rows seen so far whose position lay outside what the launch was sized for (clamped and counted)
-unsigned int kv8_range_error_count();          // kv8_attention.cu
-unsigned int kv8_prompt_error_count();         // kv8_prompt.cu
 unsigned int attention_range_error_count();
+unsigned int kv8_range_error_count();          // the same over an 8-bit cache (kv8_attention.cu)
+unsigned int kv8_prompt_error_count();         // waits of kv8_prompt.cu that ran out
+// Several kernels' counts as one: ~0u, which says that it cannot be read, where that is so of any of them; else their sum, which stops short of it
+inline unsigned int sum_of_counts(std::initializer_list<unsigned int> counts) {
+    unsigned int sum = 0;
+    for (const unsigned int n : counts) {
+        if (n == ~0u) return ~0u;
+        sum = n < ~0u - 1 - sum ? sum + n : ~0u - 1;
+    }
+    return sum;
+}
 cudaError_t set_attention_error_sink(unsigned int* device_visible_word);
 int set_attention_mode(int mode);
 int attention_mode();
