@@ -595,16 +595,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         if (parts > 1 && real) *reinterpret_cast<float2*>(part_at + 2 * kTileRows * HD + 2 * r) = make_float2(top, total);
         int head;
         const size_t token = item.span.first + place_of(min(r, columns - 1), head), at = (size_t)(item.kv_head * group + head) * HD;
+        const bool gave_up = __any_sync(0xffffffffu, *abort_flag != 0);
 #pragma unroll 1
         for (int c = 0; c < HD; c += 64) {
             uint32_t o[2][32];
+            __syncwarp();                                              // the loads are the whole warp's, what comes before and behind them is not
             if (own > 0) {
                 tmem_load_32(o_at + c, o[0]);
                 tmem_load_32(o_at + c + 32, o[1]);
                 tmem_wait_load(o[0]);
                 tmem_wait_load(o[1]);
             }
-            if (!real || *abort_flag != 0) continue;
+            if (!real || gave_up) continue;
             // (8 dims)
 #pragma unroll
             for (int j = 0; j < 64; j += 8) {
