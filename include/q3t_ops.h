@@ -437,7 +437,8 @@ QWEN3_TTS_API int32_t q3t_launch_kv8_append(const Q3tKv8Cache* cache, const uint
  * Scores, statistics and sums are fp32; query and weights enter the products as fp16 with 11 bits kept, scaled by powers of two so
  * that neither size matters; the scales of a row's value pages may lie 2^80 apart, and values below 2^-71 lose bits.  Bounds that the host gives (tokens, max_row_tokens, max_sequence_length) cut what the device finds
  * larger: a row is then computed over its first max_sequence_length tokens and counted by q3t_attention_range_error_count. A page id
- * outside 0..pages - 1 is left out of the attention, as if masked, and counted by q3t_kv8_page_error_count. */
+ * outside 0..pages - 1 is left out of the attention, as if masked, and counted by q3t_kv8_page_error_count.  New tokens whose block of a
+ * prompt gave up a bounded wait (q3t_kernel_error_count) keep the output that they had. */
 typedef struct Q3tKv8AttentionDesc {
     uint32_t struct_size;        /* sizeof(Q3tKv8AttentionDesc) */
     int32_t rows;                /* 1..Q3T_MAX_TABLE_ROWS */
@@ -553,12 +554,14 @@ QWEN3_TTS_API int32_t q3t_test_set_chain_numbers(Qwen3TtsModelHandle model, uint
  * all as measured); only the time of a frame depends on them, and no frame may be in flight.  sort_chain_places: what a load makes of the cycles that each of 256 SMs
  * needs for 8 pages (0: no such SM) and one SM, by[page], for each of 2304 pages; the groups that are die 0's, or 8, and
  * nothing written, where the dies cannot be told apart; on the host alone.  hold_sms: a kernel on `stream` that takes `ctas` SMs for `ns`
- * nanoseconds, 10^9 at most. */
+ * nanoseconds, 10^9 at most.  kv8_lose_block: the block of the launches to come of q3t_launch_kv8_attention's kernel for prompts that ends as
+ * if one of its waits had run out; -1: none. */
 QWEN3_TTS_API int32_t q3t_test_set_chain_places(Qwen3TtsModelHandle model, const uint8_t* die_of_sm, const uint32_t* pages,
                                                 int32_t grid);
 QWEN3_TTS_API int32_t q3t_test_sort_chain_places(const uint32_t* of_sm, const uint32_t* of_page, const uint32_t* by, int32_t sms,
                                                  uint8_t* die_of_sm, uint32_t* pages);
 QWEN3_TTS_API int32_t q3t_test_hold_sms(int32_t ctas, uint64_t ns, void* stream);
+QWEN3_TTS_API void q3t_test_kv8_lose_block(int32_t block);
 
 /* Number of this library's kernels launched so far through frame graphs of the model. */
 QWEN3_TTS_API int32_t q3t_model_kernel_launches(Qwen3TtsModelHandle model, uint64_t* launches,

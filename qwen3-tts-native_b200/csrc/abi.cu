@@ -1158,6 +1158,7 @@ int32_t q3t_test_sort_chain_places(const uint32_t* of_sm, const uint32_t* of_pag
     }
     return groups;
 }
+void q3t_test_kv8_lose_block(int32_t block) { lose_kv8_block(block); }
 int32_t q3t_test_hold_sms(int32_t ctas, uint64_t ns, void* stream) { return static_cast<int32_t>(launch_hold_sms(ctas, ns, S(stream))); }
 
 uint32_t q3t_kernel_error_count(void) {

@@ -41,6 +41,7 @@ constexpr int kPartTokens = 1024;                       // what a row sees is cu
 constexpr float kMostWeight = 32768.0f;                 // of a page's weights together
 constexpr long long kBudgetCycles = 4000000000ll;        // about two seconds
 
+std::atomic<int> g_lost_block{-1};
 __device__ unsigned int g_kv8_prompt_errors = 0;
 __device__ unsigned int g_kv8_prompt_page_errors = 0;
 __device__ unsigned int g_kv8_prompt_range_errors = 0;
@@ -151,9 +152,11 @@ __device__ __forceinline__ void tmem_store_16(uint32_t taddr, const uint32_t (&r
         : "memory");
 }
 
-// PARTS: items may come in parts (without: two divisions and a branch an item fewer, 1.3 us of a prompt of 1,500 tokens)
+// PARTS: items may come in parts (without: two divisions and a branch an item fewer, 1.3 us of a prompt of 1,500 tokens).  lost_block: the one that
+// ends as if a wait of its had run out, -1: none
 template <int HD, bool E4M3, bool PARTS>
-__global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8AttentionArgs a, const int block_columns, const int parts_asked, unsigned char* const left) {
+__global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8AttentionArgs a, const int block_columns, const int parts_asked, unsigned char* const left,
+                                                                       const int lost_block) {
     const int most_parts = PARTS ? parts_asked : 1;
     using Smem = PromptSmem<HD>;
     extern __shared__ unsigned char smem_raw[];
@@ -592,10 +595,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const float inverse = parts > 1 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
         float* const part_at = reinterpret_cast<float*>(left + kJointBytes) + (size_t)blockIdx.x * Part<HD>::kFloats;
-        if (parts > 1 && real) *reinterpret_cast<float2*>(part_at + 2 * kTileRows * HD + 2 * r) = make_float2(top, total);
         int head;
         const size_t token = item.span.first + place_of(min(r, columns - 1), head), at = (size_t)(item.kv_head * group + head) * HD;
-        const bool gave_up = __any_sync(0xffffffffu, *abort_flag != 0);
+        // Rows whose block gave up are left as they were: the mark of a part's, which no row has as its reference, is NaN
+        const bool gave_up = __any_sync(0xffffffffu, *abort_flag != 0) || (int)blockIdx.x == lost_block;
+        if (parts > 1 && real) *reinterpret_cast<float2*>(part_at + 2 * kTileRows * HD + 2 * r) = make_float2(gave_up ? NAN : top, total);
 #pragma unroll 1
         for (int c = 0; c < HD; c += 64) {
             uint32_t o[2][32];
@@ -634,7 +638,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
     }
     __syncwarp();
     __syncthreads();
-    if (*abort_flag != 0) {
+    if (*abort_flag != 0 || (int)blockIdx.x == lost_block) {
         if (tid == 0) {
             atomicAdd(&g_kv8_prompt_errors, 1u);
             const unsigned long long until = tc::now_ns() + 200000ull;       // products that are still under way
@@ -650,7 +654,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
     pdl_trigger();
 }
 
-// An item's parts, one after the other: a CTA 32 of its rows, a warp 8 dims of them at a time
+// An item's parts, one after the other: a CTA 32 of its rows, a warp 8 dims of them at a time.  Rows of which a part is missing are left as they were
 template <int HD>
 __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8AttentionArgs a, const int most_parts, const unsigned char* const left) {
     pdl_wait();
@@ -663,12 +667,16 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8AttentionArgs a,
     const size_t token = joint.first + i, at = (size_t)(joint.kv_head * group + joint.column0 + r - i * group) * HD;
     for (int d = (int)threadIdx.x / kWarp * 8; d < HD; d += 64) {
         Merged v;
+        bool missing = false;
 #pragma unroll 4
         for (int n = 0; n < joint.parts; ++n) {
             const float* const part = from + n * Part<HD>::kFloats;
             const float4* const o = reinterpret_cast<const float4*>(part) + d / 4 * (2 * kTileRows) + r;
-            v.add(*reinterpret_cast<const float2*>(part + 2 * kTileRows * HD + 2 * r), o[0], o[2 * kTileRows]);
+            const float2 stats = *reinterpret_cast<const float2*>(part + 2 * kTileRows * HD + 2 * r);
+            missing |= stats.x != stats.x;
+            v.add(stats, o[0], o[2 * kTileRows]);
         }
+        if (missing) return;
         const float inverse = v.total == 0.0f ? 0.0f : 1.0f / v.total;
         __nv_bfloat162 x[4];
 #pragma unroll
@@ -721,7 +729,8 @@ cudaError_t launch_cut(const Kv8AttentionArgs& a, const PromptCut& cut, unsigned
     const cudaError_t e = kv8_allow_smem(allowed, kv8_prompt_kernel<HD, E4M3, PARTS>, (int)PromptSmem<HD>::kBytes);
     if (e != cudaSuccess) return e;
     const unsigned grid = (unsigned)(cut.items > 0 ? cut.items * cut.parts : 1);
-    return launch_pdl(kv8_prompt_kernel<HD, E4M3, PARTS>, dim3(grid), dim3(kPromptThreads), PromptSmem<HD>::kBytes, stream, a, cut.block_columns, cut.parts, left);
+    return launch_pdl(kv8_prompt_kernel<HD, E4M3, PARTS>, dim3(grid), dim3(kPromptThreads), PromptSmem<HD>::kBytes, stream, a, cut.block_columns, cut.parts, left,
+                      g_lost_block.load(std::memory_order_relaxed));
 }
 
 template <int HD, bool E4M3>
@@ -744,6 +753,8 @@ cudaError_t launch_kv8_prompts(const Kv8AttentionArgs& a, int head_dim, bool e4m
     if (head_dim == 128) return e4m3 ? launch_prompts<128, true>(a, stream) : launch_prompts<128, false>(a, stream);
     return e4m3 ? launch_prompts<64, true>(a, stream) : launch_prompts<64, false>(a, stream);
 }
+
+void lose_kv8_block(int block) { g_lost_block.store(block, std::memory_order_relaxed); }
 
 unsigned int kv8_prompt_error_count() {
     unsigned int v = 0;

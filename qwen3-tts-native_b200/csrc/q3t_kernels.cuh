@@ -217,7 +217,8 @@ cudaError_t launch_attention_reference_order(const AttentionArgs& args, cudaStre
 // rows seen so far whose position lay outside what the launch was sized for (clamped and counted)
 unsigned int attention_range_error_count();
 unsigned int kv8_range_error_count();          // the same over an 8-bit cache (kv8_attention.cu)
-unsigned int kv8_prompt_error_count();         // waits of kv8_prompt.cu that ran out
+unsigned int kv8_prompt_error_count();         // blocks of kv8_prompt.cu that gave up a wait
+void lose_kv8_block(int block);                // of its next launches: the block that ends as if it had (tests), -1: none
 // Several kernels' counts as one: ~0u, which says that it cannot be read, where that is so of any of them; else their sum, which stops short of it
 inline unsigned int sum_of_counts(std::initializer_list<unsigned int> counts) {
     unsigned int sum = 0;

@@ -1,6 +1,8 @@
 """Calls of the 8-bit KV cache's operators beside those of test_gpu_kv8_attention.py."""
 import importlib.util
 import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -39,3 +41,48 @@ def test_a_measured_case_goes_to_the_stream_that_is_current():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(state["output"], want)
+
+
+# a block that is lost, in a process of its own: others look for an error count of zero
+LOST = """
+import sys
+sys.path[:0] = [{tests!r}, {root!r}]
+import importlib
+import numpy as np
+import kv8_oracle as plain
+q3t = importlib.import_module("qwen3-tts-native_b200")
+ops = importlib.import_module("qwen3-tts-native_b200.ops")
+lib = q3t.library()
+rng = np.random.default_rng(3)
+heads, group, dim = {heads}, 2, 64
+lengths, new = {lengths}, {new}
+starts = np.concatenate([[0], np.cumsum(new)])
+planes = plain.cache(rng, 900, heads, dim, False)
+table = plain.tables_of(rng, lengths, 900, {room})
+q = plain.to_bf16(rng.standard_normal((sum(new), heads * group * dim)).astype(np.float32))
+call = lambda: ops.kv8_attention(q, *planes, table, lengths, starts, fill=0x1234)[0].reshape(len(q), heads, group * dim)
+want = call()
+assert lib.q3t_kernel_error_count() == 0
+lib.q3t_test_kv8_lose_block({block})
+got = call()
+assert lib.q3t_kernel_error_count() == 1
+lib.q3t_test_kv8_lose_block(-1)
+lost = np.zeros(got.shape[:2], dtype=bool)
+lost[{tokens}, {head}] = True
+assert (got[lost] == 0x1234).all(), "rows of the lost block were written"
+assert np.array_equal(got[~lost], want[~lost])
+assert np.array_equal(call(), want) and lib.q3t_kernel_error_count() == 1
+"""
+
+
+@pytest.mark.parametrize("heads,lengths,new,room,block,tokens,head", [
+    # one part an item: blocks of 128 columns (64 tokens), the last tokens' and first head's first
+    (16, [300, 40], [300, 40], None, 1, slice(256, 300), 1), (16, [300, 40], [300, 40], None, 16 * 5, slice(300, 340), 0),
+    # eight parts an item, of which one of the first head's second block (tokens 128 .. 199) or one of the second row's is lost
+    (2, [5000, 4100], [200, 60], LONG, 5, slice(128, 200), 0), (2, [5000, 4100], [200, 60], LONG, 8 * 4 + 8, slice(200, 260), 1)])
+def test_what_a_block_that_gave_up_does_not_write(heads, lengths, new, room, block, tokens, head):
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = LOST.format(tests=here, root=os.path.dirname(here), heads=heads, lengths=lengths, new=new, room=room, block=block,
+                       tokens="slice(%d, %d)" % (tokens.start, tokens.stop), head=head)
+    ran = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert ran.returncode == 0, ran.stderr[-2000:]
