@@ -46,13 +46,17 @@ constexpr int kClusterCtas = 8;                        // the most of a segment
 // 8,192 11.4 / 12.7, of 16,384 18.6 / 14.9; 8 rows of 4,096 15.6 / 18.5; 16 of 2,048 15.3 / 18.7, of 4,096 27.4 / 29.7; 32 of 1,024 15.2 / 20.2, of 2,048
 // 28.7 / 30.7.  (Rows of one length, which suits the clusters: others leave some idle where ranges are even.  Hence the bound on the near side.)
 // Short rows also in two rounds: 64 rows of 64 8.1 / 11.1, of 256 12.3 / 14.7, of 512 17.7 / 19.8, of 1 to 512 13.7 / 15.2, of 1,024 31.5 / 30.7.
-constexpr int kFewCtas = 256, kFewTokens = 1024, kFewest = 64;
+// One row has so many segments where it is a prompt, which kv8_prompt.cu takes in one launch: as soon where some SM here has a fourth CTA.  Clusters /
+// prompts, 16 query heads on 8 of 128, from nothing: 136 tokens (272 CTAs) 6.3 / 9.9, 160 9.8 / 9.8, 216 (432) 10.6 / 10.5, 232 (464) 12.3 / 10.5, 256
+// (512) 12.7 / 10.8; over 512: 136 9.5 / 14.4, 216 14.8 / 14.4, 232 17.3 / 14.4, 256 17.5 / 14.2.  (Heads of 64, 256 tokens: 9.7 / 8.9 and 12.7 / 11.7.)  Two
+// rows of 128 tokens (512 CTAs), behind the launches for rows that are none: 8.8 / 11.4.
+constexpr int kFewCtas = 256, kOnePromptCtas = 3 * 148, kFewTokens = 1024, kFewest = 64;
 // Rows of more columns than this are kv8_prompt.cu's, which takes 64 tokens for 128 columns in the time it takes them for one.  64 rows over 2,048
 // tokens, here / there in us: 32 columns 127 / 132, 48 167 / 132; 16 rows: 32 36 / 37, 48 45 / 37.
 constexpr int kRowColumns = 32;
 // But too few of them leave SMs idle there: they stay here while (query heads x new tokens x tokens seen) is below 2^23, unless even the longest
-// context takes no time there.  One row, 8 KV heads, here / there: over 16,384 48 columns 34 / 40, 64 (2^23) 40 / 40, 256 111 / 51; over
-// 2,048 256 columns 27 / 31, 512 (2^23) 39 / 31; over 1,024 512 columns 27 / 21; over 256 512 columns 17 / 11.  A row alone that goes there is the only
+// context takes no time there.  One row, 8 KV heads, the ranges / there: over 16,384 48 columns 34 / 40, 64 (2^23) 40 / 40, 256 111 / 51; over
+// 2,048 256 columns 27 / 30, 512 (2^23) 39 / 31; over 1,024 512 columns 27 / 21; over 256 512 columns 16 / 11.  A row alone that goes there is the only
 // one, so that nothing is launched here (a prompt of 1,500 tokens 27.5 us, with two launches for rows that are not there 29.2).
 constexpr long long kPromptWork = 1 << 23;
 constexpr int kShort = 1024;
@@ -758,7 +762,7 @@ Plan plan_of(Kv8AttentionArgs& a, int head_dim) {
     a.prompts = 0;
     a.row_columns = INT_MAX;
     a.scratch_taken = kCounterBytes + kRowCtas * 2 * 2 * kTileColumns * (head_dim + 4) * (int)sizeof(float);
-    if ((segments * cluster <= kFewCtas && a.max_sequence <= kFewTokens * cluster) || (segments <= 2 * kFewCtas && a.max_sequence <= kFewTokens / 2)) {
+    if ((segments * cluster <= kFewCtas && a.max_sequence <= kFewTokens * cluster) || (segments <= (a.rows == 1 ? kOnePromptCtas : 2 * kFewCtas) && a.max_sequence <= kFewTokens / 2)) {
         return Plan{cluster, (int)blocks, 0};
     }
     if (columns > kRowColumns && ((long long)a.tokens * a.query_heads * a.max_sequence >= kPromptWork || a.max_sequence <= kShort)) {

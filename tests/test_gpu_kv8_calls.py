@@ -7,7 +7,8 @@ import sys
 import numpy as np
 import pytest
 
-from test_gpu_kv8_attention import LONG, _run
+import kv8_oracle as plain
+from test_gpu_kv8_attention import LONG, _compare, _query, _run
 
 pytestmark = pytest.mark.gpu
 
@@ -19,6 +20,20 @@ def test_warps_whose_last_columns_are_not_there(ops, dim, heads, group, new, roo
     """Prompts, in one part and in several, whose columns end anywhere in a warp of 32: what it loads together it stores in part."""
     lengths = [n + 100 * i for i, n in enumerate(new)]
     _run(ops, np.random.default_rng(sum(new) + dim), heads, dim, group, lengths, new, dim == 64, room=room)
+
+
+@pytest.mark.parametrize("heads,group,dim,new,length", [(8, 2, 128, 256, 256), (8, 2, 64, 256, 500), (8, 1, 128, 512, 512), (1, 64, 64, 64, 64)])
+def test_a_prompt_of_512_blocks_of_columns_is_a_prompt_however_short(ops, heads, group, dim, new, length):
+    """With a bound of 1,024 tokens kv8_prompt.cu has it; the sums of the kernel of few new tokens run in another order, so equal bits say that
+    a tight bound does not send it there, where it takes a fifth longer."""
+    rng = np.random.default_rng(length + new)
+    planes = plain.cache(rng, 40, heads, dim, False)
+    table = plain.tables_of(rng, [length], 40, 64)
+    q = _query(rng, new, heads * group, dim)
+    tight, loose = (ops.kv8_attention(q, *planes, table, [length], [0, new], max_seq=bound, want_f32=True) for bound in (length, 1024))
+    want, tol = plain.attention(q, planes, table, [length], [0, new], False)
+    _compare(*tight, want, tol)
+    assert np.array_equal(tight[0], loose[0]) and np.array_equal(tight[1], loose[1])
 
 
 def test_a_measured_case_goes_to_the_stream_that_is_current():
