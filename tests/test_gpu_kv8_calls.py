@@ -101,3 +101,28 @@ def test_what_a_block_that_gave_up_does_not_write(heads, lengths, new, room, blo
                        tokens="slice(%d, %d)" % (tokens.start, tokens.stop), head=head)
     ran = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert ran.returncode == 0, ran.stderr[-2000:]
+
+
+@pytest.mark.parametrize("heads,group,lengths,new,room", [
+    (2, 2, [100, 250, 31], None, None), (2, 2, [3000, 250, 31], None, None), (2, 2, [100, 250, 31], None, 520), (8, 2, [2000, 900, 700] + [300] * 60, None, None),
+    (2, 2, [300, 260, 31], [40, 90, 1], None), (16, 2, [300, 260, 31], [140, 90, 1], None), (16, 2, [500], [300], None),
+    (2, 2, [5000, 4100, 60], [200, 60, 1], LONG), (2, 2, [9000], [300], None), (4, 2, [3000, 2100], [30, 9], None)])
+def test_a_bad_page_is_counted_once(ops, q3t, heads, group, lengths, new, room):
+    """However many heads, blocks of columns, warps and parts come by it."""
+    rng = np.random.default_rng(sum(lengths))
+    pages = sum(-(-n // 16) for n in lengths) + 3
+    planes = plain.cache(rng, pages, heads, 64, False)
+    table = plain.tables_of(rng, lengths, pages, room)
+    bad = 0
+    for r, n in enumerate(lengths[:3]):
+        for page in {0, 2, -(-n // 16) // 2, -(-n // 16) - 1}:
+            if page < -(-n // 16):
+                table[r, page] = rng.choice([-1, pages, 2 ** 31 - 1, -2 ** 31])
+                bad += 1
+    starts = None if new is None else np.concatenate([[0], np.cumsum(new)])
+    q = _query(rng, len(lengths) if new is None else sum(new), heads * group, 64)
+    before, waits = q3t.library().q3t_kv8_page_error_count(), q3t.library().q3t_kernel_error_count()
+    out, f32 = ops.kv8_attention(q, *planes, table, lengths, starts, want_f32=True)
+    assert q3t.library().q3t_kv8_page_error_count() == before + bad and q3t.library().q3t_kernel_error_count() == waits
+    want, tol = plain.attention(q, planes, table, lengths, starts, False)
+    _compare(out, f32, want, tol)
