@@ -396,12 +396,20 @@ def sample(logits, rng_state: int, *, suppress=False, history: Optional[Sequence
     return int(dt.item()), int(dr.cpu().numpy().view(np.uint64)[0])
 
 
+def _is_shaped(**arrays):
+    """name=(array, shape): a launch reads as far as the other arguments say, so one of another shape never gets to it."""
+    for name, (a, shape) in arrays.items():
+        if np.shape(a) != shape:
+            raise ValueError(f"{name} is {np.shape(a)} where the other arguments make it {shape}")
+
+
 def page_tables(lengths, changes, page_table, free_pages, free_count, *, token_capacity=None, fill=-7, want_slots=True):
     """Block tables and slot maps of a batch.  Returns dict(page_table, free_pages, free_count, lengths, status, starts,
     positions, slots): copies of what the launch leaves; positions and slots of `token_capacity` entries, `fill` where nothing was written."""
     lengths = np.asarray(lengths, dtype=np.int32)
     rows = lengths.size
     free_pages = np.asarray(free_pages, dtype=np.int32)
+    _is_shaped(lengths=(lengths, (rows,)), changes=(changes, (rows,)), page_table=(page_table, (rows, np.shape(page_table)[-1])), free_pages=(free_pages, (free_pages.size,)))
     capacity = int(np.clip(np.asarray(changes, dtype=np.int64), 0, None).sum()) if token_capacity is None else token_capacity
     held = {"lengths": _dev(lengths), "changes": _dev(np.asarray(changes, dtype=np.int32)),
             "page_table": _dev(np.asarray(page_table, dtype=np.int32)), "free_pages": _dev(free_pages),
@@ -449,6 +457,8 @@ def _planes(key, value, key_scales, value_scales, e4m3):
 def kv8_append(key, value, key_scales, value_scales, k_new, v_new, slots, *, e4m3=False, count=None):
     """Quantises bf16 rows k_new, v_new [tokens][heads * dim] into planes of codes [pages][heads][16][dim] (uint8 bit patterns) with scales
     [pages][heads]; `count`: read on the device in place of the rows' number.  Returns the four arrays afterwards."""
+    width = np.shape(key)[1] * np.shape(key)[3]
+    _is_shaped(slots=(slots, (len(slots),)), k_new=(k_new, (len(slots), width)), v_new=(v_new, (len(slots), width)))
     planes = _planes(key, value, key_scales, value_scales, e4m3)
     c = kv8_cache(*planes)
     dk, dv = _dev(np.asarray(k_new, dtype=np.uint16)), _dev(np.asarray(v_new, dtype=np.uint16))
@@ -464,12 +474,14 @@ def kv8_attention(q, key, value, key_scales, value_scales, page_table, lengths, 
     """Attention of the new tokens q [tokens][query heads * dim] (bf16) over an 8-bit cache.  Returns (out, f32 or None); rows of `out`
     that no token fills keep the bits `fill`."""
     lib = native.library()
-    planes = _planes(key, value, key_scales, value_scales, e4m3)
-    c = kv8_cache(*planes)
     q = np.ascontiguousarray(q, dtype=np.uint16)
     lengths = np.asarray(lengths, dtype=np.int32)
     page_table = np.asarray(page_table, dtype=np.int32)
     dim = key.shape[3]
+    _is_shaped(q=(q, (len(q), q.shape[-1] // dim * dim)), lengths=(lengths, (lengths.size,)), page_table=(page_table, (lengths.size, page_table.shape[-1])),
+               starts=(lengths.size * [0] if starts is None else starts[1:], (lengths.size,)))
+    planes = _planes(key, value, key_scales, value_scales, e4m3)
+    c = kv8_cache(*planes)
     held = {"query": _dev(q), "page_table": _dev(page_table), "lengths": _dev(lengths),
             "output": _dev(np.full(q.shape, fill, dtype=np.uint16))}
     if starts is not None:
