@@ -421,7 +421,9 @@ typedef struct Q3tKv8Cache {
  *   code  = round(x * (1 / scale)), to nearest even, every operation in fp32.
  * A page is filled from its first slot on: tokens in slots below the new ones are held.  With such, the scale is the larger of that
  * and the page's own, and where it has grown the held codes become round(code * (own scale * (1 / scale))); nothing else of the
- * page changes.  The same tokens appended again change nothing, and slots may be filled anew from any point on.
+ * page changes.  A page's last tokens appended again change nothing, and slots may be filled anew from any point on: those above the new
+ * tokens then hold nothing, since the scale is no longer theirs.  A page's scale does not shrink before its first slot is filled
+ * anew: tokens that are given back (a refused draft) leave theirs, and what the page holds stays rounded to it.
  * Tokens of one page stand next to each other; where they name a slot twice the last one is kept.  (Tokens of a page that
  * stand apart leave some of its values and its scale unspecified.)  A value that is not finite is stored as the largest finite
  * bf16 of its sign and its page, head and plane counted (process-wide per device) by q3t_kv8_nonfinite_count; a slot past the
@@ -435,7 +437,10 @@ QWEN3_TTS_API int32_t q3t_launch_kv8_append(const Q3tKv8Cache* cache, const uint
  * the positions up to its own.  Query head h reads key/value head h / (query_heads / key_value_heads).  A token without a
  * position (a row shorter than its new tokens) gets zeros; output behind the last token is left as it was.
  * Scores, statistics and sums are fp32; query and weights enter the products as fp16 with 11 bits kept, scaled by powers of two so
- * that neither size matters; the scales of a row's value pages may lie 2^80 apart, and values below 2^-71 lose bits.  Bounds that the host gives (tokens, max_row_tokens, max_sequence_length) cut what the device finds
+ * that neither size matters (output_f32 has no more bits than that either); the scales of a row's value pages may lie 2^80 apart, and values
+ * below 2^-71 lose bits.  The same call gives the same bits; but the bounds choose the kernel, and where many rows share the GPU the lengths
+ * of all of them say where a row's sum is cut, so that its last bits may change with the rows beside it (over bf16 pages they do not).
+ * Bounds that the host gives (tokens, max_row_tokens, max_sequence_length) cut what the device finds
  * larger: a row is then computed over its first max_sequence_length tokens and counted by q3t_attention_range_error_count. A page id
  * outside 0..pages - 1 is left out of the attention, as if masked, and counted by q3t_kv8_page_error_count.  New tokens whose block of a
  * prompt gave up a bounded wait (q3t_kernel_error_count) keep the output that they had. */

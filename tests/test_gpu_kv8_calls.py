@@ -126,3 +126,21 @@ def test_a_bad_page_is_counted_once(ops, q3t, heads, group, lengths, new, room):
     assert q3t.library().q3t_kv8_page_error_count() == before + bad and q3t.library().q3t_kernel_error_count() == waits
     want, tol = plain.attention(q, planes, table, lengths, starts, False)
     _compare(out, f32, want, tol)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_a_refused_draft_leaves_its_scale_until_the_page_begins_anew(ops, e4m3):
+    rng = np.random.default_rng(17)
+    planes = plain.cache(rng, 2, 1, 64, e4m3)
+    tokens = lambda count, size: plain.to_bf16((rng.standard_normal((count, 64)) * size).astype(np.float32))  # noqa: E731
+    first, large, small = tokens(6, 1.0), tokens(3, 50.0), tokens(3, 1.0)
+    slots = lambda a, b: np.arange(16 + a, 16 + b, dtype=np.int64)  # noqa: E731
+    held = ops.kv8_append(*planes, first, first, slots(0, 6), e4m3=e4m3)
+    drafted = ops.kv8_append(*held, large, large, slots(6, 9), e4m3=e4m3)
+    taken = ops.kv8_append(*drafted, small, small, slots(6, 9), e4m3=e4m3)            # the draft's slots, filled anew
+    for i in range(2):
+        assert drafted[i + 2][1, 0] > 5 * held[i + 2][1, 0] and taken[i + 2][1, 0] == drafted[i + 2][1, 0]
+        assert np.array_equal(taken[i][1, :, :6], drafted[i][1, :, :6])
+    again = ops.kv8_append(*taken, first, first, slots(0, 6), e4m3=e4m3)              # from the first slot on
+    for i in range(2):
+        assert again[i + 2][1, 0] == held[i + 2][1, 0] and np.array_equal(again[i][1, :, :6], held[i][1, :, :6])
