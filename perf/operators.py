@@ -343,22 +343,22 @@ def _own_cache(ops, s):
     return ops.kv8_cache(s["key"], s["value"], s["key_scales"], s["value_scales"])
 
 
-def _own_call(s):
-    """What a host keeps of a call: the function and its arguments but for the stream, addresses and sizes alone."""
+def _own_call(s, stream):
+    """What a host keeps of a call on one of its streams: the function and its arguments, addresses and sizes alone."""
     package = importlib.import_module("qwen3-tts-native_b200")
     ops = importlib.import_module("qwen3-tts-native_b200.ops")
-    lib, case = package.library(), s["case"]
+    lib, case, stream = package.library(), s["case"], C.c_void_p(stream)
     if case["kind"] == "tables":
         d = ops.PageTablesDescC(rows=case["rows"], page_table_stride=case["stride"], pages=s["pages"], token_capacity=s["capacity"])
         d.struct_size = C.sizeof(d)
         for name in ("lengths", "changes", "new_lengths", "page_table", "free_pages", "free_count", "new_free_count", "status",
                      "token_starts", "positions", "slots"):
             setattr(d, name, _pointer(s[name]))
-        return lib.q3t_launch_page_tables, (C.byref(d),), [d]
+        return lib.q3t_launch_page_tables, (C.byref(d), stream), [d]
     cache = _own_cache(ops, s)
     if case["kind"] == "append":
         args = (C.byref(cache), C.c_void_p(_pointer(s["keys"])), C.c_void_p(_pointer(s["values"])), C.c_void_p(_pointer(s["slots"])), None,
-                s["tokens"], s["keys"].stride(0), s["values"].stride(0))
+                s["tokens"], s["keys"].stride(0), s["values"].stride(0), stream)
         return lib.q3t_launch_kv8_append, args, [cache]
     d = ops.Kv8AttentionDescC(rows=case["rows"], query_heads=case["query_heads"], page_table_stride=s["page_table"].shape[1], tokens=s["tokens"],
                               max_row_tokens=s["most"], max_sequence_length=s["longest"])
@@ -369,16 +369,18 @@ def _own_call(s):
     size = int(lib.q3t_kv8_attention_scratch_bytes(C.byref(d)))
     scratch = torch.empty(max(size, 16), dtype=torch.uint8, device="cuda")
     d.scratch, d.scratch_bytes = _pointer(scratch), size
-    return lib.q3t_launch_kv8_attention, (C.byref(d),), [d, cache, scratch]
+    return lib.q3t_launch_kv8_attention, (C.byref(d), stream), [d, cache, scratch]
 
 
 def _own(s):
-    stream = torch.cuda.current_stream().cuda_stream
     calls = s.setdefault("call", {})                                                          # one a stream: calls that share scratch have to be ordered
+    if not calls:
+        s["device"] = torch.cuda.current_device()
+    stream = torch._C._cuda_getCurrentRawStream(s["device"])                                  # the handle alone: a stream object takes microseconds
     if stream not in calls:
-        calls[stream] = _own_call(s)
+        calls[stream] = _own_call(s, stream)
     function, arguments, _ = calls[stream]
-    status = function(*arguments, C.c_void_p(stream))
+    status = function(*arguments)
     if status != 0:
         raise RuntimeError("launch returned %d" % status)
     kind = s["case"]["kind"]
