@@ -14,9 +14,9 @@
 //   a prompt of 512 tokens 4.5 / 4.1 / 4.5, of 1,024 6.2 / 4.6 / 4.5, of 2,048 9.2 / 5.7 / 4.8, of 4,096 15.4 / 8.4 / 5.8, of 8,192 27.8 / 13.7 / 8.8;
 //   512 rows of one token 8.0 / 8.7 / 21, 1,024 14.1 / 14.0 / 21, 2,048 26.0 / 23.0 / 28, 4,096 51.8 / 43.9 / 50.3.
 //
-// What bounds it: a decode step the latency of five loads and sums one behind the other (64 rows: 3.0 us); a large batch memory (65,536
-// tokens in rows of 1 to 8,192, 302 MB: 54.5 us, 5.5 TB/s;
-// three CTAs an SM instead of four, with more registers: 60.9 us).  A prompt of 1,500 tokens takes 4.8 us (4 an SM: 5.1).
+// What bounds it: a decode step the latency of five loads and sums one behind the other (64 rows: 3.0 us); a large batch memory (49,174
+// tokens in 43 rows, 303 MB: 54.5 us, 5.6 TB/s, on inputs that change from call to call 58; three CTAs an SM instead of four, with more
+// registers, take 12 % longer).  A prompt of 1,500 tokens takes 4.8 us (4 an SM: 5.1).
 
 #include "kv8.cuh"
 #include "q3t_kernels.cuh"

@@ -17,9 +17,10 @@
 // the CTA leaves (reference, sum, output) and the one with the last ticket folds them in order, so a result depends on
 // the batch's lengths, not on timing.
 //
-// What bounds it: one row, latencies one behind the other (3,000 tokens, 8 heads of 128: 7.0 us); a full batch memory (64 rows of 64 to 2,048 tokens,
-// 140 MB: 31 us, of which 21 are memory's; 7 rows of 90,000 to 131,072, 4 heads, 804 MB: 130 us, 6.2 TB/s); rows of several tokens the conversions
-// and products of 4 warps a scheduler that each wait for their next page (23 drafts of five, heads of 64, 48 MB: 23 us).
+// What bounds it: one row, latencies one behind the other (3,000 tokens, 8 heads of 128: 7.1 us); a full batch memory (64 rows of 64 to 2,048 tokens,
+// 140 MB: 31 us, of which 21 are memory's; 7 rows of 90,000 to 131,072, 4 heads, 804 MB: 133 us, 6.0 TB/s); rows of several tokens the conversions
+// and products of 4 warps a scheduler that each wait for their next page (23 drafts of five, heads of 64, 48 MB: 23 us).  (Times here and below are
+// those of the same call 20 times in a graph; on inputs that change from call to call these four take 8.2, 33, 143 and 24 us.)
 
 #include "kv8.cuh"
 #include "q3t_kernels.cuh"

@@ -11,13 +11,16 @@
 // While a tile's half is in the softmax the products of its other half and of the other tile run.  A row's reference follows its scores
 // only when its weights outgrow fp16, so that the output in tensor memory is rescaled almost never.
 //
-// Where the blocks of 256 columns are fewer than the SMs they become blocks of 128, and where each could have several SMs to itself and sees 2,048 tokens
-// and more, its steps are cut into parts, which kv8_join_kernel merges.
+// Where the blocks of 256 columns are fewer than the SMs they become blocks of 128, and where each could have several SMs to itself and rows may see
+// 2,048 tokens and more, their steps are cut into parts, which kv8_join_kernel merges.
 //
-// What bounds it: of a half's 2,000 cycles (1,550 with one tile) the products take 1,024 and the exponentials as much, on units that
-// run side by side; the rest is the way of a tile's half through barriers, tensor memory and registers, of which two tiles hide one in the other
+// What bounds it: of a half's 2,000 cycles (1,550 with one tile, heads of 128) the tensor cores take 1,024 and the exponentials as much, on units that
+// run side by side.  Shared memory is a third: at 128 bytes a cycle a score product of 64 tokens has its operands, 6 KB, in 48 cycles and is
+// done in 32, which makes the products 1,280, and the copies' stores are 256 more (arithmetic, not measured apart).  The rest is
+// the way of a tile's half through barriers, tensor memory and registers, of which two tiles hide one in the other
 // what two can.  A block costs 7 us more before and after its steps.  A chunk of 4,096 tokens over 16,384 (16 query heads, 8 KV heads of 128): 472 us,
-// 1,018 TFLOP/s; 11 prompts of 667 to 1,333 over 1,400 to 3,333 (32, 8): 408 us; a prompt of 1,500: 27.5 us; 256 tokens over 16,384: 53 us.
+// 1,018 TFLOP/s (call after call for long enough that the power limit shows: 517 us, 930); 11 prompts of 667 to 1,333 over 1,400 to 3,333 (32, 8): 415 us;
+// a prompt of 1,500: 27.5 us; 256 tokens over 16,384: 51 us.
 
 #include "kv8.cuh"
 #include "q3t_kernels.cuh"
@@ -37,7 +40,9 @@ constexpr int kLaunchRegisters = 96, kSoftmaxRegisters = 144, kCopyRegisters = 7
 static_assert(2 * kSoftmaxRegisters + 2 * kCopyRegisters + kProductRegisters <= 5 * kLaunchRegisters, "registers of the five warpgroups");
 constexpr int kScaleRing = 4;                           // steps whose scales are kept: K runs two steps ahead of the softmax
 constexpr uint32_t kTmemCols = 512, kOut = 256;         // scores of the tiles at 0 and 128, outputs at 256 and 384
-constexpr int kPartTokens = 1024;                       // what a row sees is cut into parts of so many and more
+// A launch has as many parts as its longest row may have of so many tokens, and a row takes as many of them as it has steps.  (Bound of 16,384, 256
+// tokens, parts of 1, 2, 4 and 8 steps and more in us: over 300 16.8 / 17.8 / 17.7 / 17.7, over 1,024 20.1 / 21.7 / 28.6 / 28.5, over 2,000 23.1 / 25.0 / 26.4 / 45.6.)
+constexpr int kPartTokens = 1024;
 constexpr float kMostWeight = 32768.0f;                 // of a page's weights together
 constexpr long long kBudgetCycles = 4000000000ll;        // about two seconds
 
@@ -692,9 +697,9 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8AttentionArgs a,
     }
 }
 
-// Blocks of 128 columns where 256 would leave SMs idle (one row, 8 KV heads, 128 / 256 in us, behind the short rows' launches: 1,024 tokens 23 / 29, 2,048
-// 42 / 46, 2,200 47 / 48; 3,000, past the rule, 79 / 61), and where those of 256 are so few that each could have several SMs, parts (256 tokens over
-// 16,384: 55 us, without 216; over 2,048 32.7 / 36)
+// Blocks of 128 columns where 256 would leave SMs idle (one row, 16 query heads on 8, 128 / 256 in us: 1,024 tokens 21 / 27, 2,048 40 / 44, 2,200
+// 45 / 46; 3,000, past the rule, 78 / 59), and where those of 256 are so few that each could have several SMs, parts (256 tokens over
+// 16,384: 51 us, without 214; over 4,096 32 / 59; over 2,048 31 / 33)
 PromptCut prompt_cut(const Kv8AttentionArgs& a) {
     // as many items as any split of the tokens over the rows can make
     const long long columns = (long long)a.tokens * (a.query_heads / a.cache.heads);

@@ -9,7 +9,8 @@
 // What bounds it: latency (lengths, sums, table entries: three loads one behind the other) and, with long prompts, the 12 bytes
 // a new token that are written.  A step of a token a row is one CTA's.  Others are filled in by a CTA for each 32 rows or 2,048 tokens, each of
 // which repeats the sums, and a second launch writes lengths, states and the free count, which may lie over what the first one
-// reads; it has its sums by the time the first is done.  One launch / two, in us: a token a row 3.2 / 3.8 (64 rows), 4.3 / 4.7 (512), 6.3 / 5.5
+// reads (where they do not, its first CTA could write them: not done); it has its sums by the time the first is done.  One CTA / two
+// launches, in us: a token a row 3.2 / 3.8 (64 rows), 4.3 / 4.7 (512), 6.3 / 5.5
 // (1,000); every eighth row with a prompt of up to 8 tokens and every sixteenth giving all pages back 7.0 / 6.5 (64), 13.2 / 8.7 (1,000); prompts of
 // up to 1,500 for 113,000 tokens 69.6 / 8.7 (1.4 MB written, 0.3 us of memory).
 
